@@ -44,7 +44,8 @@ enum pgqa_status {
     PGQA_ERR_DEVICE_TIMEOUT = 8,    /* a bounded device-side wait expired (device word) */
     PGQA_ERR_DEVICE_BAD_PAGE = 9,   /* a block-table entry was outside [0, num_pages)   */
     PGQA_ERR_DEVICE_BAD_SEQLEN = 10, /* a seq_len was < 0 or above the table capacity   */
-    PGQA_ERR_SCRATCH_LIMIT = 11     /* shape exceeds pgqa_decode_noalloc's fixed scratch */
+    PGQA_ERR_SCRATCH_LIMIT = 11,    /* shape exceeds pgqa_decode_noalloc's fixed scratch */
+    PGQA_ERR_DEVICE_BAD_POSITION = 12 /* a position was outside the cosine and sine tables */
 };
 
 /*
@@ -236,6 +237,132 @@ int pgqa_decode_noalloc(const void* q, const void* k_cache, const void* v_cache,
  * reference).  Returns PGQA_OK (also when no such call has run on this device) or one
  * of the PGQA_ERR_DEVICE_* codes.  Allocates nothing. */
 int pgqa_noalloc_check_device_error(void* stream);
+
+/*
+ * Operators around the decode (no counterpart in the reference).  They allocate nothing
+ * and keep nothing between calls, may be captured into a CUDA graph after one eager call
+ * on the device, and may run on several streams at once as long as the calls' outputs and
+ * pages differ.  Their device-side errors go to one word per device, which
+ * pgqa_check_device_error(NULL, stream) reads and clears.
+ */
+
+/*
+ * Rotary positions on one or several axes, and the append of the new tokens.
+ *
+ * Pair i < rotary_dim / 2 of every head of q and k_new turns by row p of the tables,
+ *     (x, y) -> (x cos[p][i] - y sin[p][i], y cos[p][i] + x sin[p][i]),
+ * p being positions[pair_axis[i]][token], or the token's place in its sequence (L_b + s)
+ * when positions is NULL.  Pairs are elements (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * interleaved = 1; elements from rotary_dim on are copied.  Arithmetic is fp32, each
+ * result is rounded once.  q goes to q_out; k_new (turned) and v_new are written at
+ * positions [L_b, L_b + S) of each sequence, as pgqa_append_kv does, in bf16 or, into e4m3
+ * pools, as e4m3(value / scale of the KV head), saturating at +-448.
+ *   q, q_out     bf16 [tokens, Hq, 128]; both NULL: nothing to turn but k_new
+ *   k_new, v_new bf16 [tokens, Hkv, 128]; both NULL: nothing to append (the pools and the
+ *                table are then not used; seq_lens only where positions is NULL)
+ *   *_strides    element strides of q, k_new, v_new between sequences, tokens and heads
+ *                (multiples of 8; the 128 elements of a head are contiguous); q_out is
+ *                contiguous
+ *   cu_seqlens   NULL: [batch_size, seqlen] tokens, tokens = batch_size * seqlen.
+ *                Else int32 [batch_size + 1], ascending from 0: tokens of all sequences
+ *                packed, those of sequence b at [cu[b], cu[b + 1]); the sequence stride is
+ *                not used.  Tokens from cu[batch_size] on are left as they are.
+ *   seq_lens     lengths before the append, int32 [batch_size], not modified
+ *   cos, sin     [table_rows, rotary_dim / 2], fp32 (table_format 0) or bf16 (1)
+ *   positions    NULL or int32 [num_axes, tokens]
+ *   pair_axis    axis of each pair (the first rotary_dim / 2 entries are read)
+ *   weights      NULL, or the fp32 weight pool [num_pages, Hkv, P] of
+ *                pgqa_accumulate_weights: the new tokens' entries become 0
+ * rotary_dim is a multiple of 16 up to 128.  A token whose position lies outside the
+ * tables, whose place lies past the table's capacity or whose page id is outside
+ * [0, num_pages) is not written and flagged in the device error word.
+ */
+typedef struct pgqa_rope_args {
+    size_t struct_size;
+    const void* q;
+    const void* k_new;
+    const void* v_new;
+    void* q_out;
+    void* k_cache;
+    void* v_cache;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    const void* cos;
+    const void* sin;
+    const int32_t* positions;
+    const int32_t* cu_seqlens;
+    float* weights;
+    const float* k_scale;
+    const float* v_scale;
+    int64_t batch_size, seqlen, tokens, num_heads, num_heads_k, headdim;
+    int64_t page_size, num_pages, bt_stride;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    int64_t table_rows, rotary_dim, num_axes;
+    int32_t interleaved, kv_format, table_format, reserved;
+    uint8_t pair_axis[64];
+} pgqa_rope_args;
+
+int pgqa_rope_append(const pgqa_rope_args* args, void* stream);
+
+/*
+ * The attention weight that each cached token receives from a decode, added to its entry
+ * of the weight pool: weights[page][kv][slot] += sum over the query rows of KV head kv
+ * that see the token of exp(scale * q.k - softmax_lse[row]).  q, the pool, the table, the
+ * lengths (of the sequences attended over, appended tokens included), causal and scale are
+ * those of the decode; softmax_lse [B, Hq, Sq] fp32 is what it returned.  weights is fp32
+ * [num_pages, Hkv, P].  A row whose log-sum-exp is -inf adds nothing; entries from a
+ * sequence's length on are not touched.  Each entry gets one addition per call, in one
+ * order, unless sequences share a page: then their sums are added in any order.
+ * seqlen_q is at most 4096 and batch_size at most about 28,000 (PGQA_ERR_UNSUPPORTED).
+ */
+typedef struct pgqa_weights_args {
+    size_t struct_size;
+    const void* q;
+    const void* k_cache;
+    const float* softmax_lse;
+    float* weights;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    const float* k_scale;
+    int64_t batch_size, seqlen_q, num_heads, num_heads_k, headdim;
+    int64_t page_size, num_pages, bt_stride, causal;
+    float scale;
+    int32_t kv_format;
+} pgqa_weights_args;
+
+int pgqa_accumulate_weights(const pgqa_weights_args* args, void* stream);
+
+/*
+ * Cuts every sequence of more than `keep` tokens to `keep`, for each KV head on its own:
+ * the first `sinks` tokens, the last `recent`, and between them the keep - sinks - recent
+ * of the highest weight (equal weights: lowest index first; NaN counts as the highest).
+ * The kept tokens' K and V rows move, in their order, to slots [0, keep) of the sequence's
+ * own pages, in place, and their weights likewise in weights_out (NULL: in place in
+ * weights; another pool of the same shape gets the weights of every sequence's first
+ * min(L, keep) slots and is otherwise left as it was).
+ *   kept      int32 [B, Hkv, keep]: the indices kept, ascending; a sequence of L <= keep
+ *             tokens is not changed and gets 0 .. L-1 and then -1
+ *   new_lens  int32 [B]: min(L, keep); not seq_lens itself, which both launches read
+ *             (PGQA_ERR_BAD_SHAPE)
+ * Sequences that share pages cannot be cut (a row kept by one would be overwritten by the
+ * other).  The pages from ceil(keep / P) on are the caller's to free.
+ */
+typedef struct pgqa_evict_args {
+    size_t struct_size;
+    void* k_cache;
+    void* v_cache;
+    float* weights;
+    float* weights_out;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    int32_t* kept;
+    int32_t* new_lens;
+    int64_t batch_size, num_heads_k, headdim, page_size, num_pages, bt_stride;
+    int64_t keep, sinks, recent;
+    int32_t kv_format, reserved;
+} pgqa_evict_args;
+
+int pgqa_evict(const pgqa_evict_args* args, void* stream);
 
 /* Bytes of workspace pgqa_decode_v1 needs for this shape on the current device
  * (no counterpart in the reference, whose workspace is a hidden static buffer,

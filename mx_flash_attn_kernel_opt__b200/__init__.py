@@ -9,6 +9,10 @@ libpgqa.so in this directory).  Python entry points:
                         several query tokens, optional append of new K/V tokens
   append_kv(...)        the append-KV step alone
   flash_attn_with_kvcache(...)  flash-attn's argument list, for the paged case
+  rope_append_kv(...)   rotary positions (one or several axes) with the append, also
+                        into e4m3 pages
+  accumulate_weights(...)  the attention weight each cached token received
+  evict_kv(...)         eviction from the cache by that weight
 """
 from ._lib import LIB_PATH, PgqaError, lib  # noqa: F401
 from .ops import (  # noqa: F401
@@ -21,6 +25,8 @@ from .ops import (  # noqa: F401
     run_kernel_cabi,
     workspace_for,
 )
+from .serving import accumulate_weights, evict_kv, rope_append_kv  # noqa: F401
 
 __all__ = ["run_kernel", "run_kernel_cabi", "decode", "append_kv", "flash_attn_with_kvcache",
-           "make_plan", "check_device_error", "workspace_for", "PgqaError", "lib", "LIB_PATH"]
+           "rope_append_kv", "accumulate_weights", "evict_kv", "make_plan",
+           "check_device_error", "workspace_for", "PgqaError", "lib", "LIB_PATH"]

@@ -53,6 +53,53 @@ class PgqaDecodeArgs(ctypes.Structure):
     ]
 
 
+class PgqaRopeArgs(ctypes.Structure):
+    """include/pgqa.h pgqa_rope_args (pgqa_rope_append)."""
+    _fields_ = [
+        ("struct_size", c_size_t),
+        ("q", c_void_p), ("k_new", c_void_p), ("v_new", c_void_p), ("q_out", c_void_p),
+        ("k_cache", c_void_p), ("v_cache", c_void_p), ("seq_lens", c_void_p),
+        ("block_table", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("positions", c_void_p), ("cu_seqlens", c_void_p), ("weights", c_void_p),
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("batch_size", c_int64), ("seqlen", c_int64), ("tokens", c_int64),
+        ("num_heads", c_int64), ("num_heads_k", c_int64), ("headdim", c_int64),
+        ("page_size", c_int64), ("num_pages", c_int64), ("bt_stride", c_int64),
+        ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3),
+        ("table_rows", c_int64), ("rotary_dim", c_int64), ("num_axes", c_int64),
+        ("interleaved", c_int32), ("kv_format", c_int32), ("table_format", c_int32),
+        ("reserved", c_int32), ("pair_axis", ctypes.c_uint8 * 64),
+    ]
+
+
+class PgqaWeightsArgs(ctypes.Structure):
+    """include/pgqa.h pgqa_weights_args (pgqa_accumulate_weights)."""
+    _fields_ = [
+        ("struct_size", c_size_t),
+        ("q", c_void_p), ("k_cache", c_void_p), ("softmax_lse", c_void_p),
+        ("weights", c_void_p), ("seq_lens", c_void_p), ("block_table", c_void_p),
+        ("k_scale", c_void_p),
+        ("batch_size", c_int64), ("seqlen_q", c_int64), ("num_heads", c_int64),
+        ("num_heads_k", c_int64), ("headdim", c_int64), ("page_size", c_int64),
+        ("num_pages", c_int64), ("bt_stride", c_int64), ("causal", c_int64),
+        ("scale", c_float), ("kv_format", c_int32),
+    ]
+
+
+class PgqaEvictArgs(ctypes.Structure):
+    """include/pgqa.h pgqa_evict_args (pgqa_evict)."""
+    _fields_ = [
+        ("struct_size", c_size_t),
+        ("k_cache", c_void_p), ("v_cache", c_void_p), ("weights", c_void_p),
+        ("weights_out", c_void_p), ("seq_lens", c_void_p), ("block_table", c_void_p),
+        ("kept", c_void_p), ("new_lens", c_void_p),
+        ("batch_size", c_int64), ("num_heads_k", c_int64), ("headdim", c_int64),
+        ("page_size", c_int64), ("num_pages", c_int64), ("bt_stride", c_int64),
+        ("keep", c_int64), ("sinks", c_int64), ("recent", c_int64),
+        ("kv_format", c_int32), ("reserved", c_int32),
+    ]
+
+
 SIGNATURES = {
     "run_kernel": (None, [c_void_p] * 4 + [c_void_p, c_void_p] + [c_int64] * 9),
     "pgqa_decode_v1": (ctypes.c_int, [c_void_p] * 6 + [c_int64] * 8 +
@@ -68,6 +115,9 @@ SIGNATURES = {
     "pgqa_append_kv_fp8": (ctypes.c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_void_p] * 2),
     "pgqa_decode_fp8": (ctypes.c_int, [c_void_p] * 8 + [c_int64] * 11 +
                         [c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "pgqa_rope_append": (ctypes.c_int, [ctypes.POINTER(PgqaRopeArgs), c_void_p]),
+    "pgqa_accumulate_weights": (ctypes.c_int, [ctypes.POINTER(PgqaWeightsArgs), c_void_p]),
+    "pgqa_evict": (ctypes.c_int, [ctypes.POINTER(PgqaEvictArgs), c_void_p]),
     "pgqa_workspace_size": (c_size_t, [c_int64] * 5),
     "pgqa_workspace_init": (ctypes.c_int, [c_void_p, c_size_t, c_void_p]),
     "pgqa_last_status": (ctypes.c_int, []),
@@ -86,6 +136,7 @@ STATUS = {
     3: "PGQA_ERR_UNSUPPORTED", 4: "PGQA_ERR_MISALIGNED", 5: "PGQA_ERR_WORKSPACE",
     6: "PGQA_ERR_CUDA", 7: "PGQA_ERR_NO_DEVICE", 8: "PGQA_ERR_DEVICE_TIMEOUT",
     9: "PGQA_ERR_DEVICE_BAD_PAGE", 10: "PGQA_ERR_DEVICE_BAD_SEQLEN", 11: "PGQA_ERR_SCRATCH_LIMIT",
+    12: "PGQA_ERR_DEVICE_BAD_POSITION",
 }
 
 _lock = threading.Lock()

@@ -9,9 +9,11 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = [os.path.join(CSRC, "pgqa_decode.cu"), os.path.join(CSRC, "pgqa_append.cu"),
-           os.path.join(CSRC, "pgqa_tc.cu")]
+           os.path.join(CSRC, "pgqa_tc.cu"), os.path.join(CSRC, "pgqa_rope.cu"),
+           os.path.join(CSRC, "pgqa_weights.cu"), os.path.join(CSRC, "pgqa_evict.cu")]
 DEPS = SOURCES + [
     os.path.join(CSRC, "pgqa_append.h"),
+    os.path.join(CSRC, "pgqa_host.h"),
     os.path.join(CSRC, "pgqa_partition.h"),
     os.path.join(CSRC, "pgqa_ptx.cuh"),
     os.path.join(CSRC, "pgqa_tc.h"),

@@ -57,6 +57,7 @@
 
 #include "../../include/pgqa.h"
 #include "pgqa_append.h"
+#include "pgqa_host.h"
 #include "pgqa_partition.h"
 #include "pgqa_ptx.cuh"
 #include "pgqa_tc.h"
@@ -1455,6 +1456,10 @@ int device_info(int dev, DevInfo* out) {
     return d.status;
 }
 
+/* ---- error word of the entry points that take no workspace (pgqa_host.h) ---- */
+static __device__ int32_t g_error_word;
+int32_t* g_error_word_ptr[kMaxDevices] = {nullptr};  // guarded by g_dev_mu
+
 /* ---- cuTensorMapEncodeTiled through the runtime's driver entry point ---- */
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1784,6 +1789,45 @@ int decode_impl(const void* q, const void* k, const void* v, void* out, const in
 }
 
 }  // namespace
+
+/* ---- pgqa_host.h ---- */
+static_assert((int)kErrTimeout == (int)kDevErrTimeout && (int)kErrBadPage == (int)kDevErrBadPage &&
+                  (int)kErrBadSeqlen == (int)kDevErrBadSeqlen,
+              "one set of error bits");
+
+int host_device(int* dev, int* sms, int* smem_optin) {
+    if (cudaGetDevice(dev) != cudaSuccess) {
+        cudaGetLastError();
+        return PGQA_ERR_NO_DEVICE;
+    }
+    DevInfo di;
+    const int st = device_info(*dev, &di);
+    *sms = di.sms;
+    *smem_optin = di.smem_optin;
+    return st;
+}
+
+int host_error_word(int dev, int32_t** err) {
+    if (dev < 0 || dev >= kMaxDevices) return PGQA_ERR_NO_DEVICE;
+    std::lock_guard<std::mutex> lk(g_dev_mu);
+    if (g_error_word_ptr[dev] == nullptr) {
+        void* ptr = nullptr;
+        if (cudaGetSymbolAddress(&ptr, g_error_word) != cudaSuccess) {
+            cudaGetLastError();
+            return PGQA_ERR_CUDA;
+        }
+        g_error_word_ptr[dev] = static_cast<int32_t*>(ptr);
+    }
+    *err = g_error_word_ptr[dev];
+    return PGQA_OK;
+}
+
+int host_set_status(int st) { return set_status(st); }
+
+bool host_pdl() { return knobs().no_pdl == 0; }
+
+void* host_encode_tiled() { return reinterpret_cast<void*>(encode_fn()); }
+
 }  // namespace pgqa
 
 /* ------------------------------------------------------------------------------------ */
@@ -2018,6 +2062,7 @@ extern "C" const char* pgqa_status_string(int status) {
         case PGQA_ERR_DEVICE_TIMEOUT: return "device-side wait timed out";
         case PGQA_ERR_DEVICE_BAD_PAGE: return "block_table entry outside [0, num_pages)";
         case PGQA_ERR_DEVICE_BAD_SEQLEN: return "seq_len outside [0, table capacity]";
+        case PGQA_ERR_DEVICE_BAD_POSITION: return "position outside the cosine and sine tables";
         case PGQA_ERR_SCRATCH_LIMIT:
             return "shape needs more scratch than the fixed 4 MiB allocation-free buffer";
         default: return "unknown status";
@@ -2041,6 +2086,7 @@ int read_error_word(void* word_ptr, cudaStream_t s) {
     if (word & kErrTimeout) return PGQA_ERR_DEVICE_TIMEOUT;
     if (word & kErrBadPage) return PGQA_ERR_DEVICE_BAD_PAGE;
     if (word & kErrBadSeqlen) return PGQA_ERR_DEVICE_BAD_SEQLEN;
+    if (word & kDevErrBadPosition) return PGQA_ERR_DEVICE_BAD_POSITION;
     return PGQA_OK;
 }
 }  // namespace
@@ -2052,6 +2098,16 @@ extern "C" int pgqa_check_device_error(void* workspace, void* stream) {
         return PGQA_ERR_NO_DEVICE;
     }
     if (workspace == nullptr) {
+        // the word of the entry points that take no workspace, when one has run here
+        int32_t* word = nullptr;
+        if (dev >= 0 && dev < kMaxDevices) {
+            std::lock_guard<std::mutex> lk(g_dev_mu);
+            word = g_error_word_ptr[dev];
+        }
+        if (word != nullptr) {
+            const int st = read_error_word(word, static_cast<cudaStream_t>(stream));
+            if (st != PGQA_OK) return st;
+        }
         std::lock_guard<std::mutex> lk(g_ws_mu);
         if (dev < 0 || dev >= kMaxDevices || g_ws[dev].ptr == nullptr) return PGQA_OK;
         workspace = g_ws[dev].ptr;

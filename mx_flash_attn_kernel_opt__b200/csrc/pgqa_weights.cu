@@ -1,0 +1,375 @@
+/*
+ * pgqa_weights.cu - the attention weight that each cached token receives, added to its
+ * entry of the weight pool [num_pages, Hkv, P]:
+ *
+ *     w[b, kv, t] += sum over rows r of KV head kv that see t of exp(scale q_r . k_t - lse_r)
+ *
+ * with the rows (query head, query token) and the masks of the decode, and lse_r the
+ * log-sum-exp that the decode returned for the row.  Scores, exponents and sums are fp32.
+ *
+ * Bound by the one pass over K (256 or 128 bytes per token and KV head against 8 bytes of
+ * weights).  Each warp owns an equal contiguous slice of 16-token chunks over the actual
+ * lengths (the same cut as the decode's, in units of warps) and works alone: no shared
+ * memory rings and no barriers in the stream.  K goes from global memory straight into
+ * mma.sync A fragments: the order of the 128 dimensions inside the dot product is free as
+ * long as q uses the same one, so lane (g, t) takes 16-byte pieces t, t + 4, ... of token
+ * rows g and g + 8, whole 64-byte runs per row, and q rows are loaded by the same
+ * addresses as B fragments.  A chunk's loads are issued one chunk ahead.  The four lanes
+ * that share a token add their partial sums by shuffles, and the token's weight gets one
+ * red.add: no other warp of the call adds to it (unless sequences share a page), so the
+ * result does not depend on any order.
+ *
+ * e4m3 keys become bf16 in registers (exact: 4 significant bits), next to bf16 q.
+ */
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pgqa_host.h"
+#include "pgqa_partition.h"
+#include "pgqa_ptx.cuh"
+
+namespace pgqa {
+namespace weights {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+struct Params {
+    const __nv_bfloat16* q;  // [B, Sq, Hq, 128]
+    const void* k_cache;
+    const float* lse;        // [B, Hq, Sq]
+    float* weights;          // [num_pages, Hkv, P]
+    const int32_t *seq_lens, *block_table;
+    const float* k_scale;
+    int32_t* err;
+    int64_t bt_stride, cap_tokens;
+    int32_t B, Sq, Hq, Hkv, g, rows, P, page_shift, num_pages, causal;
+    float scale_log2;
+};
+
+/* One 16-token chunk of one KV head in A-fragment order: per lane, pieces of rows g and g + 8. */
+template <bool KV8>
+struct Chunk {
+    static constexpr int kPieces = KV8 ? 2 : 4;
+    uint4 lo[kPieces], hi[kPieces];
+};
+
+__device__ __forceinline__ uint32_t bf16x2_of(float2 f) { return ptx::pack_bf16x2(f.x, f.y); }
+
+/* Eight e4m3 (two words) -> four bf16x2, exact. */
+__device__ __forceinline__ void e4m3x8_to_bf16(uint32_t w0, uint32_t w1, uint32_t (&o)[4]) {
+    o[0] = bf16x2_of(ptx::e4m3x2_to_f32x2(w0 & 0xffffu));
+    o[1] = bf16x2_of(ptx::e4m3x2_to_f32x2(w0 >> 16));
+    o[2] = bf16x2_of(ptx::e4m3x2_to_f32x2(w1 & 0xffffu));
+    o[3] = bf16x2_of(ptx::e4m3x2_to_f32x2(w1 >> 16));
+}
+
+/* q fragments of one group of 8 rows, in the dimension order of the chunk's pieces. */
+template <bool KV8>
+struct QFrag {
+    uint4 v[4];
+};
+
+/* Row r of the unit (b, kvh): query head r / Sq of the group, query token r % Sq. */
+__device__ __forceinline__ void row_of(const Params& p, int32_t b, int32_t kvh, int r, int64_t& qoff, int64_t& loff,
+                                       int32_t& tok) {
+    const int h = r / p.Sq;
+    tok = r - h * p.Sq;
+    const int head = kvh * p.g + h;
+    qoff = (((int64_t)b * p.Sq + tok) * p.Hq + head) * 128;
+    loff = ((int64_t)b * p.Hq + head) * p.Sq + tok;
+}
+
+/* Per lane: the q pieces of row 8 j + g, and for rows 8 j + 2 t, 8 j + 2 t + 1 (its two
+ * columns of the score tile) the negated log2-sum-exp and the number of tokens seen. */
+template <bool KV8>
+__device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t kvh, int32_t L, int j, int lane,
+                                           QFrag<KV8>& f, float (&nl)[2], int32_t (&lim)[2]) {
+    const int g = lane >> 2, t = lane & 3;
+    int64_t qo, lo;
+    int32_t tok;
+    const int r = 8 * j + g;
+    if (r < p.rows) {
+        row_of(p, b, kvh, r, qo, lo, tok);
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + qo);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            // e4m3: a 16-byte piece of K covers two consecutive pieces of q
+            f.v[i] = __ldg(src + (KV8 ? 8 * (i >> 1) + 2 * t + (i & 1) : 4 * i + t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.v[i] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int c = 8 * j + 2 * t + e;
+        nl[e] = 0.f;
+        lim[e] = 0;
+        if (c < p.rows) {
+            row_of(p, b, kvh, c, qo, lo, tok);
+            const float l = __ldg(p.lse + lo);
+            // a row that saw nothing (-inf) has no weight to give
+            if (l != -INFINITY) {
+                nl[e] = -l * 1.4426950408889634f;
+                lim[e] = p.causal ? L - p.Sq + 1 + tok : L;
+            }
+        }
+    }
+}
+
+template <bool KV8>
+__device__ __forceinline__ void load_chunk(const Params& p, int32_t pid, int32_t slot, int32_t kvh, int lane,
+                                           Chunk<KV8>& c) {
+    const int g = lane >> 2, t = lane & 3;
+    constexpr int kRow = KV8 ? 8 : 16;  // 16-byte pieces per token row
+    const int64_t row = ((int64_t)pid * p.P + slot + g) * p.Hkv + kvh;
+    const uint4* a = static_cast<const uint4*>(p.k_cache) + row * kRow + t;
+    const uint4* d = a + (int64_t)8 * p.Hkv * kRow;
+#pragma unroll
+    for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
+        c.lo[i] = __ldg(a + 4 * i);
+        c.hi[i] = __ldg(d + 4 * i);
+    }
+}
+
+/* Scores of the chunk's 16 tokens against 8 rows. */
+template <bool KV8>
+__device__ __forceinline__ void scores(const Chunk<KV8>& c, const QFrag<KV8>& f, float (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+    if (!KV8) {
+#pragma unroll
+        for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
+            ptx::mma_bf16_16816(s, c.lo[i].x, c.hi[i].x, c.lo[i].y, c.hi[i].y, f.v[i & 3].x, f.v[i & 3].y);
+            ptx::mma_bf16_16816(s, c.lo[i].z, c.hi[i].z, c.lo[i].w, c.hi[i].w, f.v[i & 3].z, f.v[i & 3].w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
+            uint32_t a[4], d[4];
+            e4m3x8_to_bf16(c.lo[i].x, c.lo[i].y, a);
+            e4m3x8_to_bf16(c.hi[i].x, c.hi[i].y, d);
+            ptx::mma_bf16_16816(s, a[0], d[0], a[1], d[1], f.v[2 * i].x, f.v[2 * i].y);
+            ptx::mma_bf16_16816(s, a[2], d[2], a[3], d[3], f.v[2 * i].z, f.v[2 * i].w);
+            e4m3x8_to_bf16(c.lo[i].z, c.lo[i].w, a);
+            e4m3x8_to_bf16(c.hi[i].z, c.hi[i].w, d);
+            ptx::mma_bf16_16816(s, a[0], d[0], a[1], d[1], f.v[2 * i + 1].x, f.v[2 * i + 1].y);
+            ptx::mma_bf16_16816(s, a[2], d[2], a[3], d[3], f.v[2 * i + 1].z, f.v[2 * i + 1].w);
+        }
+    }
+}
+
+/* NT > 0: that many groups of 8 rows, their q fragments held in registers over a unit;
+ * NT = 0: any number, the fragments re-read (from L1) for every chunk. */
+template <bool KV8, int NT>
+__global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
+    extern __shared__ uint32_t pre[];  // chunks of the sequences before b, [B + 1]
+    __shared__ uint32_t wsum[kWarps];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    {
+        const int per = (p.B + kThreads - 1) / kThreads;
+        const int s0 = min(p.B, tid * per), s1 = min(p.B, s0 + per);
+        uint32_t local = 0;
+        bool bad = false;
+        for (int b = s0; b < s1; ++b) {
+            const int32_t L = __ldg(p.seq_lens + b);
+            bad = bad || L < 0 || L > p.cap_tokens;
+            local += (uint32_t)seq_chunks(L, p.cap_tokens);
+        }
+        if (bad && blockIdx.x == 0) atomicOr(p.err, kDevErrBadSeqlen);
+        uint32_t incl = local;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        uint32_t run = incl - local;
+        for (int w = 0; w < warp; ++w) run += wsum[w];
+        for (int b = s0; b < s1; ++b) {
+            pre[b] = run;
+            run += (uint32_t)seq_chunks(__ldg(p.seq_lens + b), p.cap_tokens);
+        }
+        if (s1 == p.B) pre[p.B] = run;  // every thread past the last sequence writes the same total
+        __syncthreads();
+    }
+    const int64_t total = (int64_t)pre[p.B] * p.Hkv;
+    const int64_t nw = (int64_t)gridDim.x * kWarps;
+    const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;  // few chunks: spread over the SMs first
+    int64_t cur = slice_begin(w, nw, total);
+    const int64_t end = slice_begin(w + 1, nw, total);
+    if (cur >= end) return;
+    int32_t lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) >> 1;
+        if ((int64_t)pre[mid] * p.Hkv <= cur) lo = mid; else hi = mid;
+    }
+    int32_t b = lo;
+    int32_t n = (int32_t)(pre[b + 1] - pre[b]);
+    const int64_t in = cur - (int64_t)pre[b] * p.Hkv;
+    int32_t kvh = (int32_t)(in / n), c = (int32_t)(in - (int64_t)kvh * n);
+    const int t = lane & 3, g = lane >> 2;
+    constexpr int kHeld = NT > 0 ? NT : 1;
+    const int groups = (p.rows + 7) / 8;
+
+    while (cur < end) {
+        // the slice's part of the unit (b, kvh): chunks [c, ce)
+        const int32_t ce = (int32_t)((end - cur < n - c) ? c + (end - cur) : n);
+        const int64_t L64 = __ldg(p.seq_lens + b);
+        const int32_t L = (int32_t)(L64 > p.cap_tokens ? p.cap_tokens : L64);
+        const float ks = (KV8 && p.k_scale) ? __ldg(p.k_scale + kvh) : 1.f;
+        const float mul = p.scale_log2 * ks;
+        QFrag<KV8> qf[kHeld];
+        float nl[kHeld][2];
+        int32_t lim[kHeld][2];
+        if (NT > 0) {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j) load_group<KV8>(p, b, kvh, L, j, lane, qf[j], nl[j], lim[j]);
+        }
+        const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+        auto page_of = [&](int32_t chunk, int32_t& pid, int32_t& slot) {
+            const int32_t tok = chunk * kChunkTokens;
+            const int32_t page = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.P;
+            slot = tok - page * p.P;
+            pid = __ldg(bt + page);
+        };
+        auto check = [&](int32_t& pid) -> bool {
+            if ((uint32_t)pid < (uint32_t)p.num_pages) return true;
+            if (lane == 0) atomicOr(p.err, kDevErrBadPage);
+            pid = 0;  // read, not added to
+            return false;
+        };
+        Chunk<KV8> k;
+        int32_t pid, slot, npid = 0, nslot = 0;
+        page_of(c, pid, slot);
+        bool ok = check(pid);
+        load_chunk<KV8>(p, pid, slot, kvh, lane, k);
+        if (c + 1 < ce) page_of(c + 1, npid, nslot);
+        for (; c < ce; ++c) {
+            Chunk<KV8> kn;
+            bool nok = false;
+            int32_t fpid = 0, fslot = 0;
+            if (c + 1 < ce) {
+                nok = check(npid);
+                load_chunk<KV8>(p, npid, nslot, kvh, lane, kn);
+                if (c + 2 < ce) page_of(c + 2, fpid, fslot);
+            }
+            const int32_t tok = c * kChunkTokens + g;
+            float w0 = 0.f, w1 = 0.f;  // weights of tokens g and g + 8 over this lane's rows
+            auto add = [&](const QFrag<KV8>& f, const float (&nlj)[2], const int32_t (&limj)[2]) {
+                float s[4];
+                scores<KV8>(k, f, s);
+                // selected, never multiplied: a masked score may be infinite or NaN
+                w0 += tok < limj[0] ? ptx::ex2(fmaf(s[0], mul, nlj[0])) : 0.f;
+                w0 += tok < limj[1] ? ptx::ex2(fmaf(s[1], mul, nlj[1])) : 0.f;
+                w1 += tok + 8 < limj[0] ? ptx::ex2(fmaf(s[2], mul, nlj[0])) : 0.f;
+                w1 += tok + 8 < limj[1] ? ptx::ex2(fmaf(s[3], mul, nlj[1])) : 0.f;
+            };
+            if (NT > 0) {
+#pragma unroll
+                for (int j = 0; j < kHeld; ++j) add(qf[j], nl[j], lim[j]);
+            } else {
+                for (int j = 0; j < groups; ++j) {
+                    load_group<KV8>(p, b, kvh, L, j, lane, qf[0], nl[0], lim[0]);
+                    add(qf[0], nl[0], lim[0]);
+                }
+            }
+            w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+            w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
+            w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+            w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
+            if (ok && t < 2) {
+                const int i = g + 8 * t;
+                if (c * kChunkTokens + i < L)
+                    atomicAdd(p.weights + ((int64_t)pid * p.Hkv + kvh) * p.P + slot + i, t == 0 ? w0 : w1);
+            }
+            if (c + 1 < ce) k = kn;
+            pid = npid; slot = nslot; ok = nok;
+            npid = fpid; nslot = fslot;
+        }
+        cur = (int64_t)pre[b] * p.Hkv + (int64_t)kvh * n + ce;
+        c = 0;
+        if (cur < end && ++kvh == p.Hkv) {
+            kvh = 0;
+            do { ++b; } while (pre[b + 1] == pre[b]);
+            n = (int32_t)(pre[b + 1] - pre[b]);
+        }
+    }
+}
+
+template <bool KV8, int NT>
+int launch(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
+    static int done[kHostMaxDevices] = {0};
+    auto kern = weights_kernel<KV8, NT>;
+    int st = PGQA_OK;
+    if (smem > 48 * 1024 && (st = host_smem_limit(kern, dev, smem, done)) != PGQA_OK) return st;
+    return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, p);
+}
+
+template <bool KV8>
+int launch_nt(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
+    if (p.rows <= 8) return launch<KV8, 1>(p, dev, sms, smem, stream);
+    if (p.rows <= 16) return launch<KV8, 2>(p, dev, sms, smem, stream);
+    if (p.rows <= 32) return launch<KV8, 4>(p, dev, sms, smem, stream);
+    return launch<KV8, 0>(p, dev, sms, smem, stream);
+}
+
+int entry(const pgqa_weights_args* a, cudaStream_t stream) {
+    if (a == nullptr) return PGQA_ERR_NULL_POINTER;
+    if (a->struct_size != sizeof(pgqa_weights_args)) return PGQA_ERR_BAD_SHAPE;
+    if (!a->q || !a->k_cache || !a->softmax_lse || !a->weights || !a->seq_lens || !a->block_table)
+        return PGQA_ERR_NULL_POINTER;
+    int st = host_check_pages(a->batch_size, a->num_heads_k, a->headdim, a->page_size, a->num_pages, a->bt_stride);
+    if (st != PGQA_OK) return st;
+    if (a->num_heads <= 0 || a->num_heads % a->num_heads_k != 0 || a->num_heads > 65536) return PGQA_ERR_BAD_SHAPE;
+    if (a->seqlen_q <= 0) return PGQA_ERR_BAD_SHAPE;
+    if (a->seqlen_q > 4096) return PGQA_ERR_UNSUPPORTED;
+    if (a->causal != 0 && a->causal != 1) return PGQA_ERR_BAD_SHAPE;
+    if (!(a->scale > 0.f) || !isfinite(a->scale)) return PGQA_ERR_BAD_SHAPE;
+    if (a->kv_format != 0 && a->kv_format != 1) return PGQA_ERR_UNSUPPORTED;
+    if (a->kv_format == 0 && a->k_scale) return PGQA_ERR_BAD_SHAPE;
+    if (!host_aligned(a->q, 16) || !host_aligned(a->k_cache, 16) || !host_aligned(a->softmax_lse, 4) ||
+        !host_aligned(a->weights, 4) || !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) ||
+        !host_aligned(a->k_scale, 4))
+        return PGQA_ERR_MISALIGNED;
+    int dev, sms, optin;
+    if ((st = host_device(&dev, &sms, &optin)) != PGQA_OK) return st;
+    // the table of chunk counts before each sequence lives in shared memory (two CTAs per SM)
+    if ((a->batch_size + 1) * 4 > optin / 2 - 2048) return PGQA_ERR_UNSUPPORTED;
+    Params p = {};
+    if ((st = host_error_word(dev, &p.err)) != PGQA_OK) return st;
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.k_cache = a->k_cache;
+    p.lse = a->softmax_lse;
+    p.weights = a->weights;
+    p.seq_lens = a->seq_lens;
+    p.block_table = a->block_table;
+    p.k_scale = a->k_scale;
+    p.bt_stride = a->bt_stride;
+    p.cap_tokens = a->bt_stride * a->page_size;
+    p.B = (int32_t)a->batch_size;
+    p.Sq = (int32_t)a->seqlen_q;
+    p.Hq = (int32_t)a->num_heads;
+    p.Hkv = (int32_t)a->num_heads_k;
+    p.g = p.Hq / p.Hkv;
+    p.rows = p.g * p.Sq;
+    p.P = (int32_t)a->page_size;
+    p.page_shift = host_shift(a->page_size);
+    p.num_pages = (int32_t)a->num_pages;
+    p.causal = (int32_t)a->causal;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    const int smem = (int)(a->batch_size + 1) * 4;
+    return a->kv_format == 1 ? launch_nt<true>(p, dev, sms, smem, stream)
+                             : launch_nt<false>(p, dev, sms, smem, stream);
+}
+
+}  // namespace weights
+}  // namespace pgqa
+
+extern "C" int pgqa_accumulate_weights(const pgqa_weights_args* args, void* stream) {
+    return pgqa::host_set_status(pgqa::weights::entry(args, static_cast<cudaStream_t>(stream)));
+}

@@ -18,3 +18,4 @@ from .paged_decode import (  # noqa: F401
     split_decode_ref,
     match_stats,
 )
+from .serving import evict_ref, rope_ref, weights_ref  # noqa: F401
