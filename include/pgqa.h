@@ -364,6 +364,49 @@ typedef struct pgqa_evict_args {
 
 int pgqa_evict(const pgqa_evict_args* args, void* stream);
 
+/*
+ * Cross attention: out[x, h] = softmax(scale * q[x, h] . K^T) . V over the first seq_lens[b]
+ * tokens of sequence b's pages, for every query token x of sequence b.  No causal mask; the
+ * number of query tokens and of keys are unrelated.  A sequence without keys gives zeros
+ * (and a log-sum-exp of -inf).  bf16 in and out, fp32 scores, sums and accumulators.
+ *   q            [tokens, Hq, 128], token stride q_stride elements (a multiple of 8, at
+ *                least Hq * 128), heads contiguous
+ *   out          [tokens, Hq, 128], contiguous
+ *   cu_seqlens   NULL: [batch_size, seqlen_q] tokens, tokens = batch_size * seqlen_q.
+ *                Else int32 [batch_size + 1], ascending from 0; rows of out and softmax_lse
+ *                from cu[batch_size] on are left as they are
+ *   k, v pools   [num_pages, P, Hkv, 128] bf16, as in the decode; g = Hq / Hkv <= 128
+ *   softmax_lse  NULL or fp32: [Hq, tokens] with cu_seqlens, else [B, Hq, seqlen_q]
+ *   workspace    pgqa_cross_workspace_size(...) bytes, 256-byte aligned, any contents (may
+ *                be NULL when that is 0): partial results of calls with few query tokens.
+ *                Calls that share one must be ordered.
+ */
+typedef struct pgqa_cross_args {
+    size_t struct_size;
+    const void* q;
+    const void* k_cache;
+    const void* v_cache;
+    void* out;
+    float* softmax_lse;
+    const int32_t* seq_lens;
+    const int32_t* block_table;
+    const int32_t* cu_seqlens;
+    int64_t batch_size, seqlen_q, tokens, q_stride, num_heads, num_heads_k, headdim;
+    int64_t page_size, num_pages, bt_stride;
+    float scale;
+    int32_t reserved;
+    void* workspace;
+    size_t workspace_bytes;
+} pgqa_cross_args;
+
+int pgqa_cross_attention(const pgqa_cross_args* args, void* stream);
+
+/* Bytes of workspace pgqa_cross_attention needs on the current device (0: none, or an
+ * invalid shape; pgqa_last_status() tells which). */
+size_t pgqa_cross_workspace_size(int64_t tokens, int64_t batch_size, int64_t num_heads,
+                                 int64_t num_heads_k, int64_t headdim, int64_t page_size,
+                                 int64_t bt_stride);
+
 /* Bytes of workspace pgqa_decode_v1 needs for this shape on the current device
  * (no counterpart in the reference, whose workspace is a hidden static buffer,
  * submission_clean.cu:478-491).  Returns 0 on invalid or unsupported shapes;

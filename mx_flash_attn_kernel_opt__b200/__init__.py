@@ -13,6 +13,7 @@ libpgqa.so in this directory).  Python entry points:
                         into e4m3 pages
   accumulate_weights(...)  the attention weight each cached token received
   evict_kv(...)         eviction from the cache by that weight
+  cross_attention(...)  attention of prompt tokens over an encoder's states in pages
 """
 from ._lib import LIB_PATH, PgqaError, lib  # noqa: F401
 from .ops import (  # noqa: F401
@@ -25,8 +26,13 @@ from .ops import (  # noqa: F401
     run_kernel_cabi,
     workspace_for,
 )
-from .serving import accumulate_weights, evict_kv, rope_append_kv  # noqa: F401
+from .serving import (  # noqa: F401
+    accumulate_weights,
+    cross_attention,
+    evict_kv,
+    rope_append_kv,
+)
 
 __all__ = ["run_kernel", "run_kernel_cabi", "decode", "append_kv", "flash_attn_with_kvcache",
-           "rope_append_kv", "accumulate_weights", "evict_kv", "make_plan",
+           "rope_append_kv", "accumulate_weights", "evict_kv", "cross_attention", "make_plan",
            "check_device_error", "workspace_for", "PgqaError", "lib", "LIB_PATH"]

@@ -100,6 +100,22 @@ class PgqaEvictArgs(ctypes.Structure):
     ]
 
 
+class PgqaCrossArgs(ctypes.Structure):
+    """include/pgqa.h pgqa_cross_args (pgqa_cross_attention)."""
+    _fields_ = [
+        ("struct_size", c_size_t),
+        ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("out", c_void_p),
+        ("softmax_lse", c_void_p), ("seq_lens", c_void_p), ("block_table", c_void_p),
+        ("cu_seqlens", c_void_p),
+        ("batch_size", c_int64), ("seqlen_q", c_int64), ("tokens", c_int64),
+        ("q_stride", c_int64), ("num_heads", c_int64), ("num_heads_k", c_int64),
+        ("headdim", c_int64), ("page_size", c_int64), ("num_pages", c_int64),
+        ("bt_stride", c_int64),
+        ("scale", c_float), ("reserved", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 SIGNATURES = {
     "run_kernel": (None, [c_void_p] * 4 + [c_void_p, c_void_p] + [c_int64] * 9),
     "pgqa_decode_v1": (ctypes.c_int, [c_void_p] * 6 + [c_int64] * 8 +
@@ -118,6 +134,8 @@ SIGNATURES = {
     "pgqa_rope_append": (ctypes.c_int, [ctypes.POINTER(PgqaRopeArgs), c_void_p]),
     "pgqa_accumulate_weights": (ctypes.c_int, [ctypes.POINTER(PgqaWeightsArgs), c_void_p]),
     "pgqa_evict": (ctypes.c_int, [ctypes.POINTER(PgqaEvictArgs), c_void_p]),
+    "pgqa_cross_attention": (ctypes.c_int, [ctypes.POINTER(PgqaCrossArgs), c_void_p]),
+    "pgqa_cross_workspace_size": (c_size_t, [c_int64] * 7),
     "pgqa_workspace_size": (c_size_t, [c_int64] * 5),
     "pgqa_workspace_init": (ctypes.c_int, [c_void_p, c_size_t, c_void_p]),
     "pgqa_last_status": (ctypes.c_int, []),

@@ -10,7 +10,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = [os.path.join(CSRC, "pgqa_decode.cu"), os.path.join(CSRC, "pgqa_append.cu"),
            os.path.join(CSRC, "pgqa_tc.cu"), os.path.join(CSRC, "pgqa_rope.cu"),
-           os.path.join(CSRC, "pgqa_weights.cu"), os.path.join(CSRC, "pgqa_evict.cu")]
+           os.path.join(CSRC, "pgqa_weights.cu"), os.path.join(CSRC, "pgqa_evict.cu"),
+           os.path.join(CSRC, "pgqa_cross.cu")]
 DEPS = SOURCES + [
     os.path.join(CSRC, "pgqa_append.h"),
     os.path.join(CSRC, "pgqa_host.h"),

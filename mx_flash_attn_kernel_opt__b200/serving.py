@@ -1,10 +1,12 @@
 """Operators around the paged decode, for serving: rotary positions with the append of new
-tokens, the attention weight each cached token receives, and eviction by that weight.
+tokens, the attention weight each cached token receives, eviction by that weight, and the
+attention of prompt tokens over an encoder's states.
 
     q = rope_append_kv(q, k, v, k_cache, v_cache, block_table, seq_lens, cos, sin, ...)
     out, lse = decode(q, k_cache, v_cache, block_table, seq_lens + 1, return_lse=True)
     accumulate_weights(q, k_cache, block_table, seq_lens + 1, lse, weights)
     kept, seq_lens = evict_kv(k_cache, v_cache, weights, block_table, seq_lens + 1, keep)
+    out = cross_attention(q, enc_k, enc_v, enc_table, enc_lens, cu_seqlens_q=cu)
 
 `weights` is a float32 pool [num_pages, Hkv, P] beside the K and V pools.  Every call runs
 on torch's current stream of the tensors' device, allocates nothing but its outputs and can
@@ -282,3 +284,71 @@ def evict_kv(k_cache, v_cache, weights, block_table, seq_lens, keep, *, sinks=0,
         Hkv, D, P, num_pages, block_table.shape[1], keep, int(sinks), int(recent), int(fp8))
     _launch(lib().pgqa_evict, a, dev, "pgqa_evict")
     return kept, new_lens
+
+
+def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=None, scale=None,
+                    out=None, return_lse=False):
+    """Attention of query tokens over each sequence's encoder states, held in pages:
+    softmax(scale * q K^T) V over the first seq_lens[b] tokens of sequence b, no causal mask.
+
+    q [B, Sq, Hq, 128] bf16, or packed [tokens, Hq, 128] with `cu_seqlens_q` [B + 1] int32,
+    ascending from 0; its token stride may be any multiple of 8 elements (a slice of a
+    projection), heads contiguous.  k_cache / v_cache [num_pages, P, Hkv, 128] bf16,
+    block_table [B, width] int32, seq_lens [B] int32 (0: the sequence's rows are zeros).
+
+    Returns out (contiguous, q's shape) or (out, lse) with `return_lse`: fp32 [Hq, tokens]
+    for packed q, else [B, Hq, Sq]; -inf where a row sees no key.  Rows of packed tokens
+    behind the last sequence are left as they are in `out`."""
+    what = "cross_attention"
+    dev, fp8, num_pages, P, Hkv, D, B = _pools(what, k_cache, v_cache, block_table, seq_lens)
+    if fp8:
+        raise NotImplementedError(f"{what}: float8_e4m3fn pools are not implemented here")
+    if q.dtype != _BF16:
+        raise TypeError(f"{what}: q must be {_BF16}, got {q.dtype}")
+    if q.device != dev:
+        raise ValueError(f"{what}: q must be on {dev}, got {q.device}")
+    if cu_seqlens_q is not None:
+        _check(what, dev, ("cu_seqlens_q", cu_seqlens_q, _I32))
+        if q.dim() != 3 or tuple(cu_seqlens_q.shape) != (B + 1,):
+            raise PgqaError(2, f"{what}: with cu_seqlens_q [B + 1], q is [tokens, Hq, D]")
+        tokens, Sq, stride = q.shape[0], 0, q.stride(0)
+    else:
+        if q.dim() != 4 or q.shape[0] != B:
+            raise PgqaError(2, f"{what}: q must be [B, Sq, Hq, D], or packed with cu_seqlens_q")
+        Sq, stride = q.shape[1], q.stride(1)
+        tokens = B * Sq
+        if B > 1 and Sq > 1 and q.stride(0) != Sq * stride:
+            raise ValueError(f"{what}: the sequences of q must follow each other without a gap")
+        if Sq == 1:
+            stride = q.stride(0)
+    Hq = q.shape[-2]
+    if q.shape[-1] != D:
+        raise PgqaError(2, f"{what}: q and the pools must have one head dimension")
+    if q.stride(-1) != 1 or (Hq > 1 and q.stride(-2) != D):
+        raise ValueError(f"{what}: the heads of a token of q must be contiguous")
+    if tokens <= 1:
+        stride = Hq * D
+    if out is None:
+        out = torch.empty(q.shape, dtype=_BF16, device=dev)
+    else:
+        _check(what, dev, ("out", out, _BF16))
+        if out.shape != q.shape:
+            raise PgqaError(2, f"{what}: out must have q's shape")
+    lse = None
+    if return_lse:
+        lse = torch.empty((Hq, tokens) if cu_seqlens_q is not None else (B, Hq, Sq), dtype=_F32, device=dev)
+    if tokens:
+        L = lib()
+        with torch.cuda.device(dev):
+            need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, block_table.shape[1])
+        # a buffer of this call's own: calls on two streams or in two graphs share none
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        a = _lib.PgqaCrossArgs(
+            ctypes.sizeof(_lib.PgqaCrossArgs), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            out.data_ptr(), lse.data_ptr() if lse is not None else None, seq_lens.data_ptr(),
+            block_table.data_ptr(), cu_seqlens_q.data_ptr() if cu_seqlens_q is not None else None, B,
+            Sq, tokens, stride, Hq, Hkv, D, P, num_pages, block_table.shape[1],
+            float(scale) if scale is not None else 1.0 / math.sqrt(D), 0,
+            ws.data_ptr() if ws is not None else None, need)
+        _launch(L.pgqa_cross_attention, a, dev, "pgqa_cross_attention")
+    return (out, lse) if return_lse else out

@@ -144,3 +144,53 @@ def test_python_entry_points_refuse_bad_tensors(cuda_device):
     with pytest.raises(pgqa.PgqaError):
         pgqa.evict_kv(k, z(5, 16, 2, 128, dtype=bf), w, bt, lens, 4)
     torch.cuda.synchronize()
+
+
+def cross(**kw):
+    a = _lib.PgqaCrossArgs(struct_size=ctypes.sizeof(_lib.PgqaCrossArgs), q=A, k_cache=A, v_cache=A, out=A,
+                           seq_lens=A, block_table=A, cu_seqlens=A, batch_size=2, tokens=10, q_stride=1024,
+                           num_heads=8, num_heads_k=2, headdim=128, page_size=16, num_pages=9, bt_stride=4,
+                           scale=0.1)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return _lib.lib().pgqa_cross_attention(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("status,kw", [
+    (2, dict(struct_size=8)), (1, dict(q=None)), (1, dict(out=None)), (1, dict(block_table=None)),
+    (2, dict(tokens=-1)), (2, dict(num_heads=9)), (3, dict(num_heads=258)), (3, dict(headdim=64)),
+    (3, dict(page_size=8)), (2, dict(num_pages=0)), (3, dict(num_pages=1 << 27)), (2, dict(cu_seqlens=None)),
+    (2, dict(scale=-1.0)), (2, dict(scale=float("nan"))), (2, dict(q_stride=1016)), (4, dict(q_stride=1028)),
+    (4, dict(q=A + 8)), (4, dict(out=A + 8)), (4, dict(workspace=A + 128)), (4, dict(softmax_lse=A + 2)),
+    (3, dict(q_stride=1 << 39)), (2, dict(batch_size=0)),
+])
+def test_cross_attention(status, kw):
+    assert cross(**kw) == status
+
+
+def test_cross_attention_python_refusals():
+    z = torch.zeros
+    k = z(4, 16, 2, 128, dtype=torch.bfloat16)
+    bt, lens = z(2, 2, dtype=torch.int32), z(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        pgqa.cross_attention(z(2, 3, 8, 128, dtype=torch.bfloat16), k, k, bt, lens)
+
+
+@pytest.mark.gpu
+def test_cross_attention_refuses_bad_tensors(cuda_device):
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=cuda_device)  # noqa: E731
+    i32 = torch.int32
+    k, bt, lens, q = z(4, 16, 2, 128), z(2, 2, dtype=i32), z(2, dtype=i32), z(2, 3, 8, 128)
+    for error, args, kw in (
+            (NotImplementedError, (q, *[k.to(torch.float8_e4m3fn)] * 2), {}), (TypeError, (q.float(), k, k), {}),
+            (ValueError, (q.cpu(), k, k), {}), (ValueError, (z(2, 4, 8, 128)[:, :3], k, k), {}),
+            (ValueError, (z(2, 3, 128, 8).transpose(2, 3), k, k), {}),
+            (ValueError, (z(2, 3, 16, 128)[:, :, ::2], k, k), {}),
+            (pgqa.PgqaError, (z(3, 3, 8, 128), k, k), {}), (pgqa.PgqaError, (z(6, 8, 128), k, k), {}),
+            (pgqa.PgqaError, (z(6, 8, 128), k, k), dict(cu_seqlens_q=z(2, dtype=i32))),
+            (TypeError, (z(6, 8, 128), k, k), dict(cu_seqlens_q=z(3, dtype=torch.int64))),
+            (pgqa.PgqaError, (z(2, 3, 7, 128), k, k), {}), (pgqa.PgqaError, (q, k, k), dict(out=z(6, 8, 128))),
+            (pgqa.PgqaError, (q, k, z(5, 16, 2, 128)), {}), (pgqa.PgqaError, (q, k, k), dict(scale=0.0))):
+        with pytest.raises(error):
+            pgqa.cross_attention(*args, bt, lens, **kw)
+    torch.cuda.synchronize()
