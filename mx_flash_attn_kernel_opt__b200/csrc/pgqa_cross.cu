@@ -707,9 +707,9 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     const int64_t per = 2 * p.tile_tokens;
     int64_t ctas = (a->tokens / per + a->batch_size) * a->num_heads_k * p.splits;  // at least the items
     if (ctas > sms) ctas = sms;
-    st = host_launch(cross_kernel, dim3((unsigned)ctas), kThreads, kSmem, stream, qm, km, vm, p);
+    st = host_launch(cross_kernel, dim3((unsigned)ctas), kThreads, kSmem, stream, 1, qm, km, vm, p);
     if (st != PGQA_OK || p.splits == 1) return st;
-    return host_launch(join_kernel, dim3((unsigned)((a->tokens * a->num_heads + 7) / 8)), 256, 0, stream, p);
+    return host_launch(join_kernel, dim3((unsigned)((a->tokens * a->num_heads + 7) / 8)), 256, 0, stream, 1, p);
 }
 
 }  // namespace cross

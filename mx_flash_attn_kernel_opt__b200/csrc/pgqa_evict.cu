@@ -10,20 +10,23 @@
  *
  * Two launches:
  *
- * select_kernel, one CTA per (sequence, KV head).  The middle tokens' weights become
- * sortable 32-bit keys in shared memory (or are re-read from L2 when they do not fit); a
- * radix select over digits of 11, 11 and 10 bits finds the key of the last token kept and
- * how many of its equals stay, and one ordered pass with a block scan writes the indices.
- * 4 bytes per token are read from HBM once.
+ * select_kernel, one CTA or one cluster of CTAs per (sequence, KV head), each CTA with a
+ * contiguous range of the middle tokens.  Their weights become sortable 32-bit keys in
+ * shared memory (or are re-read from L2 when they do not fit); a radix select over digits
+ * of 11, 11 and 10 bits, the CTAs' histograms added over distributed shared memory, finds
+ * the key of the last token kept and how many of its equals stay, and one ordered pass with
+ * a block scan writes the indices.  4 bytes per token are read from HBM once; what bounds it
+ * is the latency of its dozen dependent steps.
  *
  * move_kernel, in place.  Row j of the result comes from row kept[j] >= j, and kept is
  * ascending, so a CTA that goes through j in ascending batches may overwrite [j0, j0 + n)
  * as soon as its own loads of that batch are done: every later source lies at j0 + n or
- * above.  One barrier per batch orders the two, and the next batch's loads are in flight
- * across it.  Different byte columns of the rows never meet, so (K or V) x column ranges
- * x (sequence, KV head) are independent CTAs: the rule below takes as few columns as fill
- * the SMs.  Rows before the first evicted one are not touched.  Bound by reading and
- * writing the moved rows.
+ * above.  So loads run ahead through a ring of asynchronous copies to shared memory (96 KB
+ * in flight per CTA) and one barrier per batch orders its stores behind its loads; the rows'
+ * places are looked up 2048 at a time, so no load waits for an index.  Different byte
+ * columns of the rows never meet, so (K or V) x column ranges x (sequence, KV head) are
+ * independent CTAs.  Rows before the first evicted one are not touched.  Bound by reading
+ * and writing the moved rows.
  */
 #include <cuda_runtime.h>
 #include <math.h>
@@ -36,10 +39,15 @@ namespace pgqa {
 namespace evict {
 
 constexpr int kSelThreads = 1024;
-constexpr int kMoveThreads = 256;
-constexpr int kMoveDepth = 8;          // 16-byte pieces a thread holds per batch
 constexpr int kBins = 2048;
-constexpr int kMaxKeys = 48 * 1024;    // keys held in shared memory (192 KB)
+constexpr int kMaxGroups = 12 * 1024;  // groups of four keys held in shared memory (192 KB)
+constexpr int kMaxCluster = 8;
+
+constexpr int kMoveThreads = 256;
+constexpr int kMovePieces = 4;         // 16-byte pieces of a thread per batch
+constexpr int kMoveStages = 6;         // batches in the ring
+constexpr int kMoveRows = 2048;        // rows looked up at a time
+constexpr int kMoveSmem = kMoveStages * kMoveThreads * kMovePieces * 16 + 2 * kMoveRows * 4;
 
 struct Params {
     void *k_cache, *v_cache;
@@ -50,7 +58,8 @@ struct Params {
     int32_t* err;
     int64_t bt_stride, cap_tokens;
     int32_t Hkv, P, page_shift, num_pages, keep, sinks, recent;
-    int32_t smem_keys;               // keys that fit in the launch's shared memory
+    int32_t smem_groups;             // groups of four keys that fit in the launch's shared memory
+    int32_t cluster;                 // CTAs per (sequence, KV head) of the select
     int32_t row_pieces, col_pieces;  // 16-byte pieces in a row, and in one CTA's columns
     int32_t cols;                    // column ranges per row
 };
@@ -71,110 +80,190 @@ __device__ __forceinline__ uint32_t key_of(float w) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+/* Cluster barrier and a load from another CTA's shared memory. */
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t v;
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+        : "=r"(v)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
+
+/* Sum of v over the threads before this one, and over all, of a 1024-thread block; two
+ * 16-bit counts packed in a word pass through as long as neither total reaches 2^16. */
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int lane, int warp, uint32_t& total) {
+    uint32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    __syncthreads();  // the last use of wsum is over
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    uint32_t ws = wsum[lane];
+    const uint32_t own = ws;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, ws, o);
+        if (lane >= o) ws += u;
+    }
+    total = __shfl_sync(0xffffffffu, ws, 31);
+    return incl - v + __shfl_sync(0xffffffffu, ws - own, warp);
+}
+
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
-    extern __shared__ uint32_t keys[];
+    extern __shared__ uint4 keys[];
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t wsum[32];
-    __shared__ uint32_t found[2];  // the digit of the last kept key, and how many above it
+    __shared__ uint32_t found[2];   // the digit of the last kept key, and how many lie above it
+    __shared__ uint32_t counts[2];  // this CTA's tokens above the last kept key, and equal to it
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int32_t b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
+    const int32_t C = p.cluster, item = blockIdx.x / C, rank = blockIdx.x - item * C;
+    const int32_t b = item / p.Hkv, h = item - b * p.Hkv;
     const int32_t L0 = __ldg(p.seq_lens + b);
     const int32_t L = length_of(p, b);
-    if (h == 0 && tid == 0) {
+    if (h == 0 && tid == 0 && rank == 0) {
         if (L != L0) atomicOr(p.err, kDevErrBadSeqlen);
         p.new_lens[b] = min(L, p.keep);
     }
-    int32_t* kept = p.kept + (int64_t)blockIdx.x * p.keep;
+    int32_t* kept = p.kept + (int64_t)item * p.keep;
+    const int t_all = rank * kSelThreads + tid, n_all = C * kSelThreads;
     if (L <= p.keep) {
-        for (int j = tid; j < p.keep; j += kSelThreads) kept[j] = j < L ? j : -1;
+        for (int j = t_all; j < p.keep; j += n_all) kept[j] = j < L ? j : -1;
         return;
     }
-    const int32_t M = L - p.sinks - p.recent;            // candidates
-    const int32_t m = p.keep - p.sinks - p.recent;       // of which m < M stay
-    for (int j = tid; j < p.sinks; j += kSelThreads) kept[j] = j;
-    for (int j = tid; j < p.recent; j += kSelThreads) kept[p.sinks + m + j] = L - p.recent + j;
+    const int32_t lo = p.sinks, hi = L - p.recent;       // candidates [lo, hi)
+    const int32_t m = p.keep - p.sinks - p.recent;       // of which m < hi - lo stay
+    for (int j = t_all; j < p.sinks; j += n_all) kept[j] = j;
+    for (int j = t_all; j < p.recent; j += n_all) kept[p.sinks + m + j] = L - p.recent + j;
     if (m == 0) return;
+    // this CTA's groups of four tokens (a group never crosses a page): [g0, g1)
+    const int32_t ga = lo >> 2, gn = ((hi + 3) >> 2) - ga, per = (gn + C - 1) / C;
+    const int32_t g0 = ga + min(gn, rank * per), g1 = ga + min(gn, (rank + 1) * per);
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
-    const bool held = M <= p.smem_keys;
+    const bool held = per <= p.smem_groups;
     bool bad = false;
-    auto load_key = [&](int32_t i) -> uint32_t {
-        const int32_t tok = p.sinks + i;
-        const int32_t page = page_of(p, tok);
+    auto load_group = [&](int32_t g) -> uint4 {
+        const int32_t tok = 4 * g, page = page_of(p, tok);
         const int32_t pid = __ldg(bt + page);
         if ((uint32_t)pid >= (uint32_t)p.num_pages) {
             bad = true;
-            return 0;
+            return make_uint4(0, 0, 0, 0);
         }
-        return key_of(__ldg(p.weights + ((int64_t)pid * p.Hkv + h) * p.P + (tok - page * p.P)));
+        const float4 w = __ldg(reinterpret_cast<const float4*>(p.weights + ((int64_t)pid * p.Hkv + h) * p.P +
+                                                               (tok - page * p.P)));
+        return make_uint4(key_of(w.x), key_of(w.y), key_of(w.z), key_of(w.w));
     };
-    if (held) {
-        // four loads in flight per thread
-        for (int32_t i0 = tid; i0 < M; i0 += 4 * kSelThreads) {
-            uint32_t k[4];
+    auto group_at = [&](int32_t g) -> uint4 { return held ? keys[g - g0] : load_group(g); };
+    // f(key, token) for the candidates of a group
+    auto each = [&](int32_t g, const uint4& k, auto&& f) {
+        const uint32_t v[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-            for (int u = 0; u < 4; ++u) k[u] = i0 + u * kSelThreads < M ? load_key(i0 + u * kSelThreads) : 0;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (i0 + u * kSelThreads < M) keys[i0 + u * kSelThreads] = k[u];
-        }
-        __syncthreads();
-    }
-    auto key_at = [&](int32_t i) -> uint32_t { return held ? keys[i] : load_key(i); };
+        for (int u = 0; u < 4; ++u)
+            if (4 * g + u >= lo && 4 * g + u < hi) f(v[u], u);
+    };
 
     uint32_t prefix = 0, mask = 0;  // digits fixed so far
     uint32_t need = (uint32_t)m;    // tokens still to take among those that match them
-    bool all = false;               // every match of `prefix` stays
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-        const int bits = pass == 2 ? 10 : 11;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
         for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
         __syncthreads();
-        for (int32_t i = tid; i < M; i += kSelThreads) {
-            const uint32_t k = key_at(i);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-        }
-        __syncthreads();
-        // counts from the top: thread t owns bins 2047 - 2 t and 2046 - 2 t
-        const uint32_t h0 = hist[kBins - 1 - 2 * tid], h1 = hist[kBins - 2 - 2 * tid];
-        uint32_t incl = h0 + h1;
+        auto count = [&](int32_t g, const uint4& k) {
+            each(g, k, [&](uint32_t key, int) {
+                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digits], 1u);
+            });
+        };
+        if (pass == 0 && held) {
+            // the keys come in, four groups in flight per thread, and are counted on the way
+            for (int32_t gb = g0 + tid; gb < g1; gb += 4 * kSelThreads) {
+                uint4 k[4];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
+                for (int u = 0; u < 4; ++u)
+                    if (gb + u * kSelThreads < g1) k[u] = load_group(gb + u * kSelThreads);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (gb + u * kSelThreads < g1) {
+                        keys[gb + u * kSelThreads - g0] = k[u];
+                        count(gb + u * kSelThreads, k[u]);
+                    }
+                }
+            }
+        } else {
+            for (int32_t g = g0 + tid; g < g1; g += kSelThreads) count(g, group_at(g));
         }
-        if (lane == 31) wsum[warp] = incl;
-        __syncthreads();
-        uint32_t above = incl - h0 - h1;
-        for (int w = 0; w < warp; ++w) above += wsum[w];
+        // counts from the top: thread t owns bins 2047 - 2 t and 2046 - 2 t, of all CTAs
+        uint32_t h0, h1;
+        if (C > 1) {
+            cluster_sync();
+            h0 = h1 = 0;
+            const uint32_t a = ptx::smem_u32(hist) + 4u * (kBins - 2 - 2 * tid);
+            for (int r = 0; r < C; ++r) {
+                h1 += ld_cluster(a, (uint32_t)r);
+                h0 += ld_cluster(a + 4u, (uint32_t)r);
+            }
+        } else {
+            __syncthreads();
+            h0 = hist[kBins - 1 - 2 * tid];
+            h1 = hist[kBins - 2 - 2 * tid];
+        }
+        uint32_t total;
+        const uint32_t above = block_scan(h0 + h1, wsum, lane, warp, total);
         if (above < need && need <= above + h0) {
             found[0] = (uint32_t)(kBins - 1 - 2 * tid);
-            found[1] = above;
+            found[1] = above | (h0 == need - above ? 0x80000000u : 0u);
         } else if (above + h0 < need && need <= above + h0 + h1) {
             found[0] = (uint32_t)(kBins - 2 - 2 * tid);
-            found[1] = above + h0;
+            found[1] = (above + h0) | (h1 == need - above - h0 ? 0x80000000u : 0u);
         }
-        __syncthreads();
-        const uint32_t digit = found[0];
-        need -= found[1];
+        if (C > 1) cluster_sync();  // the other CTAs have read this one's histogram
+        else __syncthreads();
+        const uint32_t digit = found[0], over = found[1];
+        need -= over & 0x7fffffffu;
         prefix |= digit << shift;
-        mask |= ((1u << bits) - 1) << shift;
-        all = hist[digit] == need;
-        if (all) break;
-        __syncthreads();
+        mask |= digits << shift;
+        if (over >> 31) break;  // every token that matches the prefix stays
     }
     // kept: keys above the prefix (under its mask), and the first `need` that match it
-    int32_t base = p.sinks;
-    uint32_t eq_before = 0;
-    for (int32_t i0 = 0; i0 < M; i0 += 4 * kSelThreads) {
+    uint32_t gt_before = 0, eq_before = 0;  // in the tokens before
+    if (C > 1) {
+        uint32_t gt = 0, eq = 0;
+        for (int32_t g = g0 + tid; g < g1; g += kSelThreads)
+            each(g, group_at(g), [&](uint32_t key, int) {
+                gt += (key & mask) > prefix;
+                eq += (key & mask) == prefix;
+            });
+        if (tid < 2) counts[tid] = 0;
+        __syncthreads();
+        gt = __reduce_add_sync(0xffffffffu, gt);
+        eq = __reduce_add_sync(0xffffffffu, eq);
+        if (lane == 0) {
+            atomicAdd(&counts[0], gt);
+            atomicAdd(&counts[1], eq);
+        }
+        cluster_sync();
+        for (int r = 0; r < rank; ++r) {
+            gt_before += ld_cluster(ptx::smem_u32(counts), (uint32_t)r);
+            eq_before += ld_cluster(ptx::smem_u32(counts) + 4u, (uint32_t)r);
+        }
+        cluster_sync();  // no CTA leaves while another reads its counts
+    }
+    for (int32_t gb = g0; gb < g1; gb += kSelThreads) {
+        const int32_t g = gb + tid;
         uint32_t cnt = 0, flags = 0;  // (above | equal << 16) of this thread's four tokens
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int32_t i = i0 + 4 * tid + u;
-            if (i < M) {
-                const uint32_t k = key_at(i) & mask;
+        if (g < g1)
+            each(g, group_at(g), [&](uint32_t key, int u) {
+                const uint32_t k = key & mask;
                 if (k > prefix) {
                     cnt += 1;
                     flags |= 1u << u;
@@ -182,39 +271,23 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
                     cnt += 0x10000u;
                     flags |= 16u << u;
                 }
-            }
-        }
-        uint32_t incl = cnt;  // at most 4096 of each kind: no carry between the halves
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-        }
-        __syncthreads();
-        if (lane == 31) wsum[warp] = incl;
-        __syncthreads();
-        uint32_t before = incl - cnt, total = 0;
-        for (int w = 0; w < 32; ++w) {
-            const uint32_t v = wsum[w];
-            if (w < warp) before += v;
-            total += v;
-        }
-        uint32_t gt = before & 0xffffu, eq = eq_before + (before >> 16);
-        const uint32_t eq0 = eq_before < need ? eq_before : need;  // equals already taken in `base`
+            });
+        uint32_t total;
+        const uint32_t before = block_scan(cnt, wsum, lane, warp, total);  // at most 4096 of each
+        uint32_t gt = gt_before + (before & 0xffffu), eq = eq_before + (before >> 16);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int32_t tok = p.sinks + i0 + 4 * tid + u;
-            const uint32_t taken = (eq < need ? eq : need) - eq0;
+            const uint32_t at = (uint32_t)p.sinks + gt + (eq < need ? eq : need);
             if (flags & (1u << u)) {
-                kept[base + gt + taken] = tok;
+                kept[at] = 4 * g + u;
                 ++gt;
             } else if (flags & (16u << u)) {
-                if (eq < need) kept[base + gt + taken] = tok;
+                if (eq < need) kept[at] = 4 * g + u;
                 ++eq;
             }
         }
+        gt_before += total & 0xffffu;
         eq_before += total >> 16;
-        base += (int32_t)((total & 0xffffu) + (eq_before < need ? eq_before : need) - eq0);
     }
     if (bad) atomicOr(p.err, kDevErrBadPage);
 }
@@ -231,6 +304,7 @@ __device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, i
 }
 
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
+    extern __shared__ uint4 ring[];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int tid = threadIdx.x;
@@ -244,7 +318,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
         const bool in_place = p.weights_out == p.weights;
         const int32_t n = min(L, p.keep);
         if (in_place && L <= p.keep) return;
-        constexpr int kU = 4;
+        constexpr int kU = 8;
         for (int32_t j0 = 0; j0 < n; j0 += kU * kMoveThreads) {
             float v[kU];
             int64_t dst[kU];
@@ -273,54 +347,80 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
     if (L <= p.keep) return;
     uint4* pool = static_cast<uint4*>(part < p.cols ? p.k_cache : p.v_cache);
     const int col = (part < p.cols ? part : part - p.cols) * p.col_pieces;
-    const int piece = col + tid % p.col_pieces, r0 = tid / p.col_pieces;
+    const int r0 = tid / p.col_pieces;
     const int rows = kMoveThreads / p.col_pieces;  // rows that the CTA covers at a time
-    const int32_t n = p.keep, batch = rows * kMoveDepth;
+    pool += (int64_t)h * p.row_pieces + col + tid % p.col_pieces;
+    const int64_t pitch = (int64_t)p.Hkv * p.row_pieces;
+    const int32_t n = p.keep, batch = rows * kMovePieces;
+    int32_t* src_slot = reinterpret_cast<int32_t*>(ring + kMoveStages * kMoveThreads * kMovePieces);
+    int32_t* dst_slot = src_slot + kMoveRows;
     // rows that stay where they are form a prefix; skip whole strides of it
     const int32_t stride = (n + kMoveThreads - 1) / kMoveThreads;
     const bool still = tid * stride < n && __ldg(kept + tid * stride) == tid * stride;
     const int32_t fixed = __syncthreads_count(still);
-    int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0;
-    uint4 v[kMoveDepth];
-    int64_t dst[kMoveDepth];
-    auto load = [&](int32_t at, uint4 (&w)[kMoveDepth], int64_t (&d)[kMoveDepth]) {
-        int64_t s[kMoveDepth];
+    for (int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0; j0 < n; j0 += kMoveRows) {
+        const int32_t here = min(kMoveRows, n - j0);
+        __syncthreads();
+        int32_t from[kMoveRows / kMoveThreads];
 #pragma unroll
-        for (int u = 0; u < kMoveDepth; ++u) {
-            const int32_t j = at + u * rows + r0;
-            d[u] = -1;
-            s[u] = -1;
-            if (j < n) {
-                const int32_t src = __ldg(kept + j);
-                if (src != j) {
+        for (int u = 0; u < kMoveRows / kMoveThreads; ++u) {
+            const int32_t i = u * kMoveThreads + tid;
+            from[u] = i < here ? __ldg(kept + j0 + i) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kMoveRows / kMoveThreads; ++u) {
+            const int32_t i = u * kMoveThreads + tid;
+            if (i < here) {
+                int32_t s = -1, d = -1;
+                if (from[u] != j0 + i) {
                     int32_t sp, dp;
-                    const int32_t ss = slot_of(p, bt, src, sp), ds = slot_of(p, bt, j, dp);
-                    if (ss >= 0 && ds >= 0) {
-                        s[u] = (((int64_t)sp * p.P + ss) * p.Hkv + h) * p.row_pieces + piece;
-                        d[u] = (((int64_t)dp * p.P + ds) * p.Hkv + h) * p.row_pieces + piece;
+                    s = slot_of(p, bt, from[u], sp);
+                    d = slot_of(p, bt, j0 + i, dp);
+                    if (s >= 0 && d >= 0) {
+                        s += sp * p.P;
+                        d += dp * p.P;
+                    } else {
+                        s = -1;
                     }
                 }
+                src_slot[i] = s;
+                dst_slot[i] = d;
             }
         }
-#pragma unroll
-        for (int u = 0; u < kMoveDepth; ++u)
-            if (s[u] >= 0) w[u] = __ldcg(pool + s[u]);
-    };
-    load(j0, v, dst);
-    for (; j0 < n; j0 += batch) {
-        uint4 vn[kMoveDepth];
-        int64_t dn[kMoveDepth];
-        // every load of this batch is back before any of its rows is overwritten
-        load(j0 + batch, vn, dn);
         __syncthreads();
+        const int32_t batches = (here + batch - 1) / batch;
+        auto fetch = [&](int32_t k) {
+            if (k < batches) {
+                uint4* to = ring + (k % kMoveStages) * (kMoveThreads * kMovePieces) + tid;
 #pragma unroll
-        for (int u = 0; u < kMoveDepth; ++u)
-            if (dst[u] >= 0) pool[dst[u]] = v[u];
+                for (int u = 0; u < kMovePieces; ++u) {
+                    const int32_t i = k * batch + u * rows + r0;
+                    const int32_t s = i < here ? src_slot[i] : -1;
+                    if (s >= 0)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                         ptx::smem_u32(to + u * kMoveThreads)),
+                                     "l"(pool + s * pitch)
+                                     : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
 #pragma unroll
-        for (int u = 0; u < kMoveDepth; ++u) {
-            v[u] = vn[u];
-            dst[u] = dn[u];
+        for (int k = 0; k < kMoveStages - 1; ++k) fetch(k);
+        for (int32_t k = 0; k < batches; ++k) {
+            fetch(k + kMoveStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kMoveStages - 1) : "memory");
+            // every load of this batch is back before any of its rows is overwritten; a
+            // thread stores what it loaded itself
+            __syncthreads();
+            const uint4* at = ring + (k % kMoveStages) * (kMoveThreads * kMovePieces) + tid;
+#pragma unroll
+            for (int u = 0; u < kMovePieces; ++u) {
+                const int32_t i = k * batch + u * rows + r0;
+                if (i < here && src_slot[i] >= 0) pool[dst_slot[i] * pitch] = at[u * kMoveThreads];
+            }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
 }
 
@@ -336,9 +436,9 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
         a->recent > a->keep - a->sinks)
         return PGQA_ERR_BAD_SHAPE;
     if (a->new_lens == a->seq_lens) return PGQA_ERR_BAD_SHAPE;
-    if (a->batch_size * a->num_heads_k > INT32_MAX) return PGQA_ERR_UNSUPPORTED;
-    if (!host_aligned(a->k_cache, 16) || !host_aligned(a->v_cache, 16) || !host_aligned(a->weights, 4) ||
-        !host_aligned(a->weights_out, 4) || !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) ||
+    if (a->batch_size * a->num_heads_k > INT32_MAX / kMaxCluster) return PGQA_ERR_UNSUPPORTED;
+    if (!host_aligned(a->k_cache, 16) || !host_aligned(a->v_cache, 16) || !host_aligned(a->weights, 16) ||
+        !host_aligned(a->weights_out, 16) || !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) ||
         !host_aligned(a->kept, 4) || !host_aligned(a->new_lens, 4))
         return PGQA_ERR_MISALIGNED;
     int dev, sms, optin;
@@ -364,21 +464,26 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
     p.recent = (int32_t)a->recent;
     p.row_pieces = a->kv_format == 1 ? 8 : 16;
     const int64_t items = a->batch_size * a->num_heads_k;
-    int64_t hold = p.cap_tokens - p.sinks - p.recent;
-    if (hold > kMaxKeys) hold = kMaxKeys;
-    if (hold < 0) hold = 0;
-    if (hold * 4 > optin - 12 * 1024) hold = (optin - 12 * 1024) / 4;
-    p.smem_keys = (int32_t)hold;
-    static int done[kHostMaxDevices] = {0};
-    const int smem = (int)hold * 4;
+    // CTAs per pair: as many as fill the SMs, each with 4096 tokens or more by the capacity
+    p.cluster = 1;
+    while (p.cluster < kMaxCluster && items * 2 * p.cluster <= sms && p.cap_tokens / (2 * p.cluster) >= 4096)
+        p.cluster *= 2;
+    int64_t hold = (p.cap_tokens / 4 + p.cluster) / p.cluster + 1;
+    if (hold > kMaxGroups) hold = kMaxGroups;
+    if (hold * 16 > optin - 12 * 1024) hold = (optin - 12 * 1024) / 16;
+    p.smem_groups = (int32_t)hold;
+    static int done[kHostMaxDevices] = {0}, done_move[kHostMaxDevices] = {0};
+    const int smem = (int)hold * 16;
     if (smem > 32 * 1024 && (st = host_smem_limit(select_kernel, dev, smem, done)) != PGQA_OK) return st;
-    st = host_launch(select_kernel, dim3((unsigned)items), kSelThreads, (size_t)smem, stream, p);
+    st = host_launch(select_kernel, dim3((unsigned)(items * p.cluster)), kSelThreads, (size_t)smem, stream, p.cluster, p);
     if (st != PGQA_OK) return st;
     // column ranges of at least 64 bytes: as few as give every SM two CTAs
     p.cols = 1;
     while (items * 2 * p.cols < 2 * sms && p.row_pieces / (2 * p.cols) >= 4) p.cols *= 2;
     p.col_pieces = p.row_pieces / p.cols;
-    return host_launch(move_kernel, dim3((unsigned)items, (unsigned)(2 * p.cols + 1)), kMoveThreads, 0, stream, p);
+    if ((st = host_smem_limit(move_kernel, dev, kMoveSmem, done_move)) != PGQA_OK) return st;
+    return host_launch(move_kernel, dim3((unsigned)items, (unsigned)(2 * p.cols + 1)), kMoveThreads, kMoveSmem, stream,
+                       1, p);
 }
 
 }  // namespace evict

@@ -48,20 +48,27 @@ int host_smem_limit(K kernel, int dev, int bytes, int (&done)[kHostMaxDevices]) 
     return PGQA_OK;
 }
 
-/* One launch on `stream`, as a programmatic dependent: every kernel launched through here
+/* One launch on `stream`, in clusters of `cluster` CTAs, as a programmatic dependent: every kernel launched through here
  * executes griddepcontrol.wait in all of its CTAs before it touches memory. */
 template <typename K, typename... Args>
-int host_launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+int host_launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster,
+                const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = host_pdl() ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (cluster > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
     if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
         cudaGetLastError();
         return PGQA_ERR_CUDA;

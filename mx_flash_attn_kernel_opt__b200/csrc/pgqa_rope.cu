@@ -354,7 +354,7 @@ int entry(const pgqa_rope_args* a, cudaStream_t stream) {
     const int64_t ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
     if (ctas > INT32_MAX) return PGQA_ERR_UNSUPPORTED;
     auto kern = kv8 ? rope_append_kernel<true> : rope_append_kernel<false>;
-    return host_launch(kern, dim3((unsigned)ctas), kThreads, 0, stream, p);
+    return host_launch(kern, dim3((unsigned)ctas), kThreads, 0, stream, 1, p);
 }
 
 }  // namespace rope

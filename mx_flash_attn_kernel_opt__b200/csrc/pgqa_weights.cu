@@ -307,7 +307,7 @@ int launch(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
     auto kern = weights_kernel<KV8, NT>;
     int st = PGQA_OK;
     if (smem > 48 * 1024 && (st = host_smem_limit(kern, dev, smem, done)) != PGQA_OK) return st;
-    return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, p);
+    return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, 1, p);
 }
 
 template <bool KV8>

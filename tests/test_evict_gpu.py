@@ -52,6 +52,17 @@ def test_long_sequences(L, keep, cuda_device):
     run_and_check(make([L, 10], 2, 16, seed=L), keep, 4, min(64, keep // 2), cuda_device)
 
 
+def test_pairs_cut_by_clusters_and_pairs_left_alone(cuda_device):
+    """Few pairs with a large capacity: several CTAs select for one pair, some of them without
+    a candidate, and short sequences beside long ones."""
+    run_and_check(make([20000, 3, 8000, 1025], 1, 32, seed=20), 1024, 4, 300, cuda_device)
+    run_and_check(make([17000], 1, 16, "e4m3", seed=21), 16000, 0, 1, cuda_device)
+    k, v, w, bt, lens = make([33000, 40], 1, 16, seed=22)
+    w[:] = 1.0  # ties across the CTAs
+    run_and_check((k, v, w, bt, lens), 20000, 1, 2, cuda_device)
+    run_and_check((k, v, w, bt, lens), 37, 30, 7, cuda_device)
+
+
 def test_longer_than_shared_memory_holds(cuda_device):
     """More candidates than the select keeps in shared memory: keys are re-read."""
     g = torch.Generator().manual_seed(1)

@@ -79,8 +79,8 @@ def evict(**kw):
     (2, dict(struct_size=8)), (1, dict(k_cache=None)), (1, dict(weights=None)), (1, dict(kept=None)),
     (1, dict(new_lens=None)), (2, dict(keep=0)), (2, dict(keep=1 << 31)), (2, dict(sinks=-1)),
     (2, dict(recent=-1)), (2, dict(sinks=21)), (2, dict(sinks=10, recent=11)), (3, dict(kv_format=2)),
-    (4, dict(v_cache=A + 8)), (4, dict(kept=A + 2)), (2, dict(new_lens=A)), (3, dict(headdim=64)),
-    (3, dict(batch_size=1 << 20, num_heads_k=1 << 12)),
+    (4, dict(v_cache=A + 8)), (4, dict(kept=A + 2)), (4, dict(weights=A + 8)), (4, dict(weights_out=A + 4)), (2, dict(new_lens=A)), (3, dict(headdim=64)),
+    (3, dict(batch_size=1 << 20, num_heads_k=1 << 9)),
 ])
 def test_evict(status, kw):
     assert evict(**kw) == status
