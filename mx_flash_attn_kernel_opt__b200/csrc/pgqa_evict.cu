@@ -8,25 +8,25 @@
  * their indices go to kept[b, kv, :].  A sequence of L <= keep stays as it is (kept: 0 .. L-1,
  * then -1).
  *
- * Two launches:
+ * One launch, a cluster of 2, 4 or 8 CTAs per (sequence, KV head), in two phases.
  *
- * select_kernel, one CTA or one cluster of CTAs per (sequence, KV head), each CTA with a
- * contiguous range of the middle tokens.  Their weights become sortable 32-bit keys in
- * shared memory (or are re-read from L2 when they do not fit); a radix select over digits
- * of 11, 11 and 10 bits, the CTAs' histograms added over distributed shared memory, finds
- * the key of the last token kept and how many of its equals stay, and one ordered pass with
- * a block scan writes the indices.  4 bytes per token are read from HBM once; what bounds it
- * is the latency of its dozen dependent steps.
+ * Select: each CTA takes a contiguous range of the middle tokens.  Their weights become
+ * sortable 32-bit keys in shared memory (or are re-read from L2 when they do not fit); a
+ * radix select over digits of 11, 11 and 10 bits, the CTAs' histograms added over
+ * distributed shared memory, finds the key of the last token kept and how many of its equals
+ * stay, and one ordered pass with a block scan writes the indices.  4 bytes per token are
+ * read from HBM once; what bounds this phase is the latency of its dozen dependent steps,
+ * which the move of another pair on the same SM covers.
  *
- * move_kernel, in place.  Row j of the result comes from row kept[j] >= j, and kept is
- * ascending, so a CTA that goes through j in ascending batches may overwrite [j0, j0 + n)
- * as soon as its own loads of that batch are done: every later source lies at j0 + n or
- * above.  So loads run ahead through a ring of asynchronous copies to shared memory (96 KB
- * in flight per CTA) and one barrier per batch orders its stores behind its loads; the rows'
- * places are looked up 2048 at a time, so no load waits for an index.  Different byte
- * columns of the rows never meet, so (K or V) x column ranges x (sequence, KV head) are
- * independent CTAs.  Rows before the first evicted one are not touched.  Bound by reading
- * and writing the moved rows.
+ * Move, in place.  Row j of the result comes from row kept[j] >= j, and kept is ascending,
+ * so whoever goes through j in ascending batches may overwrite [j0, j0 + n) as soon as the
+ * loads of that batch are done: every later source lies at j0 + n or above.  So loads run
+ * ahead through a ring of asynchronous copies to shared memory (80 KB in flight per CTA) and
+ * one barrier per batch orders its stores behind its loads.  Half of the cluster's CTAs move
+ * K, half V; the rows of a batch are dealt out among them, whole rows each, and the barrier
+ * is then the cluster's.  The rows' places are looked up 2048 at a time, so no load waits
+ * for an index.  Rows before the first evicted one are not touched.  Bound by reading and
+ * writing the moved rows.
  */
 #include <cuda_runtime.h>
 #include <math.h>
@@ -38,16 +38,17 @@
 namespace pgqa {
 namespace evict {
 
-constexpr int kSelThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kBins = 2048;
-constexpr int kMaxGroups = 12 * 1024;  // groups of four keys held in shared memory (192 KB)
+constexpr int kBinsPerThread = kBins / kThreads;
 constexpr int kMaxCluster = 8;
-
-constexpr int kMoveThreads = 256;
-constexpr int kMovePieces = 4;         // 16-byte pieces of a thread per batch
-constexpr int kMoveStages = 6;         // batches in the ring
-constexpr int kMoveRows = 2048;        // rows looked up at a time
-constexpr int kMoveSmem = kMoveStages * kMoveThreads * kMovePieces * 16 + 2 * kMoveRows * 4;
+constexpr int kPieces = 2;             // 16-byte pieces of a thread per batch
+constexpr int kStages = 5;             // batches in the ring
+constexpr int kStagePieces = kThreads * kPieces;
+constexpr int kRows = 2048;            // rows looked up at a time by a CTA
+constexpr int kRingBytes = kStages * kStagePieces * 16;
+constexpr int kSmem = kRingBytes + 2 * kRows * 4;  // with the histogram, two CTAs per SM
+constexpr int kMaxGroups = kSmem / 16;             // groups of four keys held in it before the move
 
 struct Params {
     void *k_cache, *v_cache;
@@ -58,10 +59,8 @@ struct Params {
     int32_t* err;
     int64_t bt_stride, cap_tokens;
     int32_t Hkv, P, page_shift, num_pages, keep, sinks, recent;
-    int32_t smem_groups;             // groups of four keys that fit in the launch's shared memory
-    int32_t cluster;                 // CTAs per (sequence, KV head) of the select
-    int32_t row_pieces, col_pieces;  // 16-byte pieces in a row, and in one CTA's columns
-    int32_t cols;                    // column ranges per row
+    int32_t row_pieces;              // 16-byte pieces in a row
+    int32_t cluster;                 // CTAs per (sequence, KV head)
 };
 
 __device__ __forceinline__ int32_t page_of(const Params& p, int32_t tok) {
@@ -84,17 +83,20 @@ __device__ __forceinline__ uint32_t key_of(float w) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr, uint32_t rank) {
-    uint32_t v;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint4 ld_cluster(uint32_t addr, uint32_t rank) {
+    uint4 v;
     asm volatile(
-        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
-        : "=r"(v)
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
+        "ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
         : "r"(addr), "r"(rank)
         : "memory");
     return v;
 }
 
-/* Sum of v over the threads before this one, and over all, of a 1024-thread block; two
+/* Sum of v over the threads before this one, and over all, of a block; two
  * 16-bit counts packed in a word pass through as long as neither total reaches 2^16. */
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int lane, int warp, uint32_t& total) {
     uint32_t incl = v;
@@ -106,7 +108,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int l
     __syncthreads();  // the last use of wsum is over
     if (lane == 31) wsum[warp] = incl;
     __syncthreads();
-    uint32_t ws = wsum[lane];
+    uint32_t ws = lane < kThreads / 32 ? wsum[lane] : 0;
     const uint32_t own = ws;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -117,29 +119,27 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int l
     return incl - v + __shfl_sync(0xffffffffu, ws - own, warp);
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
-    extern __shared__ uint4 keys[];
-    __shared__ uint32_t hist[kBins];
+/* Slot of token `tok` in the pool's token order, or -1 for a bad page. */
+__device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, int32_t tok, int32_t& pid) {
+    const int32_t page = page_of(p, tok);
+    pid = __ldg(bt + page);
+    if ((uint32_t)pid >= (uint32_t)p.num_pages) {
+        atomicOr(p.err, kDevErrBadPage);
+        return -1;
+    }
+    return tok - page * p.P;
+}
+
+/* Writes kept[0, keep) of a sequence of L > keep tokens: C CTAs of a cluster together, each
+ * with the keys of its range in `keys`, or (C = 1) one CTA alone. */
+__device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32_t h, int32_t* kept, int C, int rank,
+                            uint4* keys) {
+    __shared__ __align__(16) uint32_t hist[kBins];
     __shared__ uint32_t wsum[32];
     __shared__ uint32_t found[2];   // the digit of the last kept key, and how many lie above it
-    __shared__ uint32_t counts[2];  // this CTA's tokens above the last kept key, and equal to it
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
+    __shared__ __align__(16) uint32_t counts[4];  // this CTA's tokens above the last kept key, and equal to it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int32_t C = p.cluster, item = blockIdx.x / C, rank = blockIdx.x - item * C;
-    const int32_t b = item / p.Hkv, h = item - b * p.Hkv;
-    const int32_t L0 = __ldg(p.seq_lens + b);
-    const int32_t L = length_of(p, b);
-    if (h == 0 && tid == 0 && rank == 0) {
-        if (L != L0) atomicOr(p.err, kDevErrBadSeqlen);
-        p.new_lens[b] = min(L, p.keep);
-    }
-    int32_t* kept = p.kept + (int64_t)item * p.keep;
-    const int t_all = rank * kSelThreads + tid, n_all = C * kSelThreads;
-    if (L <= p.keep) {
-        for (int j = t_all; j < p.keep; j += n_all) kept[j] = j < L ? j : -1;
-        return;
-    }
+    const int t_all = rank * kThreads + tid, n_all = C * kThreads;
     const int32_t lo = p.sinks, hi = L - p.recent;       // candidates [lo, hi)
     const int32_t m = p.keep - p.sinks - p.recent;       // of which m < hi - lo stay
     for (int j = t_all; j < p.sinks; j += n_all) kept[j] = j;
@@ -148,8 +148,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
     // this CTA's groups of four tokens (a group never crosses a page): [g0, g1)
     const int32_t ga = lo >> 2, gn = ((hi + 3) >> 2) - ga, per = (gn + C - 1) / C;
     const int32_t g0 = ga + min(gn, rank * per), g1 = ga + min(gn, (rank + 1) * per);
-    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
-    const bool held = per <= p.smem_groups;
+    const bool held = per <= kMaxGroups;
     bool bad = false;
     auto load_group = [&](int32_t g) -> uint4 {
         const int32_t tok = 4 * g, page = page_of(p, tok);
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
         const uint32_t digits = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
         __syncthreads();
         auto count = [&](int32_t g, const uint4& k) {
             each(g, k, [&](uint32_t key, int) {
@@ -186,45 +185,54 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
         };
         if (pass == 0 && held) {
             // the keys come in, four groups in flight per thread, and are counted on the way
-            for (int32_t gb = g0 + tid; gb < g1; gb += 4 * kSelThreads) {
+            for (int32_t gb = g0 + tid; gb < g1; gb += 4 * kThreads) {
                 uint4 k[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (gb + u * kSelThreads < g1) k[u] = load_group(gb + u * kSelThreads);
+                    if (gb + u * kThreads < g1) k[u] = load_group(gb + u * kThreads);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (gb + u * kSelThreads < g1) {
-                        keys[gb + u * kSelThreads - g0] = k[u];
-                        count(gb + u * kSelThreads, k[u]);
+                    if (gb + u * kThreads < g1) {
+                        keys[gb + u * kThreads - g0] = k[u];
+                        count(gb + u * kThreads, k[u]);
                     }
                 }
             }
         } else {
-            for (int32_t g = g0 + tid; g < g1; g += kSelThreads) count(g, group_at(g));
+            for (int32_t g = g0 + tid; g < g1; g += kThreads) count(g, group_at(g));
         }
-        // counts from the top: thread t owns bins 2047 - 2 t and 2046 - 2 t, of all CTAs
-        uint32_t h0, h1;
+        // counts of all CTAs from the top: thread t owns the bins from top down to
+        // top - kBinsPerThread + 1
+        const int top = kBins - 1 - kBinsPerThread * tid;
+        uint32_t c[kBinsPerThread] = {0, 0, 0, 0};
+        const uint32_t at = ptx::smem_u32(hist + top - 3);
+        auto take = [&](const uint4& v) {
+            c[0] += v.w;
+            c[1] += v.z;
+            c[2] += v.y;
+            c[3] += v.x;
+        };
         if (C > 1) {
             cluster_sync();
-            h0 = h1 = 0;
-            const uint32_t a = ptx::smem_u32(hist) + 4u * (kBins - 2 - 2 * tid);
-            for (int r = 0; r < C; ++r) {
-                h1 += ld_cluster(a, (uint32_t)r);
-                h0 += ld_cluster(a + 4u, (uint32_t)r);
-            }
+            uint4 v[kMaxCluster];
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) v[r] = r < C ? ld_cluster(at, (uint32_t)r) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) take(v[r]);
         } else {
             __syncthreads();
-            h0 = hist[kBins - 1 - 2 * tid];
-            h1 = hist[kBins - 2 - 2 * tid];
+            take(ptx::lds_u4(at));
         }
+        const uint32_t sum = (c[0] + c[1]) + (c[2] + c[3]);
         uint32_t total;
-        const uint32_t above = block_scan(h0 + h1, wsum, lane, warp, total);
-        if (above < need && need <= above + h0) {
-            found[0] = (uint32_t)(kBins - 1 - 2 * tid);
-            found[1] = above | (h0 == need - above ? 0x80000000u : 0u);
-        } else if (above + h0 < need && need <= above + h0 + h1) {
-            found[0] = (uint32_t)(kBins - 2 - 2 * tid);
-            found[1] = (above + h0) | (h1 == need - above - h0 ? 0x80000000u : 0u);
+        uint32_t above = block_scan(sum, wsum, lane, warp, total);
+#pragma unroll
+        for (int i = 0; i < kBinsPerThread; ++i) {
+            if (above < need && need <= above + c[i]) {
+                found[0] = (uint32_t)(top - i);
+                found[1] = above | (c[i] == need - above ? 0x80000000u : 0u);
+            }
+            above += c[i];
         }
         if (C > 1) cluster_sync();  // the other CTAs have read this one's histogram
         else __syncthreads();
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
     uint32_t gt_before = 0, eq_before = 0;  // in the tokens before
     if (C > 1) {
         uint32_t gt = 0, eq = 0;
-        for (int32_t g = g0 + tid; g < g1; g += kSelThreads)
+        for (int32_t g = g0 + tid; g < g1; g += kThreads)
             each(g, group_at(g), [&](uint32_t key, int) {
                 gt += (key & mask) > prefix;
                 eq += (key & mask) == prefix;
@@ -252,13 +260,17 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
             atomicAdd(&counts[1], eq);
         }
         cluster_sync();
-        for (int r = 0; r < rank; ++r) {
-            gt_before += ld_cluster(ptx::smem_u32(counts), (uint32_t)r);
-            eq_before += ld_cluster(ptx::smem_u32(counts) + 4u, (uint32_t)r);
+        uint4 v[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+            v[r] = r < rank ? ld_cluster(ptx::smem_u32(counts), (uint32_t)r) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+            gt_before += v[r].x;
+            eq_before += v[r].y;
         }
-        cluster_sync();  // no CTA leaves while another reads its counts
     }
-    for (int32_t gb = g0; gb < g1; gb += kSelThreads) {
+    for (int32_t gb = g0; gb < g1; gb += kThreads) {
         const int32_t g = gb + tid;
         uint32_t cnt = 0, flags = 0;  // (above | equal << 16) of this thread's four tokens
         if (g < g1)
@@ -292,113 +304,112 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const Params p) {
     if (bad) atomicOr(p.err, kDevErrBadPage);
 }
 
-/* Slot of token `tok` in the pool's token order, or -1 for a bad page. */
-__device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, int32_t tok, int32_t& pid) {
-    const int32_t page = page_of(p, tok);
-    pid = __ldg(bt + page);
-    if ((uint32_t)pid >= (uint32_t)p.num_pages) {
-        atomicOr(p.err, kDevErrBadPage);
-        return -1;
-    }
-    return tok - page * p.P;
-}
-
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const Params p) {
     extern __shared__ uint4 ring[];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int tid = threadIdx.x;
-    const int32_t b = blockIdx.x / p.Hkv, h = blockIdx.x - b * p.Hkv;
+    const int32_t C = p.cluster, item = blockIdx.x / C, rank = blockIdx.x - item * C;
+    const int32_t b = item / p.Hkv, h = item - b * p.Hkv;
+    const int32_t L0 = __ldg(p.seq_lens + b);
     const int32_t L = length_of(p, b);
-    const int32_t* kept = p.kept + (int64_t)blockIdx.x * p.keep;
+    const int32_t n = min(L, p.keep);
+    if (h == 0 && tid == 0 && rank == 0) {
+        if (L != L0) atomicOr(p.err, kDevErrBadSeqlen);
+        p.new_lens[b] = n;
+    }
+    int32_t* kept = p.kept + (int64_t)item * p.keep;
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
-    const int part = blockIdx.y;
-    if (part == 2 * p.cols) {
-        // the weights: one 4-byte element per token
-        const bool in_place = p.weights_out == p.weights;
-        const int32_t n = min(L, p.keep);
-        if (in_place && L <= p.keep) return;
-        constexpr int kU = 8;
-        for (int32_t j0 = 0; j0 < n; j0 += kU * kMoveThreads) {
+    const bool cut = L > p.keep;  // the same in all of the cluster, as is every count of a loop with a barrier
+    if (cut) {
+        // a pair of CTAs: each selects for itself (and writes the same indices), which costs
+        // less than meeting at every step; more of them divide the tokens
+        select_kept(p, bt, L, h, kept, C == 2 ? 1 : C, C == 2 ? 0 : rank, ring);
+        // kept is complete, every weight has been read, and nobody reads another's shared memory
+        cluster_sync();
+    } else {
+        for (int j = rank * kThreads + tid; j < p.keep; j += C * kThreads) kept[j] = j < L ? j : -1;
+    }
+    // the weights, one 4-byte element per token
+    const bool in_place = p.weights_out == p.weights;
+    if (cut || !in_place) {
+        constexpr int kU = 4;
+        for (int32_t j0 = 0; j0 < n; j0 += kU * C * kThreads) {
             float v[kU];
             int64_t dst[kU];
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                const int32_t j = j0 + u * kMoveThreads + tid;
+                const int32_t j = j0 + (u * C + rank) * kThreads + tid;
                 dst[u] = -1;
                 if (j < n) {
-                    const int32_t src = __ldg(kept + j);
+                    const int32_t src = cut ? __ldcg(kept + j) : j;
                     int32_t sp, dp;
                     const int32_t ss = slot_of(p, bt, src, sp), ds = slot_of(p, bt, j, dp);
                     if (ss >= 0 && ds >= 0 && !(in_place && src == j)) {
-                        // not __ldg: in place this array is written by the same kernel
                         v[u] = __ldcg(p.weights + ((int64_t)sp * p.Hkv + h) * p.P + ss);
                         dst[u] = ((int64_t)dp * p.Hkv + h) * p.P + ds;
                     }
                 }
             }
-            __syncthreads();
+            if (in_place) cluster_sync();
 #pragma unroll
             for (int u = 0; u < kU; ++u)
                 if (dst[u] >= 0) p.weights_out[dst[u]] = v[u];
         }
-        return;
     }
-    if (L <= p.keep) return;
-    uint4* pool = static_cast<uint4*>(part < p.cols ? p.k_cache : p.v_cache);
-    const int col = (part < p.cols ? part : part - p.cols) * p.col_pieces;
-    const int r0 = tid / p.col_pieces;
-    const int rows = kMoveThreads / p.col_pieces;  // rows that the CTA covers at a time
-    pool += (int64_t)h * p.row_pieces + col + tid % p.col_pieces;
+    if (!cut) return;
+    const int32_t S = C / 2, part = rank >> 1;  // CTAs that share the rows of K, or of V
+    uint4* pool = static_cast<uint4*>((rank & 1) == 0 ? p.k_cache : p.v_cache);
+    const int r0 = tid / p.row_pieces;
+    const int rows = kThreads / p.row_pieces;        // rows that the CTA covers at a time
+    const int32_t batch = rows * kPieces;            // and in a batch
+    pool += (int64_t)h * p.row_pieces + tid % p.row_pieces;
     const int64_t pitch = (int64_t)p.Hkv * p.row_pieces;
-    const int32_t n = p.keep, batch = rows * kMovePieces;
-    int32_t* src_slot = reinterpret_cast<int32_t*>(ring + kMoveStages * kMoveThreads * kMovePieces);
-    int32_t* dst_slot = src_slot + kMoveRows;
+    int32_t* src_slot = reinterpret_cast<int32_t*>(ring + kRingBytes / 16);
+    int32_t* dst_slot = src_slot + kRows;
     // rows that stay where they are form a prefix; skip whole strides of it
-    const int32_t stride = (n + kMoveThreads - 1) / kMoveThreads;
-    const bool still = tid * stride < n && __ldg(kept + tid * stride) == tid * stride;
+    const int32_t stride = (n + kThreads - 1) / kThreads;
+    const bool still = tid * stride < n && __ldcg(kept + tid * stride) == tid * stride;
     const int32_t fixed = __syncthreads_count(still);
-    for (int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0; j0 < n; j0 += kMoveRows) {
-        const int32_t here = min(kMoveRows, n - j0);
+    for (int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0; j0 < n; j0 += kRows * S) {
+        const int32_t here = min(kRows * S, n - j0);
+        // this CTA's i-th row is row (i / batch * S + part) * batch + i % batch of them
+        auto row_of = [&](int32_t i) { return (i / batch * S + part) * batch + i % batch; };
         __syncthreads();
-        int32_t from[kMoveRows / kMoveThreads];
+        int32_t from[kRows / kThreads];
 #pragma unroll
-        for (int u = 0; u < kMoveRows / kMoveThreads; ++u) {
-            const int32_t i = u * kMoveThreads + tid;
-            from[u] = i < here ? __ldg(kept + j0 + i) : 0;
+        for (int u = 0; u < kRows / kThreads; ++u) {
+            const int32_t r = row_of(u * kThreads + tid);
+            from[u] = r < here ? __ldcg(kept + j0 + r) : -1;
         }
 #pragma unroll
-        for (int u = 0; u < kMoveRows / kMoveThreads; ++u) {
-            const int32_t i = u * kMoveThreads + tid;
-            if (i < here) {
-                int32_t s = -1, d = -1;
-                if (from[u] != j0 + i) {
-                    int32_t sp, dp;
-                    s = slot_of(p, bt, from[u], sp);
-                    d = slot_of(p, bt, j0 + i, dp);
-                    if (s >= 0 && d >= 0) {
-                        s += sp * p.P;
-                        d += dp * p.P;
-                    } else {
-                        s = -1;
-                    }
+        for (int u = 0; u < kRows / kThreads; ++u) {
+            const int32_t i = u * kThreads + tid, r = row_of(i);
+            int32_t s = -1, d = -1;
+            if (from[u] >= 0 && from[u] != j0 + r) {
+                int32_t sp, dp;
+                s = slot_of(p, bt, from[u], sp);
+                d = slot_of(p, bt, j0 + r, dp);
+                if (s >= 0 && d >= 0) {
+                    s += sp * p.P;
+                    d += dp * p.P;
+                } else {
+                    s = -1;
                 }
-                src_slot[i] = s;
-                dst_slot[i] = d;
             }
+            src_slot[i] = s;
+            dst_slot[i] = d;
         }
         __syncthreads();
-        const int32_t batches = (here + batch - 1) / batch;
+        const int32_t batches = (here + batch * S - 1) / (batch * S);  // at most kRows / batch
         auto fetch = [&](int32_t k) {
             if (k < batches) {
-                uint4* to = ring + (k % kMoveStages) * (kMoveThreads * kMovePieces) + tid;
+                uint4* to = ring + (k % kStages) * kStagePieces + tid;
 #pragma unroll
-                for (int u = 0; u < kMovePieces; ++u) {
-                    const int32_t i = k * batch + u * rows + r0;
-                    const int32_t s = i < here ? src_slot[i] : -1;
+                for (int u = 0; u < kPieces; ++u) {
+                    const int32_t s = src_slot[k * batch + u * rows + r0];
                     if (s >= 0)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                         ptx::smem_u32(to + u * kMoveThreads)),
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(to + u * kThreads)),
                                      "l"(pool + s * pitch)
                                      : "memory");
                 }
@@ -406,18 +417,27 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const Params p) {
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int k = 0; k < kMoveStages - 1; ++k) fetch(k);
-        for (int32_t k = 0; k < batches; ++k) {
-            fetch(k + kMoveStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kMoveStages - 1) : "memory");
-            // every load of this batch is back before any of its rows is overwritten; a
-            // thread stores what it loaded itself
-            __syncthreads();
-            const uint4* at = ring + (k % kMoveStages) * (kMoveThreads * kMovePieces) + tid;
+        for (int k = 0; k < kStages; ++k) fetch(k);
+        // Every load of a batch, by all who share the rows, is back before any of its rows is
+        // overwritten; a thread stores what it loaded itself.  The stores come one batch
+        // later, so the wait for the others has a batch's time to pass.
+        for (int32_t k = 0; k <= batches; ++k) {
+            if (k < batches) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+                if (S > 1) cluster_arrive();
+            }
+            if (k > 0) {
+                const uint4* at = ring + ((k - 1) % kStages) * kStagePieces + tid;
 #pragma unroll
-            for (int u = 0; u < kMovePieces; ++u) {
-                const int32_t i = k * batch + u * rows + r0;
-                if (i < here && src_slot[i] >= 0) pool[dst_slot[i] * pitch] = at[u * kMoveThreads];
+                for (int u = 0; u < kPieces; ++u) {
+                    const int32_t i = (k - 1) * batch + u * rows + r0;
+                    if (src_slot[i] >= 0) pool[dst_slot[i] * pitch] = at[u * kThreads];
+                }
+                fetch(k - 1 + kStages);
+            }
+            if (k < batches) {
+                if (S > 1) cluster_wait();
+                else __syncthreads();
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -464,26 +484,14 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
     p.recent = (int32_t)a->recent;
     p.row_pieces = a->kv_format == 1 ? 8 : 16;
     const int64_t items = a->batch_size * a->num_heads_k;
-    // CTAs per pair: as many as fill the SMs, each with 4096 tokens or more by the capacity
-    p.cluster = 1;
-    while (p.cluster < kMaxCluster && items * 2 * p.cluster <= sms && p.cap_tokens / (2 * p.cluster) >= 4096)
+    // CTAs per pair: two (K and V), or as many more as still run at once, two per SM, as
+    // long as each has 1024 tokens or more by the capacity
+    p.cluster = 2;
+    while (p.cluster < kMaxCluster && items * p.cluster <= sms && p.cap_tokens / (2 * p.cluster) >= 1024)
         p.cluster *= 2;
-    int64_t hold = (p.cap_tokens / 4 + p.cluster) / p.cluster + 1;
-    if (hold > kMaxGroups) hold = kMaxGroups;
-    if (hold * 16 > optin - 12 * 1024) hold = (optin - 12 * 1024) / 16;
-    p.smem_groups = (int32_t)hold;
-    static int done[kHostMaxDevices] = {0}, done_move[kHostMaxDevices] = {0};
-    const int smem = (int)hold * 16;
-    if (smem > 32 * 1024 && (st = host_smem_limit(select_kernel, dev, smem, done)) != PGQA_OK) return st;
-    st = host_launch(select_kernel, dim3((unsigned)(items * p.cluster)), kSelThreads, (size_t)smem, stream, p.cluster, p);
-    if (st != PGQA_OK) return st;
-    // column ranges of at least 64 bytes: as few as give every SM two CTAs
-    p.cols = 1;
-    while (items * 2 * p.cols < 2 * sms && p.row_pieces / (2 * p.cols) >= 4) p.cols *= 2;
-    p.col_pieces = p.row_pieces / p.cols;
-    if ((st = host_smem_limit(move_kernel, dev, kMoveSmem, done_move)) != PGQA_OK) return st;
-    return host_launch(move_kernel, dim3((unsigned)items, (unsigned)(2 * p.cols + 1)), kMoveThreads, kMoveSmem, stream,
-                       1, p);
+    static int done[kHostMaxDevices] = {0};
+    if ((st = host_smem_limit(evict_kernel, dev, kSmem, done)) != PGQA_OK) return st;
+    return host_launch(evict_kernel, dim3((unsigned)(items * p.cluster)), kThreads, kSmem, stream, p.cluster, p);
 }
 
 }  // namespace evict
