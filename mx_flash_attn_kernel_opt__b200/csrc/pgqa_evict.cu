@@ -47,8 +47,10 @@ constexpr int kStages = 5;             // batches in the ring
 constexpr int kStagePieces = kThreads * kPieces;
 constexpr int kRows = 2048;            // rows looked up at a time by a CTA
 constexpr int kRingBytes = kStages * kStagePieces * 16;
-constexpr int kSmem = kRingBytes + 2 * kRows * 4;  // with the histogram, two CTAs per SM
-constexpr int kMaxGroups = kSmem / 16;             // groups of four keys held in it before the move
+constexpr int kSmem = kRingBytes + 2 * kRows * 4;  // so many that kCtasPerSm fit
+constexpr int kCtasPerSm = 1024 / kThreads;
+constexpr int kMaxGroups = kRingBytes / 16;        // groups of four keys held in the ring before the move
+static_assert(2 * kRows >= kBins, "the select's histogram lies in the rows' places");
 
 struct Params {
     void *k_cache, *v_cache;
@@ -83,7 +85,12 @@ __device__ __forceinline__ uint32_t key_of(float w) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+/* Arrival that orders no memory: for a barrier that only says that loads have returned.  A
+ * releasing arrival waits for the thread's stores to reach L2 as well (evict-long-e4m3: the
+ * first stall reason). */
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint4 ld_cluster(uint32_t addr, uint32_t rank) {
     uint4 v;
@@ -133,8 +140,7 @@ __device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, i
 /* Writes kept[0, keep) of a sequence of L > keep tokens: C CTAs of a cluster together, each
  * with the keys of its range in `keys`, or (C = 1) one CTA alone. */
 __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32_t h, int32_t* kept, int C, int rank,
-                            uint4* keys) {
-    __shared__ __align__(16) uint32_t hist[kBins];
+                            uint4* keys, uint32_t* hist) {
     __shared__ uint32_t wsum[32];
     __shared__ uint32_t found[2];   // the digit of the last kept key, and how many lie above it
     __shared__ __align__(16) uint32_t counts[4];  // this CTA's tokens above the last kept key, and equal to it
@@ -204,26 +210,32 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
         // counts of all CTAs from the top: thread t owns the bins from top down to
         // top - kBinsPerThread + 1
         const int top = kBins - 1 - kBinsPerThread * tid;
-        uint32_t c[kBinsPerThread] = {0, 0, 0, 0};
-        const uint32_t at = ptx::smem_u32(hist + top - 3);
-        auto take = [&](const uint4& v) {
-            c[0] += v.w;
-            c[1] += v.z;
-            c[2] += v.y;
-            c[3] += v.x;
-        };
-        if (C > 1) {
-            cluster_sync();
-            uint4 v[kMaxCluster];
+        uint32_t c[kBinsPerThread], sum = 0;
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) v[r] = r < C ? ld_cluster(at, (uint32_t)r) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kBinsPerThread; ++i) c[i] = 0;
+        if (C > 1) cluster_sync();
+        else __syncthreads();
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) take(v[r]);
-        } else {
-            __syncthreads();
-            take(ptx::lds_u4(at));
+        for (int q = 0; q < kBinsPerThread; q += 4) {
+            const uint32_t at = ptx::smem_u32(hist + top - q - 3);
+            auto take = [&](const uint4& v) {
+                c[q] += v.w;
+                c[q + 1] += v.z;
+                c[q + 2] += v.y;
+                c[q + 3] += v.x;
+            };
+            if (C > 1) {
+                uint4 v[kMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) v[r] = r < C ? ld_cluster(at, (uint32_t)r) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) take(v[r]);
+            } else {
+                take(ptx::lds_u4(at));
+            }
         }
-        const uint32_t sum = (c[0] + c[1]) + (c[2] + c[3]);
+#pragma unroll
+        for (int i = 0; i < kBinsPerThread; ++i) sum += c[i];
         uint32_t total;
         uint32_t above = block_scan(sum, wsum, lane, warp, total);
 #pragma unroll
@@ -304,7 +316,7 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
     if (bad) atomicOr(p.err, kDevErrBadPage);
 }
 
-__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Params p) {
     extern __shared__ uint4 ring[];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
@@ -324,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const Params p) {
     if (cut) {
         // a pair of CTAs: each selects for itself (and writes the same indices), which costs
         // less than meeting at every step; more of them divide the tokens
-        select_kept(p, bt, L, h, kept, C == 2 ? 1 : C, C == 2 ? 0 : rank, ring);
+        select_kept(p, bt, L, h, kept, C == 2 ? 1 : C, C == 2 ? 0 : rank, ring,
+                    reinterpret_cast<uint32_t*>(ring + kRingBytes / 16));
         // kept is complete, every weight has been read, and nobody reads another's shared memory
         cluster_sync();
     } else {
@@ -424,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const Params p) {
         for (int32_t k = 0; k <= batches; ++k) {
             if (k < batches) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-                if (S > 1) cluster_arrive();
+                if (S > 1) cluster_arrive_relaxed();
             }
             if (k > 0) {
                 const uint4* at = ring + ((k - 1) % kStages) * kStagePieces + tid;
@@ -484,10 +497,10 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
     p.recent = (int32_t)a->recent;
     p.row_pieces = a->kv_format == 1 ? 8 : 16;
     const int64_t items = a->batch_size * a->num_heads_k;
-    // CTAs per pair: two (K and V), or as many more as still run at once, two per SM, as
+    // CTAs per pair: two (K and V), or as many more as still run at once (kCtasPerSm), as
     // long as each has 1024 tokens or more by the capacity
     p.cluster = 2;
-    while (p.cluster < kMaxCluster && items * p.cluster <= sms && p.cap_tokens / (2 * p.cluster) >= 1024)
+    while (p.cluster < kMaxCluster && items * 2 * p.cluster <= kCtasPerSm * sms && p.cap_tokens / (2 * p.cluster) >= 1024)
         p.cluster *= 2;
     static int done[kHostMaxDevices] = {0};
     if ((st = host_smem_limit(evict_kernel, dev, kSmem, done)) != PGQA_OK) return st;
