@@ -53,6 +53,8 @@ class PgqaDecodeArgs(ctypes.Structure):
     ]
 
 
+# Argument structs of the operators around the decode.  serving.py packs them with `struct`
+# (a quarter of the time that setting ctypes fields takes); these mirrors name the fields.
 class PgqaRopeArgs(ctypes.Structure):
     """include/pgqa.h pgqa_rope_args (pgqa_rope_append)."""
     _fields_ = [
@@ -131,10 +133,10 @@ SIGNATURES = {
     "pgqa_append_kv_fp8": (ctypes.c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_void_p] * 2),
     "pgqa_decode_fp8": (ctypes.c_int, [c_void_p] * 8 + [c_int64] * 11 +
                         [c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "pgqa_rope_append": (ctypes.c_int, [ctypes.POINTER(PgqaRopeArgs), c_void_p]),
-    "pgqa_accumulate_weights": (ctypes.c_int, [ctypes.POINTER(PgqaWeightsArgs), c_void_p]),
-    "pgqa_evict": (ctypes.c_int, [ctypes.POINTER(PgqaEvictArgs), c_void_p]),
-    "pgqa_cross_attention": (ctypes.c_int, [ctypes.POINTER(PgqaCrossArgs), c_void_p]),
+    "pgqa_rope_append": (ctypes.c_int, [c_void_p, c_void_p]),
+    "pgqa_accumulate_weights": (ctypes.c_int, [c_void_p, c_void_p]),
+    "pgqa_evict": (ctypes.c_int, [c_void_p, c_void_p]),
+    "pgqa_cross_attention": (ctypes.c_int, [c_void_p, c_void_p]),
     "pgqa_cross_workspace_size": (c_size_t, [c_int64] * 7),
     "pgqa_workspace_size": (c_size_t, [c_int64] * 5),
     "pgqa_workspace_init": (ctypes.c_int, [c_void_p, c_size_t, c_void_p]),

@@ -11,10 +11,14 @@
  * and the division are in fp32 and the result is rounded once.  The slot's entries of the
  * attention-weight pool are set to zero, so that a page used again starts empty.
  *
- * Bound by HBM traffic (a few operations per byte): a warp carries one token and up to 16
- * of its Hq + 2 Hkv rows, 8 lanes per row with two 16-byte pieces each, all row loads
- * issued before the position and the table entries are known.  A lane's 8 pairs are the
- * same in every row it visits, so cosines and sines are read once per warp into registers.
+ * Bound by HBM traffic (a few operations per byte): a warp carries one token and up to 12
+ * of its Hq + 2 Hkv rows, 8 lanes per row with two 16-byte pieces each.  A lane's 8 pairs are
+ * the same in every row it visits, so cosines and sines are read once per warp into
+ * registers.  What a warp waits for is a chain of small loads (sequence, length, page), so
+ * the loads that depend on the token's number alone, rows and positions, go first, and 64
+ * registers a thread let 32 warps of an SM wait at once.  Prompts of 18,000 tokens with 28 + 8
+ * heads: 63.7 us (4.8 TB/s); with 16 rows per warp and 80 registers 69.0 us, with 8 rows per
+ * warp 75.7 us.
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -27,7 +31,7 @@ namespace pgqa {
 namespace rope {
 
 constexpr int kThreads = 128;
-constexpr int kRowsPerLane = 4;  // rows a lane visits: 16 rows of a token per warp
+constexpr int kRowsPerLane = 3;  // rows a lane visits: 12 rows of a token per warp
 
 struct Params {
     const __nv_bfloat16 *q, *k, *v;
@@ -84,7 +88,7 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
 }
 
 template <bool KV8>
-__global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p) {
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
@@ -92,17 +96,6 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
     const int64_t x = unit / p.blocks;
     if (x >= p.T) return;
     const int32_t block = (int32_t)(unit - x * p.blocks);
-    int32_t b;
-    int64_t s;
-    if (p.cu != nullptr) {
-        b = find_sequence(p.cu, p.B, x, lane);
-        s = x - __ldg(p.cu + b);
-        // in front of the first sequence or behind the last: left as it was
-        if (s < 0 || x >= __ldg(p.cu + b + 1)) return;
-    } else {
-        b = (int32_t)(x / p.S);
-        s = x - (int64_t)b * p.S;
-    }
     const int t = lane & 7, sub = lane >> 3;
     // a lane's two 16-byte pieces of a row
     const int turned = p.R >> 4;  // lanes that hold pairs
@@ -117,7 +110,9 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
         c0 = 2 * t;  // past the pairs: 2 * turned + 2 * (t - turned)
         c1 = c0 + 1;
     }
-    const int64_t sq = p.cu ? 0 : (int64_t)b, sx = p.cu ? x : s;
+    // what depends on the token's number alone: its rows and positions
+    const int32_t b_pad = p.cu ? 0 : (int32_t)(x / p.S);
+    const int64_t sx = x - (int64_t)b_pad * p.S;
     uint4 a[kRowsPerLane], e[kRowsPerLane];
     const int row0 = block * p.rows_per_block + sub;
     const int row_end = min(p.Hq + 2 * p.Hk, (block + 1) * p.rows_per_block);
@@ -126,44 +121,45 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
         const int r = row0 + 4 * i;
         if (r < row_end) {
             const __nv_bfloat16* src;
-            if (r < p.Hq) src = p.q + sq * p.qs[0] + sx * p.qs[1] + r * p.qs[2];
-            else if (r < p.Hq + p.Hk) src = p.k + sq * p.ks[0] + sx * p.ks[1] + (r - p.Hq) * p.ks[2];
-            else src = p.v + sq * p.vs[0] + sx * p.vs[1] + (r - p.Hq - p.Hk) * p.vs[2];
+            if (r < p.Hq) src = p.q + b_pad * p.qs[0] + sx * p.qs[1] + r * p.qs[2];
+            else if (r < p.Hq + p.Hk) src = p.k + b_pad * p.ks[0] + sx * p.ks[1] + (r - p.Hq) * p.ks[2];
+            else src = p.v + b_pad * p.vs[0] + sx * p.vs[1] + (r - p.Hq - p.Hk) * p.vs[2];
             const uint4* s4 = reinterpret_cast<const uint4*>(src);
             a[i] = __ldg(s4 + c0);
             e[i] = __ldg(s4 + c1);
         }
     }
-    // the token's place in the cache (page -1: no append for this token)
-    const int64_t tok = (p.seq_lens != nullptr ? (int64_t)__ldg(p.seq_lens + b) : 0) + s;
-    int32_t pid = -1, slot = 0;
-    if (p.Hk > 0) {
-        if (tok < s || tok >= p.cap_tokens) {  // a negative length, or past the table
-            if (lane == 0) atomicOr(p.err, kDevErrBadSeqlen);
-            return;
-        }
-        const int32_t page = p.page_shift >= 0 ? (int32_t)(tok >> p.page_shift) : (int32_t)(tok / p.P);
-        slot = (int32_t)(tok - (int64_t)page * p.P);
-        pid = __ldg(p.block_table + (int64_t)b * p.bt_stride + page);
-        if ((uint32_t)pid >= (uint32_t)p.num_pages) {
-            if (lane == 0) atomicOr(p.err, kDevErrBadPage);
-            return;
+    // positions of this lane's pairs [8 t, 8 t + 8): one, or one per pair
+    int32_t pos[8];
+    if (t < turned && p.positions != nullptr) {
+        pos[0] = __ldg(p.positions + (int64_t)p.axis[8 * t] * p.T + x);
+        if (!p.runs8) {
+#pragma unroll
+            for (int j = 1; j < 8; ++j) pos[j] = __ldg(p.positions + (int64_t)p.axis[8 * t + j] * p.T + x);
         }
     }
-    // cosines and sines of this lane's pairs [8 t, 8 t + 8)
+    int32_t b = b_pad;
+    int64_t s = sx;
+    if (p.cu != nullptr) {
+        b = find_sequence(p.cu, p.B, x, lane);
+        s = x - __ldg(p.cu + b);
+        // in front of the first sequence or behind the last: left as it was
+        if (s < 0 || x >= __ldg(p.cu + b + 1)) return;
+    }
+    const int64_t tok = (p.seq_lens != nullptr ? (int64_t)__ldg(p.seq_lens + b) : 0) + s;
+    // cosines and sines
     float c[8], n[8];
     bool bad = false;
     if (t < turned) {
-        auto row_of = [&](int ax) -> int64_t {
-            const int64_t pos = p.positions ? (int64_t)__ldg(p.positions + (int64_t)ax * p.T + x) : tok;
-            if (pos < 0 || pos >= p.table_rows) {
+        auto row_of = [&](int64_t q) -> int64_t {
+            if (q < 0 || q >= p.table_rows) {
                 bad = true;
                 return 0;
             }
-            return pos * (p.R >> 1);
+            return q * (p.R >> 1);
         };
-        if (p.runs8) {  // the eight pairs turn about one axis
-            const int64_t at = row_of(p.axis[8 * t]) + 8 * t;
+        if (p.runs8 || p.positions == nullptr) {  // the eight pairs turn about one axis
+            const int64_t at = row_of(p.positions ? (int64_t)pos[0] : tok) + 8 * t;
             if (p.table_bf16) {
                 unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + at)), c);
                 unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.sin) + at)), n);
@@ -177,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int64_t at = row_of(p.axis[8 * t + j]) + 8 * t + j;
+                const int64_t at = row_of(pos[j]) + 8 * t + j;
                 if (p.table_bf16) {
                     c[j] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.cos) + at));
                     n[j] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.sin) + at));
@@ -186,6 +182,21 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const Params p) {
                     n[j] = __ldg(static_cast<const float*>(p.sin) + at);
                 }
             }
+        }
+    }
+    // the token's place in the cache
+    int32_t pid = -1, slot = 0;
+    if (p.Hk > 0) {
+        if (tok < s || tok >= p.cap_tokens) {  // a negative length, or past the table
+            if (lane == 0) atomicOr(p.err, kDevErrBadSeqlen);
+            return;
+        }
+        const int32_t page = p.page_shift >= 0 ? (int32_t)(tok >> p.page_shift) : (int32_t)(tok / p.P);
+        slot = (int32_t)(tok - (int64_t)page * p.P);
+        pid = __ldg(p.block_table + (int64_t)b * p.bt_stride + page);
+        if ((uint32_t)pid >= (uint32_t)p.num_pages) {
+            if (lane == 0) atomicOr(p.err, kDevErrBadPage);
+            return;
         }
     }
     if (__any_sync(0xffffffffu, bad)) {  // nothing of this token is written

@@ -14,12 +14,17 @@
  * mma.sync A fragments: the order of the 128 dimensions inside the dot product is free as
  * long as q uses the same one, so lane (g, t) takes 16-byte pieces t, t + 4, ... of token
  * rows g and g + 8, whole 64-byte runs per row, and q rows are loaded by the same
- * addresses as B fragments.  A chunk's loads are issued one chunk ahead.  The four lanes
+ * addresses as B fragments.  Two to four chunks
+ * are held, one at work and the others in flight.  The four lanes
  * that share a token add their partial sums by shuffles, and the token's weight gets one
  * red.add: no other warp of the call adds to it (unless sequences share a page), so the
  * result does not depend on any order.
  *
- * e4m3 keys become bf16 in registers (exact: 4 significant bits), next to bf16 q.
+ * e4m3 keys become 16-bit numbers in registers, exactly (4 significant bits).  With q held
+ * over a unit they become f16, one conversion per pair, and q is turned into f16 once: each
+ * row times the power of two that brings its largest element to [2^14, 2^15), undone in
+ * fp32 (8 significant bits fit f16's 11; an element 2^28 times smaller than its row's largest
+ * is rounded to 2^-25).  With q re-read for every chunk the keys become bf16 instead.
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -58,19 +63,14 @@ struct Chunk {
 
 __device__ __forceinline__ uint32_t bf16x2_of(float2 f) { return ptx::pack_bf16x2(f.x, f.y); }
 
-/* Eight e4m3 (two words) -> four bf16x2, exact. */
-__device__ __forceinline__ void e4m3x8_to_bf16(uint32_t w0, uint32_t w1, uint32_t (&o)[4]) {
-    o[0] = bf16x2_of(ptx::e4m3x2_to_f32x2(w0 & 0xffffu));
-    o[1] = bf16x2_of(ptx::e4m3x2_to_f32x2(w0 >> 16));
-    o[2] = bf16x2_of(ptx::e4m3x2_to_f32x2(w1 & 0xffffu));
-    o[3] = bf16x2_of(ptx::e4m3x2_to_f32x2(w1 >> 16));
-}
-
 /* q fragments of one group of 8 rows, in the dimension order of the chunk's pieces. */
-template <bool KV8>
 struct QFrag {
     uint4 v[4];
 };
+
+__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t v, float up) {
+    return ptx::pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
+}
 
 /* Row r of the unit (b, kvh): query head r / Sq of the group, query token r % Sq. */
 __device__ __forceinline__ void row_of(const Params& p, int32_t b, int32_t kvh, int r, int64_t& qoff, int64_t& loff,
@@ -83,10 +83,11 @@ __device__ __forceinline__ void row_of(const Params& p, int32_t b, int32_t kvh, 
 }
 
 /* Per lane: the q pieces of row 8 j + g, and for rows 8 j + 2 t, 8 j + 2 t + 1 (its two
- * columns of the score tile) the negated log2-sum-exp and the number of tokens seen. */
-template <bool KV8>
-__device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t kvh, int32_t L, int j, int lane,
-                                           QFrag<KV8>& f, float (&nl)[2], int32_t (&lim)[2]) {
+ * columns of the score tile) the score's factor in log2 units, the negated log2-sum-exp and
+ * the number of tokens seen. */
+template <bool KV8, bool F16>
+__device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t kvh, int32_t L, float mul, int j,
+                                           int lane, QFrag& f, float (&ml)[2], float (&nl)[2], int32_t (&lim)[2]) {
     const int g = lane >> 2, t = lane & 3;
     int64_t qo, lo;
     int32_t tok;
@@ -102,9 +103,30 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.v[i] = make_uint4(0, 0, 0, 0);
     }
+    float down = 1.f;
+    if (F16) {
+        uint32_t mx = 0;  // largest magnitude of the row, as its bits
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w[4] = {f.v[i].x, f.v[i].y, f.v[i].z, f.v[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = max(mx, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+        }
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e = max(-100, min(100, 14 - ((int)(mx >> 23) - 127)));
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f.v[i] = make_uint4(bf16x2_to_f16x2(f.v[i].x, up), bf16x2_to_f16x2(f.v[i].y, up),
+                                bf16x2_to_f16x2(f.v[i].z, up), bf16x2_to_f16x2(f.v[i].w, up));
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int c = 8 * j + 2 * t + e;
+        ml[e] = mul;
+        if (F16) ml[e] *= __shfl_sync(0xffffffffu, down, 4 * (2 * t + e));
         nl[e] = 0.f;
         lim[e] = 0;
         if (c < p.rows) {
@@ -134,36 +156,73 @@ __device__ __forceinline__ void load_chunk(const Params& p, int32_t pid, int32_t
     }
 }
 
-/* Scores of the chunk's 16 tokens against 8 rows. */
-template <bool KV8>
-__device__ __forceinline__ void scores(const Chunk<KV8>& c, const QFrag<KV8>& f, float (&s)[4]) {
-    s[0] = s[1] = s[2] = s[3] = 0.f;
-    if (!KV8) {
+/* A chunk's A fragments of the eight 16-dimension steps. */
+struct AFrag {
+    uint32_t a[8][4];
+};
+
+/* e4m3 is converted once per chunk, not per group of rows: the conversions are what the SM
+ * does fewest of per clock here. */
+template <bool KV8, bool F16>
+__device__ __forceinline__ void fragments(const Chunk<KV8>& c, AFrag& f) {
 #pragma unroll
-        for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
-            ptx::mma_bf16_16816(s, c.lo[i].x, c.hi[i].x, c.lo[i].y, c.hi[i].y, f.v[i & 3].x, f.v[i & 3].y);
-            ptx::mma_bf16_16816(s, c.lo[i].z, c.hi[i].z, c.lo[i].w, c.hi[i].w, f.v[i & 3].z, f.v[i & 3].w);
-        }
-    } else {
+    for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
+        const uint32_t lo[4] = {c.lo[i].x, c.lo[i].y, c.lo[i].z, c.lo[i].w};
+        const uint32_t hi[4] = {c.hi[i].x, c.hi[i].y, c.hi[i].z, c.hi[i].w};
+        if (!KV8) {
 #pragma unroll
-        for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
-            uint32_t a[4], d[4];
-            e4m3x8_to_bf16(c.lo[i].x, c.lo[i].y, a);
-            e4m3x8_to_bf16(c.hi[i].x, c.hi[i].y, d);
-            ptx::mma_bf16_16816(s, a[0], d[0], a[1], d[1], f.v[2 * i].x, f.v[2 * i].y);
-            ptx::mma_bf16_16816(s, a[2], d[2], a[3], d[3], f.v[2 * i].z, f.v[2 * i].w);
-            e4m3x8_to_bf16(c.lo[i].z, c.lo[i].w, a);
-            e4m3x8_to_bf16(c.hi[i].z, c.hi[i].w, d);
-            ptx::mma_bf16_16816(s, a[0], d[0], a[1], d[1], f.v[2 * i + 1].x, f.v[2 * i + 1].y);
-            ptx::mma_bf16_16816(s, a[2], d[2], a[3], d[3], f.v[2 * i + 1].z, f.v[2 * i + 1].w);
+            for (int s = 0; s < 2; ++s) {
+                uint32_t(&a)[4] = f.a[(2 * i + s) & 7];
+                a[0] = lo[2 * s];
+                a[1] = hi[2 * s];
+                a[2] = lo[2 * s + 1];
+                a[3] = hi[2 * s + 1];
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                uint32_t(&a)[4] = f.a[(4 * i + s) & 7];
+                if (F16) {
+                    ptx::e4m3x4_to_f16(lo[s], a[0], a[2]);
+                    ptx::e4m3x4_to_f16(hi[s], a[1], a[3]);
+                } else {
+                    a[0] = bf16x2_of(ptx::e4m3x2_to_f32x2(lo[s] & 0xffffu));
+                    a[2] = bf16x2_of(ptx::e4m3x2_to_f32x2(lo[s] >> 16));
+                    a[1] = bf16x2_of(ptx::e4m3x2_to_f32x2(hi[s] & 0xffffu));
+                    a[3] = bf16x2_of(ptx::e4m3x2_to_f32x2(hi[s] >> 16));
+                }
+            }
         }
     }
 }
 
+/* Scores of the chunk's 16 tokens against 8 rows: two chains of four products each. */
+template <bool F16>
+__device__ __forceinline__ void scores(const AFrag& f, const QFrag& q, float (&s)[4]) {
+    float u[4] = {0.f, 0.f, 0.f, 0.f};
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint4 v = q.v[i >> 1];
+        const uint32_t b0 = (i & 1) ? v.z : v.x, b1 = (i & 1) ? v.w : v.y;
+        float(&d)[4] = (i & 1) ? u : s;
+        if (F16) ptx::mma_f16_16816(d, f.a[i][0], f.a[i][1], f.a[i][2], f.a[i][3], b0, b1);
+        else ptx::mma_bf16_16816(d, f.a[i][0], f.a[i][1], f.a[i][2], f.a[i][3], b0, b1);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] += u[e];
+}
+
+/* CTAs of 8 warps on an SM: one where the q fragments of more than 8 rows (32 registers per
+ * 16 rows) would not leave room for the chunks in flight otherwise. */
+__host__ __device__ constexpr int ctas_per_sm(int NT) { return NT >= 2 ? 1 : 2; }
+/* Chunks held by a warp: the one at work and those in flight. */
+__host__ __device__ constexpr int depth(bool KV8, int NT) { return NT >= 2 ? (KV8 ? 4 : 3) : (NT == 1 && KV8 ? 3 : 2); }
+
 /* NT > 0: that many groups of 8 rows, their q fragments held in registers over a unit;
  * NT = 0: any number, the fragments re-read (from L1) for every chunk. */
 template <bool KV8, int NT>
-__global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(const Params p) {
     extern __shared__ uint32_t pre[];  // chunks of the sequences before b, [B + 1]
     __shared__ uint32_t wsum[kWarps];
     ptx::griddep_wait();
@@ -214,6 +273,8 @@ __global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
     int32_t kvh = (int32_t)(in / n), c = (int32_t)(in - (int64_t)kvh * n);
     const int t = lane & 3, g = lane >> 2;
     constexpr int kHeld = NT > 0 ? NT : 1;
+    constexpr bool F16 = KV8 && NT > 0;
+    constexpr int D = depth(KV8, NT);
     const int groups = (p.rows + 7) / 8;
 
     while (cur < end) {
@@ -223,12 +284,12 @@ __global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
         const int32_t L = (int32_t)(L64 > p.cap_tokens ? p.cap_tokens : L64);
         const float ks = (KV8 && p.k_scale) ? __ldg(p.k_scale + kvh) : 1.f;
         const float mul = p.scale_log2 * ks;
-        QFrag<KV8> qf[kHeld];
-        float nl[kHeld][2];
+        QFrag qf[kHeld];
+        float ml[kHeld][2], nl[kHeld][2];
         int32_t lim[kHeld][2];
         if (NT > 0) {
 #pragma unroll
-            for (int j = 0; j < kHeld; ++j) load_group<KV8>(p, b, kvh, L, j, lane, qf[j], nl[j], lim[j]);
+            for (int j = 0; j < kHeld; ++j) load_group<KV8, F16>(p, b, kvh, L, mul, j, lane, qf[j], ml[j], nl[j], lim[j]);
         }
         const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
         auto page_of = [&](int32_t chunk, int32_t& pid, int32_t& slot) {
@@ -243,39 +304,40 @@ __global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
             pid = 0;  // read, not added to
             return false;
         };
-        Chunk<KV8> k;
-        int32_t pid, slot, npid = 0, nslot = 0;
-        page_of(c, pid, slot);
-        bool ok = check(pid);
-        load_chunk<KV8>(p, pid, slot, kvh, lane, k);
-        if (c + 1 < ce) page_of(c + 1, npid, nslot);
-        for (; c < ce; ++c) {
-            Chunk<KV8> kn;
-            bool nok = false;
-            int32_t fpid = 0, fslot = 0;
-            if (c + 1 < ce) {
-                nok = check(npid);
-                load_chunk<KV8>(p, npid, nslot, kvh, lane, kn);
-                if (c + 2 < ce) page_of(c + 2, fpid, fslot);
+        Chunk<KV8> ring[D];
+        int32_t pid[D], slot[D];
+        bool ok[D];
+#pragma unroll
+        for (int u = 0; u < D; ++u) {
+            if (c + u < ce) {
+                page_of(c + u, pid[u], slot[u]);
+                ok[u] = check(pid[u]);
+                load_chunk<KV8>(p, pid[u], slot[u], kvh, lane, ring[u]);
             }
+        }
+        int32_t npid = 0, nslot = 0;  // of the chunk to be loaded next
+        if (c + D < ce) page_of(c + D, npid, nslot);
+        auto work = [&](const Chunk<KV8>& k, int32_t pid, int32_t slot, bool ok, int32_t c) {
             const int32_t tok = c * kChunkTokens + g;
+            AFrag fr;
+            fragments<KV8, F16>(k, fr);
             float w0 = 0.f, w1 = 0.f;  // weights of tokens g and g + 8 over this lane's rows
-            auto add = [&](const QFrag<KV8>& f, const float (&nlj)[2], const int32_t (&limj)[2]) {
+            auto add = [&](const QFrag& f, const float (&m)[2], const float (&nlj)[2], const int32_t (&limj)[2]) {
                 float s[4];
-                scores<KV8>(k, f, s);
+                scores<F16>(fr, f, s);
                 // selected, never multiplied: a masked score may be infinite or NaN
-                w0 += tok < limj[0] ? ptx::ex2(fmaf(s[0], mul, nlj[0])) : 0.f;
-                w0 += tok < limj[1] ? ptx::ex2(fmaf(s[1], mul, nlj[1])) : 0.f;
-                w1 += tok + 8 < limj[0] ? ptx::ex2(fmaf(s[2], mul, nlj[0])) : 0.f;
-                w1 += tok + 8 < limj[1] ? ptx::ex2(fmaf(s[3], mul, nlj[1])) : 0.f;
+                w0 += tok < limj[0] ? ptx::ex2(fmaf(s[0], m[0], nlj[0])) : 0.f;
+                w0 += tok < limj[1] ? ptx::ex2(fmaf(s[1], m[1], nlj[1])) : 0.f;
+                w1 += tok + 8 < limj[0] ? ptx::ex2(fmaf(s[2], m[0], nlj[0])) : 0.f;
+                w1 += tok + 8 < limj[1] ? ptx::ex2(fmaf(s[3], m[1], nlj[1])) : 0.f;
             };
             if (NT > 0) {
 #pragma unroll
-                for (int j = 0; j < kHeld; ++j) add(qf[j], nl[j], lim[j]);
+                for (int j = 0; j < kHeld; ++j) add(qf[j], ml[j], nl[j], lim[j]);
             } else {
                 for (int j = 0; j < groups; ++j) {
-                    load_group<KV8>(p, b, kvh, L, j, lane, qf[0], nl[0], lim[0]);
-                    add(qf[0], nl[0], lim[0]);
+                    load_group<KV8, F16>(p, b, kvh, L, mul, j, lane, qf[0], ml[0], nl[0], lim[0]);
+                    add(qf[0], ml[0], nl[0], lim[0]);
                 }
             }
             w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
@@ -287,9 +349,20 @@ __global__ void __launch_bounds__(kThreads) weights_kernel(const Params p) {
                 if (c * kChunkTokens + i < L)
                     atomicAdd(p.weights + ((int64_t)pid * p.Hkv + kvh) * p.P + slot + i, t == 0 ? w0 : w1);
             }
-            if (c + 1 < ce) k = kn;
-            pid = npid; slot = nslot; ok = nok;
-            npid = fpid; nslot = fslot;
+        };
+        for (; c < ce; c += D) {
+#pragma unroll
+            for (int u = 0; u < D; ++u) {
+                if (c + u >= ce) break;
+                work(ring[u], pid[u], slot[u], ok[u], c + u);
+                if (c + u + D < ce) {
+                    pid[u] = npid;
+                    slot[u] = nslot;
+                    ok[u] = check(pid[u]);
+                    load_chunk<KV8>(p, pid[u], slot[u], kvh, lane, ring[u]);
+                    if (c + u + D + 1 < ce) page_of(c + u + D + 1, npid, nslot);
+                }
+            }
         }
         cur = (int64_t)pre[b] * p.Hkv + (int64_t)kvh * n + ce;
         c = 0;
@@ -307,7 +380,7 @@ int launch(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
     auto kern = weights_kernel<KV8, NT>;
     int st = PGQA_OK;
     if (smem > 48 * 1024 && (st = host_smem_limit(kern, dev, smem, done)) != PGQA_OK) return st;
-    return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, 1, p);
+    return host_launch(kern, dim3((unsigned)(ctas_per_sm(NT) * sms)), kThreads, (size_t)smem, stream, 1, p);
 }
 
 template <bool KV8>

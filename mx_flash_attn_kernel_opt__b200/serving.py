@@ -13,78 +13,99 @@ on torch's current stream of the tensors' device, allocates nothing but its outp
 be captured into a CUDA graph after one eager call.  Errors that only the device sees (a
 page id, length or position out of range) are read with `check_device_error()`.
 """
-import ctypes
 import math
+import struct
 
 import torch
 
-from . import _lib
 from ._lib import PgqaError, check, lib
 from .ops import FP8, _scale_array
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
-
-def _check(what, device, *named):
-    """named: (name, tensor, dtype); every tensor contiguous and on `device`."""
-    for name, t, dt in named:
-        if t.dtype != dt:
-            raise TypeError(f"{what}: {name} must be {dt}, got {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{what}: {name} must be on {device}, got {t.device}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous")
+# include/pgqa.h's argument structs, field by field
+_ROPE = struct.Struct("N15P21q4i64s")
+_WEIGHTS = struct.Struct("N7P9qfi")
+_EVICT = struct.Struct("N8P9q2i")
+_CROSS = struct.Struct("N8P10qfiPN")
 
 
-def _pools(what, k_cache, v_cache, block_table, seq_lens):
-    """Checks pools, table and lengths; returns (device, e4m3, num_pages, P, Hkv, D, B)."""
+def _ptr(what, name, t, dtype, dev):
+    """Address of a contiguous tensor of `dtype` on CUDA device number `dev`."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} must be on cuda:{dev}, got {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous")
+    return t.data_ptr()
+
+
+def _cache(what, k_cache, block_table, seq_lens):
+    """Checks a pool, its table and lengths.  Returns (device number, e4m3, pool shape,
+    B, table width, address of the pool, of the table, of the lengths)."""
     if not k_cache.is_cuda:
         raise ValueError(f"{what}: k_cache must be a CUDA tensor")
-    dt = FP8 if k_cache.dtype == FP8 else _BF16
-    dev = k_cache.device
-    _check(what, dev, ("k_cache", k_cache, dt), ("block_table", block_table, _I32),
-           ("seq_lens", seq_lens, _I32))
-    if k_cache.dim() != 4 or block_table.dim() != 2:
+    dev, fp8 = k_cache.get_device(), k_cache.dtype is FP8
+    pool = _ptr(what, "k_cache", k_cache, FP8 if fp8 else _BF16, dev)
+    table = _ptr(what, "block_table", block_table, _I32, dev)
+    lens = _ptr(what, "seq_lens", seq_lens, _I32, dev)
+    shape, bt = k_cache.shape, block_table.shape
+    if len(shape) != 4 or len(bt) != 2:
         raise PgqaError(2, f"{what}: pools must be [num_pages, P, Hkv, D], block_table [B, width]")
-    if v_cache is not None:
-        _check(what, dev, ("v_cache", v_cache, dt))
-        if v_cache.shape != k_cache.shape:
-            raise PgqaError(2, f"{what}: K and V pools must have one shape")
-    B = block_table.shape[0]
-    if seq_lens.dim() != 1 or seq_lens.shape[0] != B:
+    if seq_lens.shape != bt[:1]:
         raise PgqaError(2, f"{what}: seq_lens must be [B]")
-    return (dev, dt is FP8, *k_cache.shape, B)
+    return dev, fp8, shape, bt[0], bt[1], pool, table, lens
 
 
-def _weight_pool(what, weights, name, dev, num_pages, Hkv, P):
-    _check(what, dev, (name, weights, _F32))
-    if tuple(weights.shape) != (num_pages, Hkv, P):
-        raise PgqaError(2, f"{what}: {name} must be [num_pages, Hkv, P] = {(num_pages, Hkv, P)}")
+def _v_pool(what, v_cache, k_cache, dev):
+    p = _ptr(what, "v_cache", v_cache, k_cache.dtype, dev)
+    if v_cache.shape != k_cache.shape:
+        raise PgqaError(2, f"{what}: K and V pools must have one shape")
+    return p
 
 
-def _launch(fn, args, device, what):
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    if device.index == torch.cuda.current_device():
-        st = fn(ctypes.byref(args), stream)
+def _weight_pool(what, name, weights, dev, shape):
+    p = _ptr(what, name, weights, _F32, dev)
+    if weights.shape != (shape[0], shape[2], shape[1]):
+        raise PgqaError(2, f"{what}: {name} must be [num_pages, Hkv, P] = {(shape[0], shape[2], shape[1])}")
+    return p
+
+
+def _scales(x, Hkv, dev):
+    """Per-head factors as a float32 tensor of the device (None stays None)."""
+    if torch.is_tensor(x) and x.dtype is _F32 and x.get_device() == dev and x.shape == (Hkv,) \
+            and x.is_contiguous():
+        return x
+    return _scale_array(x, Hkv, torch.device("cuda", dev))
+
+
+def _call(fn, args, dev, what):
+    """Launches on torch's current stream of the device, with that device current."""
+    if dev == torch.cuda.current_device():
+        st = fn(args, torch.cuda.current_stream(dev).cuda_stream)
     else:
-        with torch.cuda.device(device):
-            st = fn(ctypes.byref(args), stream)
+        with torch.cuda.device(dev):
+            st = fn(args, torch.cuda.current_stream(dev).cuda_stream)
     check(st, what)
 
 
-def _rows(what, name, x, lead, D, device):
-    """Checks q / k_new / v_new [*lead, heads, D] (heads contiguous inside, any strides that
-    are multiples of 16 bytes); returns (heads, element strides of sequence, token, head)."""
-    if x.dtype != _BF16:
+def _rows(what, name, x, lead, D, dev, step):
+    """Checks q / k_new / v_new [*lead, heads, D] (a head's elements contiguous, any other
+    strides); returns (address, heads, element strides of sequence, token, head).  step: the
+    one leading dimension counts sequences rather than tokens."""
+    if x.dtype is not _BF16:
         raise TypeError(f"{what}: {name} must be {_BF16}, got {x.dtype}")
-    if x.device != device:
-        raise ValueError(f"{what}: {name} must be on {device}, got {x.device}")
-    if x.dim() != len(lead) + 2 or tuple(x.shape[:-2]) != lead or x.shape[-1] != D:
+    if x.get_device() != dev:
+        raise ValueError(f"{what}: {name} must be on cuda:{dev}, got {x.device}")
+    n = len(lead)
+    shape, s = x.shape, x.stride()
+    if len(shape) != n + 2 or shape[:n] != lead or shape[-1] != D:
         raise PgqaError(2, f"{what}: {name} must be [{', '.join(map(str, lead))}, heads, {D}]")
-    if x.stride(-1) != 1:
+    if s[-1] != 1:
         raise ValueError(f"{what}: the elements of a head of {name} must be contiguous")
-    s = x.stride()
-    return x.shape[-2], ((s[0], s[1], s[2]) if len(lead) == 2 else (0, s[0], s[1]))
+    s = (s[0], s[1], s[2]) if n == 2 else ((s[0], 0, s[1]) if step else (0, s[0], s[1]))
+    return x.data_ptr(), shape[-2], s
 
 
 def _turn(what, q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos, sin, positions,
@@ -98,95 +119,89 @@ def _turn(what, q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos, s
         raise ValueError(f"{what}: k_new and v_new go together")
     if not first.is_cuda:
         raise ValueError(f"{what}: q / k_new must be CUDA tensors")
-    dev = first.device
-    a = _lib.PgqaRopeArgs(struct_size=ctypes.sizeof(_lib.PgqaRopeArgs))
-    D = first.shape[-1]
+    dev, full = first.get_device(), first.shape
+    D = full[-1]
+    Hkv = P = num_pages = width = fp8 = 0
+    kp = vp = tp = lp = wp = cup = posp = qp = qo = knp = vnp = ksp = vsp = 0
     if k_new is not None:
-        _, fp8, num_pages, P, Hkv, D, B = _pools(what, k_cache, v_cache, block_table, seq_lens)
-        if k_cache.device != dev:
+        at, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
+        if at != dev:
             raise ValueError(f"{what}: all tensors must be on one device")
-        if not fp8 and (k_scale is not None or v_scale is not None):
+        vp = _v_pool(what, v_cache, k_cache, dev)
+        num_pages, P, Hkv, D = shape
+        if weights is not None:
+            wp = _weight_pool(what, "weights", weights, dev, shape)
+        if fp8:
+            ks, vs = _scales(k_scale, Hkv, dev), _scales(v_scale, Hkv, dev)
+            ksp = 0 if ks is None else ks.data_ptr()
+            vsp = 0 if vs is None else vs.data_ptr()
+        elif k_scale is not None or v_scale is not None:
             raise ValueError("k_scale / v_scale apply to float8_e4m3fn pools only")
-        a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-        a.block_table, a.bt_stride = block_table.data_ptr(), block_table.shape[1]
-        a.num_pages, a.page_size, a.num_heads_k, a.kv_format = num_pages, P, Hkv, int(fp8)
     else:
         if weights is not None:
             raise ValueError(f"{what}: weights goes with k_new and v_new")
         B = seq_lens.shape[0] if seq_lens is not None else (
-            cu_seqlens.shape[0] - 1 if cu_seqlens is not None else first.shape[0])
-    if seq_lens is not None:
-        _check(what, dev, ("seq_lens", seq_lens, _I32))
-        a.seq_lens = seq_lens.data_ptr()
+            cu_seqlens.shape[0] - 1 if cu_seqlens is not None else full[0])
+        if seq_lens is not None:
+            lp = _ptr(what, "seq_lens", seq_lens, _I32, dev)
+    seqlen, step = 0, False
     if cu_seqlens is not None:
-        _check(what, dev, ("cu_seqlens", cu_seqlens, _I32))
-        if tuple(cu_seqlens.shape) != (B + 1,) or first.dim() != 3:
+        cup = _ptr(what, "cu_seqlens", cu_seqlens, _I32, dev)
+        if cu_seqlens.shape != (B + 1,) or len(full) != 3:
             raise PgqaError(2, f"{what}: with cu_seqlens [B + 1], q / k_new are [tokens, heads, D]")
-        lead = (first.shape[0],)
-        a.cu_seqlens = cu_seqlens.data_ptr()
+        lead = full[:1]
+        tokens = full[0]
     else:
-        if first.dim() not in (3, 4) or first.shape[0] != B:
+        if len(full) not in (3, 4) or full[0] != B:
             raise PgqaError(2, f"{what}: q / k_new must be [B, heads, D] or [B, S, heads, D]")
-        lead = tuple(first.shape[:-2])
-        a.seqlen = lead[1] if len(lead) == 2 else 1
-    a.tokens = math.prod(lead)
-    a.batch_size, a.headdim = B, D
-
-    def strides(x):
-        heads, s = _rows(what, x[0], x[1], lead, D, dev)
-        # [B, heads, D]: one token per sequence, so the first stride is the sequence's
-        return heads, (ctypes.c_int64 * 3)(s[1], 0, s[2]) if cu_seqlens is None and len(lead) == 1 \
-            else (ctypes.c_int64 * 3)(*s)
-
+        step = len(full) == 3
+        lead = full[:-2]
+        seqlen = 1 if step else full[1]
+        tokens = B * seqlen
+    none = (0, 0, 0)
+    qs = kst = vst = none
+    Hq = 0
     if k_new is not None:
-        hk, a.k_strides = strides(("k_new", k_new))
-        hv, a.v_strides = strides(("v_new", v_new))
+        knp, hk, kst = _rows(what, "k_new", k_new, lead, D, dev, step)
+        vnp, hv, vst = _rows(what, "v_new", v_new, lead, D, dev, step)
         if hk != Hkv or hv != Hkv:
             raise PgqaError(2, f"{what}: k_new / v_new must have the pools' {Hkv} heads")
-        a.k_new, a.v_new = k_new.data_ptr(), v_new.data_ptr()
     if q is not None:
-        a.num_heads, a.q_strides = strides(("q", q))
+        qp, Hq, qs = _rows(what, "q", q, lead, D, dev, step)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=_BF16, device=dev)
+            q_out = q.new_empty(full)
+            qo = q_out.data_ptr()
         else:
-            _check(what, dev, ("q_out", q_out, _BF16))
-            if q_out.shape != q.shape:
+            qo = _ptr(what, "q_out", q_out, _BF16, dev)
+            if q_out.shape != full:
                 raise PgqaError(2, f"{what}: q_out must have q's shape")
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
-
-    dt = _BF16 if cos.dtype == _BF16 else _F32
-    _check(what, dev, ("cos", cos, dt), ("sin", sin, dt))
+    tdt = _BF16 if cos.dtype is _BF16 else _F32
+    cp, sp = _ptr(what, "cos", cos, tdt, dev), _ptr(what, "sin", sin, tdt, dev)
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise PgqaError(2, f"{what}: cos and sin must be [rows, rotary_dim / 2]")
-    pairs = cos.shape[1]
-    a.cos, a.sin, a.table_rows, a.rotary_dim = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * pairs
-    a.table_format, a.interleaved = int(dt is _BF16), int(bool(interleaved))
-    a.num_axes = 1
+    rows, pairs = cos.shape
+    num_axes = 1
     if positions is not None:
-        _check(what, dev, ("positions", positions, _I32))
-        if tuple(positions.shape) != lead:
-            if tuple(positions.shape[1:]) != lead or positions.dim() != len(lead) + 1:
+        posp = _ptr(what, "positions", positions, _I32, dev)
+        ps = positions.shape
+        if ps != lead:
+            if ps[1:] != lead or len(ps) != len(lead) + 1:
                 raise PgqaError(2, f"{what}: positions must be [axes, {', '.join(map(str, lead))}], "
                                    "or without the first dimension for one axis")
-            a.num_axes = positions.shape[0]
-        a.positions = positions.data_ptr()
+            num_axes = ps[0]
     if axes is not None:
-        if len(axes) != pairs or pairs > 64 or not all(0 <= int(x) < a.num_axes for x in axes):
-            raise PgqaError(2, f"{what}: axes must name one of the {a.num_axes} axes for each of "
+        if len(axes) != pairs or pairs > 64 or min(axes) < 0 or max(axes) >= num_axes:
+            raise PgqaError(2, f"{what}: axes must name one of the {num_axes} axes for each of "
                                f"the {pairs} pairs")
-        a.pair_axis[:pairs] = [int(x) for x in axes]
-    elif a.num_axes > 1:
+        axes = bytes(axes)
+    elif num_axes > 1:
         raise ValueError(f"{what}: positions on several axes need axes, the axis of each pair")
-    if weights is not None:
-        _weight_pool(what, weights, "weights", dev, num_pages, Hkv, P)
-        a.weights = weights.data_ptr()
-    ks = vs = None
-    if k_new is not None and fp8:
-        ks, vs = _scale_array(k_scale, Hkv, dev), _scale_array(v_scale, Hkv, dev)
-        a.k_scale = ks.data_ptr() if ks is not None else None
-        a.v_scale = vs.data_ptr() if vs is not None else None
-    if a.tokens:  # torch gives empty tensors no address
-        _launch(lib().pgqa_rope_append, a, dev, "pgqa_rope_append")
+    if tokens:  # torch gives empty tensors no address
+        _call(lib().pgqa_rope_append, _ROPE.pack(
+            _ROPE.size, qp, knp, vnp, qo, kp, vp, lp, tp, cp, sp, posp, cup, wp, ksp, vsp, B, seqlen,
+            tokens, Hq, Hkv, D, P, num_pages, width, *qs, *kst, *vst, rows, 2 * pairs, num_axes,
+            1 if interleaved else 0, 1 if fp8 else 0, 1 if tdt is _BF16 else 0, 0, axes or b""),
+            dev, "pgqa_rope_append")
     return q_out
 
 
@@ -231,25 +246,25 @@ def accumulate_weights(q, k_cache, block_table, seq_lens, lse, weights, *, scale
     sees no token (lse -inf) adds nothing, and entries past a sequence's length are left as
     they are.  Unless sequences share pages, the result does not depend on any order."""
     what = "accumulate_weights"
-    dev, fp8, num_pages, P, Hkv, D, B = _pools(what, k_cache, None, block_table, seq_lens)
-    _check(what, dev, ("q", q, _BF16), ("lse", lse, _F32))
-    if q.dim() not in (3, 4) or q.shape[0] != B or q.shape[-1] != D:
+    dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
+    num_pages, P, Hkv, D = shape
+    qp, lsep = _ptr(what, "q", q, _BF16, dev), _ptr(what, "lse", lse, _F32, dev)
+    qs = q.shape
+    if len(qs) not in (3, 4) or qs[0] != B or qs[-1] != D:
         raise PgqaError(2, f"{what}: q must be [B, Hq, D] or [B, Sq, Hq, D]")
-    Sq = q.shape[1] if q.dim() == 4 else 1
-    Hq = q.shape[-2]
-    if tuple(lse.shape) != (B, Hq, Sq):
+    Sq, Hq = qs[1] if len(qs) == 4 else 1, qs[-2]
+    if lse.shape != (B, Hq, Sq):
         raise PgqaError(2, f"{what}: lse must be [B, Hq, Sq] = {(B, Hq, Sq)}")
-    _weight_pool(what, weights, "weights", dev, num_pages, Hkv, P)
-    if not fp8 and k_scale is not None:
+    wp = _weight_pool(what, "weights", weights, dev, shape)
+    ks = None
+    if fp8:
+        ks = _scales(k_scale, Hkv, dev)
+    elif k_scale is not None:
         raise ValueError("k_scale applies to float8_e4m3fn pools only")
-    ks = _scale_array(k_scale, Hkv, dev) if fp8 else None
-    a = _lib.PgqaWeightsArgs(
-        ctypes.sizeof(_lib.PgqaWeightsArgs), q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(),
-        weights.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(),
-        ks.data_ptr() if ks is not None else None, B, Sq, Hq, Hkv, D, P, num_pages,
-        block_table.shape[1], int(bool(causal)),
-        float(scale) if scale is not None else 1.0 / math.sqrt(D), int(fp8))
-    _launch(lib().pgqa_accumulate_weights, a, dev, "pgqa_accumulate_weights")
+    _call(lib().pgqa_accumulate_weights, _WEIGHTS.pack(
+        _WEIGHTS.size, qp, kp, lsep, wp, lp, tp, 0 if ks is None else ks.data_ptr(), B, Sq, Hq, Hkv, D,
+        P, num_pages, width, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale,
+        1 if fp8 else 0), dev, "pgqa_accumulate_weights")
     return weights
 
 
@@ -268,21 +283,17 @@ def evict_kv(k_cache, v_cache, weights, block_table, seq_lens, keep, *, sinks=0,
     first new_lens slots; the others are left as they are).  Pages from ceil(keep / P) on
     are the caller's to free.  Sequences that share pages cannot be cut."""
     what = "evict_kv"
-    dev, fp8, num_pages, P, Hkv, D, B = _pools(what, k_cache, v_cache, block_table, seq_lens)
-    _weight_pool(what, weights, "weights", dev, num_pages, Hkv, P)
-    if weights_out is not None:
-        _weight_pool(what, weights_out, "weights_out", dev, num_pages, Hkv, P)
-    keep = int(keep)
+    dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
+    num_pages, P, Hkv, D = shape
+    vp = _v_pool(what, v_cache, k_cache, dev)
+    wp = _weight_pool(what, "weights", weights, dev, shape)
+    op = 0 if weights_out is None else _weight_pool(what, "weights_out", weights_out, dev, shape)
     if keep < 1:
         raise PgqaError(2, f"{what}: keep must be at least 1")
-    kept = torch.empty(B, Hkv, keep, dtype=_I32, device=dev)
-    new_lens = torch.empty(B, dtype=_I32, device=dev)
-    a = _lib.PgqaEvictArgs(
-        ctypes.sizeof(_lib.PgqaEvictArgs), k_cache.data_ptr(), v_cache.data_ptr(),
-        weights.data_ptr(), weights_out.data_ptr() if weights_out is not None else None,
-        seq_lens.data_ptr(), block_table.data_ptr(), kept.data_ptr(), new_lens.data_ptr(), B,
-        Hkv, D, P, num_pages, block_table.shape[1], keep, int(sinks), int(recent), int(fp8))
-    _launch(lib().pgqa_evict, a, dev, "pgqa_evict")
+    kept, new_lens = seq_lens.new_empty((B, Hkv, keep)), seq_lens.new_empty((B,))
+    _call(lib().pgqa_evict, _EVICT.pack(
+        _EVICT.size, kp, vp, wp, op, lp, tp, kept.data_ptr(), new_lens.data_ptr(), B, Hkv, D, P,
+        num_pages, width, keep, sinks, recent, 1 if fp8 else 0, 0), dev, "pgqa_evict")
     return kept, new_lens
 
 
@@ -300,55 +311,60 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     for packed q, else [B, Hq, Sq]; -inf where a row sees no key.  Rows of packed tokens
     behind the last sequence are left as they are in `out`."""
     what = "cross_attention"
-    dev, fp8, num_pages, P, Hkv, D, B = _pools(what, k_cache, v_cache, block_table, seq_lens)
+    dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
+    num_pages, P, Hkv, D = shape
     if fp8:
         raise NotImplementedError(f"{what}: float8_e4m3fn pools are not implemented here")
-    if q.dtype != _BF16:
+    vp = _v_pool(what, v_cache, k_cache, dev)
+    if q.dtype is not _BF16:
         raise TypeError(f"{what}: q must be {_BF16}, got {q.dtype}")
-    if q.device != dev:
-        raise ValueError(f"{what}: q must be on {dev}, got {q.device}")
+    if q.get_device() != dev:
+        raise ValueError(f"{what}: q must be on cuda:{dev}, got {q.device}")
+    qs, st = q.shape, q.stride()
+    cup = 0
     if cu_seqlens_q is not None:
-        _check(what, dev, ("cu_seqlens_q", cu_seqlens_q, _I32))
-        if q.dim() != 3 or tuple(cu_seqlens_q.shape) != (B + 1,):
+        cup = _ptr(what, "cu_seqlens_q", cu_seqlens_q, _I32, dev)
+        if len(qs) != 3 or cu_seqlens_q.shape != (B + 1,):
             raise PgqaError(2, f"{what}: with cu_seqlens_q [B + 1], q is [tokens, Hq, D]")
-        tokens, Sq, stride = q.shape[0], 0, q.stride(0)
+        tokens, Sq, stride = qs[0], 0, st[0]
     else:
-        if q.dim() != 4 or q.shape[0] != B:
+        if len(qs) != 4 or qs[0] != B:
             raise PgqaError(2, f"{what}: q must be [B, Sq, Hq, D], or packed with cu_seqlens_q")
-        Sq, stride = q.shape[1], q.stride(1)
+        Sq, stride = qs[1], st[1]
         tokens = B * Sq
-        if B > 1 and Sq > 1 and q.stride(0) != Sq * stride:
+        if B > 1 and Sq > 1 and st[0] != Sq * stride:
             raise ValueError(f"{what}: the sequences of q must follow each other without a gap")
         if Sq == 1:
-            stride = q.stride(0)
-    Hq = q.shape[-2]
-    if q.shape[-1] != D:
+            stride = st[0]
+    Hq = qs[-2]
+    if qs[-1] != D:
         raise PgqaError(2, f"{what}: q and the pools must have one head dimension")
-    if q.stride(-1) != 1 or (Hq > 1 and q.stride(-2) != D):
+    if st[-1] != 1 or (Hq > 1 and st[-2] != D):
         raise ValueError(f"{what}: the heads of a token of q must be contiguous")
     if tokens <= 1:
         stride = Hq * D
     if out is None:
-        out = torch.empty(q.shape, dtype=_BF16, device=dev)
+        out = q.new_empty(qs)
+        op = out.data_ptr()
     else:
-        _check(what, dev, ("out", out, _BF16))
-        if out.shape != q.shape:
+        op = _ptr(what, "out", out, _BF16, dev)
+        if out.shape != qs:
             raise PgqaError(2, f"{what}: out must have q's shape")
     lse = None
     if return_lse:
-        lse = torch.empty((Hq, tokens) if cu_seqlens_q is not None else (B, Hq, Sq), dtype=_F32, device=dev)
+        lse = seq_lens.new_empty((Hq, tokens) if cup else (B, Hq, Sq), dtype=_F32)
     if tokens:
         L = lib()
-        with torch.cuda.device(dev):
-            need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, block_table.shape[1])
+        if dev == torch.cuda.current_device():
+            need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, width)
+        else:
+            with torch.cuda.device(dev):
+                need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, width)
         # a buffer of this call's own: calls on two streams or in two graphs share none
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        a = _lib.PgqaCrossArgs(
-            ctypes.sizeof(_lib.PgqaCrossArgs), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            out.data_ptr(), lse.data_ptr() if lse is not None else None, seq_lens.data_ptr(),
-            block_table.data_ptr(), cu_seqlens_q.data_ptr() if cu_seqlens_q is not None else None, B,
-            Sq, tokens, stride, Hq, Hkv, D, P, num_pages, block_table.shape[1],
-            float(scale) if scale is not None else 1.0 / math.sqrt(D), 0,
-            ws.data_ptr() if ws is not None else None, need)
-        _launch(L.pgqa_cross_attention, a, dev, "pgqa_cross_attention")
+        ws = seq_lens.new_empty((need,), dtype=torch.uint8) if need else None
+        _call(L.pgqa_cross_attention, _CROSS.pack(
+            _CROSS.size, q.data_ptr(), kp, vp, op, 0 if lse is None else lse.data_ptr(), lp, tp, cup, B,
+            Sq, tokens, stride, Hq, Hkv, D, P, num_pages, width,
+            1.0 / math.sqrt(D) if scale is None else scale, 0, 0 if ws is None else ws.data_ptr(), need),
+            dev, "pgqa_cross_attention")
     return (out, lse) if return_lse else out

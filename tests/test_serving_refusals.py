@@ -42,6 +42,13 @@ def test_rope_append(status, kw):
     assert _lib.lib().pgqa_last_status() == status
 
 
+def test_packed_structs_match_the_mirrors():
+    from mx_flash_attn_kernel_opt__b200 import serving
+    for packed, mirror in ((serving._ROPE, _lib.PgqaRopeArgs), (serving._WEIGHTS, _lib.PgqaWeightsArgs),
+                           (serving._EVICT, _lib.PgqaEvictArgs), (serving._CROSS, _lib.PgqaCrossArgs)):
+        assert packed.size == ctypes.sizeof(mirror)
+
+
 def test_rope_append_null_struct():
     assert _lib.lib().pgqa_rope_append(None, None) == 1
 
