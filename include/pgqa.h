@@ -378,9 +378,9 @@ int pgqa_evict(const pgqa_evict_args* args, void* stream);
  *                from cu[batch_size] on are left as they are
  *   k, v pools   [num_pages, P, Hkv, 128] bf16, as in the decode; g = Hq / Hkv <= 128
  *   softmax_lse  NULL or fp32: [Hq, tokens] with cu_seqlens, else [B, Hq, seqlen_q]
- *   workspace    pgqa_cross_workspace_size(...) bytes, 256-byte aligned, any contents (may
- *                be NULL when that is 0): partial results of calls with few query tokens.
- *                Calls that share one must be ordered.
+ *   workspace    pgqa_cross_workspace_size(...) bytes (at most 40 MB on a B200), 256-byte
+ *                aligned, any contents: parts of results that several CTAs share.  Calls
+ *                that share one must be ordered.
  */
 typedef struct pgqa_cross_args {
     size_t struct_size;
@@ -402,7 +402,7 @@ typedef struct pgqa_cross_args {
 
 int pgqa_cross_attention(const pgqa_cross_args* args, void* stream);
 
-/* Bytes of workspace pgqa_cross_attention needs on the current device (0: none, or an
+/* Bytes of workspace pgqa_cross_attention needs on the current device (0: no tokens, or an
  * invalid shape; pgqa_last_status() tells which). */
 size_t pgqa_cross_workspace_size(int64_t tokens, int64_t batch_size, int64_t num_heads,
                                  int64_t num_heads_k, int64_t headdim, int64_t page_size,

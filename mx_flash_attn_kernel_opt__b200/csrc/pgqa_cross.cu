@@ -10,26 +10,27 @@
  * Tensor-core bound: 4 * 128 flop per (query row, key) against 512 bytes of K and V per key
  * that all rows of a KV head share.  The g query heads of a KV head are rows of one tile
  * (row = token * g + head), so a 128-row tile holds 128 / g tokens and K and V are read
- * once per 256 rows.  A work item is (sequence, KV head, two such tiles, a range of keys);
- * one persistent CTA per SM walks the items in the same order in all of its roles:
+ * once per 256 rows.  A work item is (sequence, KV head, two such tiles).  The items' key
+ * tiles, one after the other, are cut into equal slices, one per persistent CTA (one CTA per
+ * SM); a cut that would fall within 1/24 of a slice of an item's end is moved there.  An item
+ * that is cut all the same leaves its parts' normalised O (fp32) and log-sum-exps in the
+ * workspace, and a second launch joins them.  Every role of a CTA walks the same items:
  *
- *   warps 0-3, 4-7  softmax and output of tile 0 and tile 1: thread = row = TMEM lane.  The
- *                   running maximum is moved only when a score exceeds it by 2^8 (O is then
- *                   rescaled in TMEM), so the O accumulator is touched once per item in the
- *                   usual case; sums and statistics are fp32, P is rounded to bf16 (half a
- *                   step, 2^-9 relative to its power of two, of weights that are summed in
+ *   warps 0-3, 4-7  softmax and output of tile 0 and tile 1: thread = row = TMEM lane, 64
+ *                   keys at a time.  The running maximum is moved only when a score exceeds
+ *                   it by 2^8 (O is then rescaled in TMEM), so the O accumulator is touched
+ *                   once per item in the usual case; sums and statistics are fp32, P is
+ *                   rounded to bf16 (2^-8 relative at most, of weights that are summed in
  *                   fp32) and goes back to TMEM over the scores it came from.
  *   warp 8          TMA: Q tiles, and 128-key tiles of K and V by page boxes through one
  *                   ring of five 32 KB slots; it zeroes V rows behind the last key, so that
  *                   a weight of 0 never meets a NaN left in a page.
  *   warp 9          issues the MMAs (one thread): S_w = Q_w K^T (both from shared memory),
- *                   O_w += P_w V (P from TMEM).  The score tile of the next keys is issued
+ *                   O_w += P_w V (P from TMEM), the latter 64 keys at a time, as soon as
+ *                   their weights are there.  The score tile of the next keys is issued
  *                   right behind the PV of the present ones, and the two tiles alternate,
  *                   so the tensor core works for one while the other's softmax runs.
  * TMEM: S and P of the tiles at columns 0 and 128, O at 256 and 384.
- *
- * With fewer items than SMs the keys are cut into ranges as well: each range writes its
- * normalised O (fp32) and log-sum-exp, and a second launch joins them.
  *
  * Every wait is bounded: one that expires sets the device error word and the CTA's abort
  * flag, every role leaves its loop, loads and MMAs in flight are drained and TMEM is freed.
@@ -42,6 +43,7 @@
 #include <stdlib.h>
 
 #include "pgqa_host.h"
+#include "pgqa_partition.h"
 #include "pgqa_ptx.cuh"
 
 namespace pgqa {
@@ -53,23 +55,25 @@ constexpr int kHalf = kTile * 128;         // one 64-dimension half of a tile, b
 constexpr int kSlot = 2 * kHalf;
 constexpr int kSlots = 5;
 constexpr int kQOff = 0, kRingOff = 2 * kSlot, kBarOff = kRingOff + kSlots * kSlot;
-constexpr int kBars = 2 * kSlots + 10;
+constexpr int kBars = 2 * kSlots + 14;
 constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
+constexpr int kRows = 2 * kTile;           // rows of a work item
+constexpr int kMinTiles = 2;               // key tiles of a slice, at least
+constexpr int kSnap = 24;
 constexpr float kLazyLog2 = 8.f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
-constexpr int kMaxSplits = 32;
 
 struct Params {
     __nv_bfloat16* out;      // [T, Hq, 128]
     float* lse;              // optional: [Hq, T] packed, [B, Hq, S] padded
-    float *part_o, *part_lse;  // key ranges: [splits][T][Hq][128] and [splits][T][Hq] (log2 units)
+    float *rec_o, *rec_lse;  // parts of cut items: [2 * grid][256 rows][128], [2 * grid][256] (log2 units)
     const int32_t *seq_lens, *block_table, *cu;
     int32_t* err;
     int64_t bt_stride, cap_tokens;
     int32_t B, S, T, Hq, Hkv, g, P, page_shift, num_pages;
     int32_t tile_tokens;     // prompt tokens per tile: 128 / g
     int32_t box;             // tokens of one TMA box of a pool: a power of two that divides P
-    int32_t splits;
+    int32_t grid;            // CTAs of the first launch
     float scale_log2;
     uint64_t wait_limit_ns;
 };
@@ -83,71 +87,156 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-struct Item {
-    int32_t b, kvh, tok0, tok_end, L, t0, t1, split;  // prompt tokens from tok0, key tiles [t0, t1)
+/* A sequence's prompt tokens [tok0, tok1), keys L, key tiles n (at least 1), items. */
+struct Seq {
+    int32_t tok0, tok1, L, n, pairs, items;
+    __device__ int64_t tiles() const { return (int64_t)items * n; }
 };
 
-/* Walks this CTA's items; called by whole warps, every role with a copy of its own. */
-struct Walker {
-    int64_t at, base;        // next item, items before sequence b0
-    int32_t b0, total;       // block of 32 sequences, and its items
-    int32_t cnt, incl, tok0, tok1;  // this lane's sequence: items, running sum, prompt tokens
-    __device__ void load(const Params& p, int lane) {
-        const int32_t b = b0 + lane;
-        cnt = 0;
-        tok0 = tok1 = 0;
-        if (b < p.B) {
-            tok0 = p.cu ? __ldg(p.cu + b) : b * p.S;
-            tok1 = p.cu ? __ldg(p.cu + b + 1) : tok0 + p.S;
-            if (tok0 < 0 || tok1 < tok0 || tok1 > p.T) {
-                atomicOr(p.err, kDevErrBadSeqlen);
-                tok0 = max(0, min(tok0, p.T));
-                tok1 = max(tok0, min(tok1, p.T));
-            }
-            cnt = (tok1 - tok0 + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens) * p.Hkv * p.splits;
-        }
-        incl = cnt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-        }
-        total = __shfl_sync(0xffffffffu, incl, 31);
+__device__ __forceinline__ Seq load_seq(const Params& p, int32_t b, bool report) {
+    Seq q;
+    q.tok0 = q.tok1 = q.L = q.pairs = q.items = 0;
+    q.n = 1;
+    if (b >= p.B) return q;
+    q.tok0 = p.cu ? __ldg(p.cu + b) : b * p.S;
+    q.tok1 = p.cu ? __ldg(p.cu + b + 1) : q.tok0 + p.S;
+    int64_t L = __ldg(p.seq_lens + b);
+    if (q.tok0 < 0 || q.tok1 < q.tok0 || q.tok1 > p.T || L < 0 || L > p.cap_tokens) {
+        if (report) atomicOr(p.err, kDevErrBadSeqlen);
+        q.tok0 = max(0, min(q.tok0, p.T));
+        q.tok1 = max(q.tok0, min(q.tok1, p.T));
+        L = L < 0 ? 0 : (L > p.cap_tokens ? p.cap_tokens : L);
     }
-    __device__ void init(const Params& p, int lane) {
-        at = blockIdx.x;
-        base = 0;
-        b0 = 0;
-        load(p, lane);
+    q.L = (int32_t)L;
+    q.n = max(1, (q.L + kTile - 1) / kTile);
+    q.pairs = (q.tok1 - q.tok0 + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+    q.items = q.pairs * p.Hkv;
+    return q;
+}
+
+/* Slice [lo, hi) of CTA c of the n active ones, and the item at each end. */
+struct Slice {
+    int64_t lo, hi;
+    int64_t base;            // first tile of sequence b, which holds tile lo
+    int32_t b;
+    int64_t item_lo, item_len;  // the item that holds tile lo: its first tile, its length
+    int64_t n, total;        // active CTAs, tiles of all slices
+};
+
+/* A cut at most 1/kSnap of a slice away from an item's end is moved there. */
+__device__ __forceinline__ int64_t snap_range(int64_t n, int64_t total) { return total / n / kSnap; }
+__device__ __forceinline__ int64_t snapped(int64_t off, int64_t len, int64_t tol) {
+    return off <= tol ? 0 : (len - off <= tol ? len : off);
+}
+
+/* By all threads of a block (a multiple of 32, at most 1024); the result in shared memory. */
+template <int kT>
+__device__ void find_slice(const Params& p, int32_t c, Slice& out) {
+    __shared__ int64_t wsum[kT / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (p.B + kT - 1) / kT;
+    const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+    int64_t local = 0;
+    for (int b = b0; b < b1; ++b) local += load_seq(p, b, blockIdx.x == 0).tiles();
+    int64_t incl = local;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int64_t run = incl - local, total = 0;
+    for (int w = 0; w < kT / 32; ++w) {
+        if (w < warp) run += wsum[w];
+        total += wsum[w];
+    }
+    int64_t n = total / kMinTiles;
+    n = n < 1 ? 1 : (n > p.grid ? p.grid : n);
+    if (tid == 0) {
+        out.n = n;
+        out.total = total;
+    }
+    if (c >= n || total == 0) {
+        if (tid == 0) out.lo = out.hi = total;
+    } else {
+        const int64_t x0 = slice_begin(c, n, total), x1 = slice_begin(c + 1, n, total), tol = snap_range(n, total);
+        if (tid == 0 && c + 1 == n) out.hi = total;
+        for (int b = b0; b < b1; ++b) {
+            const Seq q = load_seq(p, b, false);
+            const int64_t end = run + q.tiles();
+            auto snap = [&](int64_t x) {
+                const int64_t off = (x - run) % q.n;
+                return x - off + snapped(off, q.n, tol);
+            };
+            if (run <= x0 && x0 < end) {
+                const int64_t lo = snap(x0);
+                out.lo = lo;
+                out.base = run;
+                out.b = b;
+                out.item_lo = lo - (lo - run) % q.n;
+                out.item_len = q.n;
+            }
+            if (c + 1 < n && run <= x1 && x1 < end) out.hi = snap(x1);
+            run = end;
+        }
+    }
+    __syncthreads();
+}
+
+struct Item {
+    int32_t b, kvh, tok0, tok_end, L, t0, t1;  // prompt tokens from tok0, key tiles [t0, t1)
+    bool cut;                                  // other CTAs have tiles of it too
+};
+
+/* Walks a slice's items; called by whole warps, every role with a copy of its own. */
+struct Walker {
+    int64_t pos, hi, base;
+    int32_t b;
+    Seq mine, cur;  // this lane's of the 32 sequences from b - cur_lane, and the one at work
+    int cur_lane;
+    __device__ void pick() {
+        cur.tok0 = __shfl_sync(0xffffffffu, mine.tok0, cur_lane);
+        cur.tok1 = __shfl_sync(0xffffffffu, mine.tok1, cur_lane);
+        cur.L = __shfl_sync(0xffffffffu, mine.L, cur_lane);
+        cur.n = __shfl_sync(0xffffffffu, mine.n, cur_lane);
+        cur.pairs = __shfl_sync(0xffffffffu, mine.pairs, cur_lane);
+        cur.items = __shfl_sync(0xffffffffu, mine.items, cur_lane);
+    }
+    __device__ void init(const Params& p, const Slice& s, int lane) {
+        pos = s.lo;
+        hi = s.hi;
+        base = s.base;
+        b = s.b;
+        cur_lane = 0;
+        if (pos < hi) {
+            mine = load_seq(p, b + lane, false);
+            pick();
+        }
     }
     __device__ bool next(const Params& p, int lane, Item& it) {
-        while (at >= base + total) {
-            base += total;
-            b0 += 32;
-            if (b0 >= p.B) return false;
-            load(p, lane);
+        if (pos >= hi) return false;
+        while (pos >= base + cur.tiles()) {
+            base += cur.tiles();
+            ++b;
+            if (++cur_lane == 32) {
+                cur_lane = 0;
+                mine = load_seq(p, b + lane, false);
+            }
+            pick();
         }
-        const int32_t r0 = (int32_t)(at - base);
-        const int f = __ffs(__ballot_sync(0xffffffffu, incl > r0)) - 1;
-        const int32_t r = r0 - __shfl_sync(0xffffffffu, incl - cnt, f);
-        const int32_t t_lo = __shfl_sync(0xffffffffu, tok0, f);
-        it.tok_end = __shfl_sync(0xffffffffu, tok1, f);
-        it.b = b0 + f;
-        const int32_t pairs = (it.tok_end - t_lo + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
-        const int32_t unit = r / p.splits;
-        it.split = r - unit * p.splits;
-        it.kvh = unit / pairs;
-        it.tok0 = t_lo + (unit - it.kvh * pairs) * 2 * p.tile_tokens;
-        int64_t L = __ldg(p.seq_lens + it.b);
-        if (L < 0 || L > p.cap_tokens) {
-            if (lane == 0) atomicOr(p.err, kDevErrBadSeqlen);
-            L = L < 0 ? 0 : p.cap_tokens;
-        }
-        it.L = (int32_t)L;
-        const int32_t n = (it.L + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
-        it.t0 = min(n, it.split * per);
-        it.t1 = min(n, it.t0 + per);
-        at += gridDim.x;
+        const int64_t in = pos - base;
+        const int32_t unit = (int32_t)(in / cur.n);
+        it.b = b;
+        it.kvh = unit / cur.pairs;
+        it.tok0 = cur.tok0 + (unit - it.kvh * cur.pairs) * 2 * p.tile_tokens;
+        it.tok_end = cur.tok1;
+        it.L = cur.L;
+        it.t0 = (int32_t)(in - (int64_t)unit * cur.n);
+        it.t1 = hi - pos < cur.n - it.t0 ? it.t0 + (int32_t)(hi - pos) : cur.n;
+        it.cut = it.t0 > 0 || it.t1 < cur.n;
+        pos += it.t1 - it.t0;
+        if (it.L == 0) it.t1 = it.t0;  // a sequence without keys: one item length, no tiles
         return true;
     }
 };
@@ -162,10 +251,11 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     auto FULL = [&](int s) { return bars + 8u * s; };
     auto EMPTY = [&](int s) { return bars + 8u * (kSlots + s); };
     auto SFULL = [&](int w) { return bars + 8u * (2 * kSlots + w); };
-    auto PFULL = [&](int w) { return bars + 8u * (2 * kSlots + 2 + w); };
-    auto PVDONE = [&](int w) { return bars + 8u * (2 * kSlots + 4 + w); };
-    const uint32_t QFULL = bars + 8u * (2 * kSlots + 6), QEMPTY = bars + 8u * (2 * kSlots + 7);
-    const uint32_t TAIL = bars + 8u * (2 * kSlots + 8), MMADONE = bars + 8u * (2 * kSlots + 9);
+    // of tile w and keys [0, 64) or [64, 128) of a key tile
+    auto PFULL = [&](int w, int h) { return bars + 8u * (2 * kSlots + 2 + 2 * w + h); };
+    auto PVDONE = [&](int w, int h) { return bars + 8u * (2 * kSlots + 6 + 2 * w + h); };
+    const uint32_t QFULL = bars + 8u * (2 * kSlots + 10), QEMPTY = bars + 8u * (2 * kSlots + 11);
+    const uint32_t TAIL = bars + 8u * (2 * kSlots + 12), MMADONE = bars + 8u * (2 * kSlots + 13);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarOff + kBars * 8);
     volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
 
@@ -180,8 +270,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         for (int w = 0; w < 2; ++w) {
             ptx::mbar_init(SFULL(w), 1);
-            ptx::mbar_init(PFULL(w), 4);  // one arrival per warp
-            ptx::mbar_init(PVDONE(w), 1);
+            for (int h = 0; h < 2; ++h) {
+                ptx::mbar_init(PFULL(w, h), 4);  // one arrival per warp
+                ptx::mbar_init(PVDONE(w, h), 1);
+            }
         }
         ptx::mbar_init(QFULL, 1);
         ptx::mbar_init(QEMPTY, 1);
@@ -230,8 +322,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         return __all_sync(0xffffffffu, wait_bar(bar, parity));
     };
 
+    __shared__ Slice slice;
+    find_slice<kThreads>(p, blockIdx.x, slice);
     Walker wk;
-    wk.init(p, lane);
+    wk.init(p, slice, lane);
     Item it;
 
     if (warp == 8) {
@@ -353,9 +447,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                 ks > 0 ? 1u : 0u);
             }
         };
-        auto pv = [&](int w, int slot, int steps, bool first) {
+        // 16-key steps [k0, k1) of a tile
+        auto pv = [&](int w, int slot, int k0, int k1, bool first) {
             const uint32_t vb = sb + kRingOff + (uint32_t)slot * kSlot;
-            for (int ks = 0; ks < steps; ++ks)
+            for (int ks = k0; ks < k1; ++ks)
                 ptx::tc_mma_f16_ts(tmem + 256u + (uint32_t)w * 128u, tmem + (uint32_t)(w * 128 + ks * 8),
                                    sdesc(vb + (uint32_t)ks * 2048u, kHalf, 1024), idesc(1), (first && ks == 0) ? 0u : 1u);
         };
@@ -378,13 +473,19 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         const int kv_v = n_kv + 2 * j + 1, kv_k = kv_v + 1;
                         const int nvalid = min(kTile, it.L - (it.t0 + j) * kTile);
                         for (int w = 0; w <= last; ++w) {
-                            ok = wait_bar(PFULL(w), n_s[w] & 1) &&
+                            const int steps = (nvalid + 15) >> 4;
+                            ok = wait_bar(PFULL(w, 0), n_s[w] & 1) &&
                                  (w > 0 || wait_bar(FULL(kv_v % kSlots), (kv_v / kSlots) & 1));
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            pv(w, kv_v % kSlots, 0, min(4, steps), j == 0);
+                            ptx::tc_commit(PVDONE(w, 0));
+                            ok = wait_bar(PFULL(w, 1), n_s[w] & 1);
                             if (!ok) break;
                             ++n_s[w];
                             ptx::tc_fence_after();
-                            pv(w, kv_v % kSlots, (nvalid + 15) >> 4, j == 0);
-                            ptx::tc_commit(PVDONE(w));
+                            pv(w, kv_v % kSlots, 4, steps, false);
+                            ptx::tc_commit(PVDONE(w, 1));
                             if (w == last) ptx::tc_commit(EMPTY(kv_v % kSlots));
                             if (j + 1 < n) {
                                 ok = w > 0 || wait_bar(FULL(kv_k % kSlots), (kv_k / kSlots) & 1);
@@ -432,67 +533,72 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     break;
                 }
                 ptx::tc_fence_after();
-                float s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) ptx::tc_ld32(tS + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-                ptx::tc_wait_ld();
                 const int32_t nvalid = it.L - tile * kTile;
-                if (nvalid < kTile) {
+                float s[64];
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] = i < nvalid ? s[i] : -INFINITY;
-                }
-                float m4[4] = {s[0], s[1], s[2], s[3]};
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 4; i < 128; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
-                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-                const bool raise = mx > m_ref + kLazyLog2;
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float m_new = raise ? mx : m_ref;
-                    const float alpha = raise ? ptx::ex2(m_ref - m_new) : 1.f;
-                    m_ref = m_new;
-                    l *= alpha;
-                    if (tile > it.t0) {
-                        if (!wait_all(PVDONE(w), (n_s - 1) & 1)) {
-                            ok = false;
-                            break;
-                        }
-                        ptx::tc_fence_after();
+                    for (int c = 0; c < 2; ++c)
+                        ptx::tc_ld32(tS + 64u * h + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                    ptx::tc_wait_ld();
+                    if (nvalid < kTile) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            float o[16];
-                            ptx::tc_ld16(tO + 16u * c, o);
-                            ptx::tc_wait_ld();
+                        for (int i = 0; i < 64; ++i) s[i] = 64 * h + i < nvalid ? s[i] : -INFINITY;
+                    }
+                    float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] *= alpha;
-                            ptx::tc_st16(tO + 16u * c, o);
+                    for (int i = 4; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
+                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+                    const bool raise = mx > m_ref + kLazyLog2;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float m_new = raise ? mx : m_ref;
+                        const float alpha = raise ? ptx::ex2(m_ref - m_new) : 1.f;
+                        m_ref = m_new;
+                        l *= alpha;
+                        if (tile > it.t0 || h > 0) {
+                            // the products so far: of the 64 keys before these
+                            if (!wait_all(PVDONE(w, h ^ 1), (h ? n_s : n_s - 1) & 1)) {
+                                ok = false;
+                                break;
+                            }
+                            ptx::tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < 8; ++c) {
+                                float o[16];
+                                ptx::tc_ld16(tO + 16u * c, o);
+                                ptx::tc_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) o[i] *= alpha;
+                                ptx::tc_st16(tO + 16u * c, o);
+                            }
                         }
                     }
-                }
-                const float base = m_ref == -INFINITY ? 0.f : m_ref;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                    const float base = m_ref == -INFINITY ? 0.f : m_ref;
+                    const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                     uint32_t pk[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float a = ptx::ex2(fmaf(s[64 * c + 2 * i], p.scale_log2, -base));
-                        const float b = ptx::ex2(fmaf(s[64 * c + 2 * i + 1], p.scale_log2, -base));
-                        l4[(2 * i) & 3] += a;
-                        l4[(2 * i + 1) & 3] += b;
-                        pk[i] = ptx::pack_bf16x2(a, b);
+                        float2 x = ptx::fma2(make_float2(s[2 * i], s[2 * i + 1]), mul2, sub2);
+                        x.x = ptx::ex2(x.x);
+                        x.y = ptx::ex2(x.y);
+                        sum[i & 1] = ptx::add2(sum[i & 1], x);
+                        pk[i] = ptx::pack_bf16x2(x.x, x.y);
                     }
-                    ptx::tc_st32(tS + 32u * c, pk);
+                    ptx::tc_st32(tS + 32u * h, pk);
+                    sum[0] = ptx::add2(sum[0], sum[1]);
+                    l += sum[0].x + sum[0].y;
+                    ptx::tc_wait_st();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(PFULL(w, h));
                 }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                ptx::tc_wait_st();
-                ptx::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(PFULL(w));
+                if (!ok) break;
             }
             if (!ok) break;
             const bool none = !(it.t1 > it.t0);
             if (!none) {
-                if (!wait_all(PVDONE(w), (n_s - 1) & 1)) {
+                if (!wait_all(PVDONE(w, 1), (n_s - 1) & 1)) {
                     ok = false;
                     break;
                 }
@@ -501,7 +607,8 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             // a row whose scores are all -inf has no weight to normalise by
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t at = (int64_t)tok * p.Hq + head;
-            const int64_t part = (int64_t)it.split * p.T * p.Hq + at;
+            // part of a cut item: the slice's first one if it begins before the slice, else its last
+            const int64_t rec = (int64_t)(2 * blockIdx.x + (it.t0 > 0 ? 0 : 1)) * kRows + w * kTile + row;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -513,7 +620,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
                 if (!valid) continue;
-                if (p.splits == 1) {
+                if (!it.cut) {
                     uint4* dst = reinterpret_cast<uint4*>(p.out + at * 128 + 32 * c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -525,7 +632,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
                     }
                 } else if (l != 0.f) {
-                    float4* dst = reinterpret_cast<float4*>(p.part_o + part * 128 + 32 * c);
+                    float4* dst = reinterpret_cast<float4*>(p.rec_o + rec * 128 + 32 * c);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
@@ -535,7 +642,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             ptx::tc_fence_before();
             if (valid) {
                 const float l2 = l == 0.f ? -INFINITY : m_ref + log2f(l);
-                if (p.splits > 1) p.part_lse[part] = l2;
+                if (it.cut) p.rec_lse[rec] = l2;
                 else if (p.lse != nullptr)
                     p.lse[p.cu ? (int64_t)head * p.T + tok : ((int64_t)it.b * p.Hq + head) * p.S + (tok - it.b * p.S)] =
                         l2 * 0.6931471805599453f;
@@ -550,44 +657,65 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     }
 }
 
-/* Joins the key ranges of one (token, head) per warp: out = sum_s 2^(l_s - l) O_s with
- * 2^l = sum_s 2^(l_s).  A range without keys has l_s = -inf and no O. */
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+/* Joins the parts of cut items: out = sum_s 2^(l_s - l) O_s with 2^l = sum_s 2^(l_s); a
+ * part without weight has l_s = -inf and no O.  Block (j, y) looks at the cut before slice
+ * j + 1: where it is the first inside its item, the block joins 32 of the item's rows, each
+ * thread 16 dimensions of one. */
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
+    __shared__ Slice a, nx;
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int64_t rows = (int64_t)p.T * p.Hq;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const int32_t tok = (int32_t)(row / p.Hq), head = (int32_t)(row - (int64_t)tok * p.Hq);
-    if (p.cu != nullptr && (tok < __ldg(p.cu) || tok >= __ldg(p.cu + p.B))) return;  // no sequence's
-    const float mine = lane < p.splits ? __ldcg(p.part_lse + lane * rows + row) : -INFINITY;
-    float m = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    // NaN ranges reach the sum through their own weight
+    const int32_t j = blockIdx.x;
+    find_slice<kJoinThreads>(p, j + 1, nx);
+    // (uniform) no such slice, or it begins with a whole item
+    if (nx.lo >= nx.hi || nx.item_lo == nx.lo) return;
+    find_slice<kJoinThreads>(p, j, a);
+    if (nx.item_lo < a.lo) return;  // an earlier cut is the item's first
+    // the item's parts: of slices j, j + 1, ... up to the one that holds its last tile
+    int32_t last = (int32_t)slice_owner(nx.item_lo + nx.item_len - 1, nx.n, nx.total);
+    const int64_t off = slice_begin(last, nx.n, nx.total) - nx.item_lo;
+    if (off > 0 && snapped(off, nx.item_len, snap_range(nx.n, nx.total)) == nx.item_len) --last;
+    const Seq q = load_seq(p, nx.b, false);
+    const int32_t unit = (int32_t)((nx.item_lo - nx.base) / q.n);
+    const int32_t kvh = unit / q.pairs, tok0 = q.tok0 + (unit - kvh * q.pairs) * 2 * p.tile_tokens;
+    const int32_t r = blockIdx.y * 32 + (threadIdx.x >> 3), d = (threadIdx.x & 7) * 16;
+    const int32_t w = r >> 7, row = r & (kTile - 1), t = row / p.g;
+    const int32_t tok = tok0 + w * p.tile_tokens + t, head = kvh * p.g + (row - t * p.g);
+    if (t >= p.tile_tokens || tok >= q.tok1) return;
+    auto rec_of = [&](int32_t c) { return (int64_t)(2 * c + (c == j ? 1 : 0)) * kRows + r; };
+    float m = -INFINITY;
+    for (int32_t c = j; c <= last; ++c) m = fmaxf(m, __ldcg(p.rec_lse + rec_of(c)));
     const float base = m == -INFINITY ? 0.f : m;
-    const float wgt = mine == -INFINITY ? 0.f : exp2f(mine - base);
-    float sum = wgt;
+    float sum = 0.f, acc[16];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-        const float ws = __shfl_sync(0xffffffffu, wgt, s);
-        if (__shfl_sync(0xffffffffu, mine, s) == -INFINITY) continue;
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 128) + lane);
-        acc.x = fmaf(ws, o.x, acc.x);
-        acc.y = fmaf(ws, o.y, acc.y);
-        acc.z = fmaf(ws, o.z, acc.z);
-        acc.w = fmaf(ws, o.w, acc.w);
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+    for (int32_t c = j; c <= last; ++c) {
+        const float l2 = __ldcg(p.rec_lse + rec_of(c));
+        if (l2 == -INFINITY) continue;
+        const float wgt = exp2f(l2 - base);  // NaN parts reach the result through their weight
+        sum += wgt;
+        const float4* src = reinterpret_cast<const float4*>(p.rec_o + rec_of(c) * 128 + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 o = __ldcg(src + i);
+            acc[4 * i] = fmaf(wgt, o.x, acc[4 * i]);
+            acc[4 * i + 1] = fmaf(wgt, o.y, acc[4 * i + 1]);
+            acc[4 * i + 2] = fmaf(wgt, o.z, acc[4 * i + 2]);
+            acc[4 * i + 3] = fmaf(wgt, o.w, acc[4 * i + 3]);
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    reinterpret_cast<uint2*>(p.out + row * 128)[lane] =
-        make_uint2(ptx::pack_bf16x2(acc.x * inv, acc.y * inv), ptx::pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (lane == 0 && p.lse != nullptr) {
+    uint4* dst = reinterpret_cast<uint4*>(p.out + ((int64_t)tok * p.Hq + head) * 128 + d);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        dst[i] = make_uint4(ptx::pack_bf16x2(acc[8 * i] * inv, acc[8 * i + 1] * inv),
+                            ptx::pack_bf16x2(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv),
+                            ptx::pack_bf16x2(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv),
+                            ptx::pack_bf16x2(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
+    if (d == 0 && p.lse != nullptr) {
         const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-        const int32_t b = p.cu ? 0 : tok / p.S;
-        p.lse[p.cu ? (int64_t)head * p.T + tok : ((int64_t)b * p.Hq + head) * p.S + (tok - b * p.S)] =
+        p.lse[p.cu ? (int64_t)head * p.T + tok : ((int64_t)nx.b * p.Hq + head) * p.S + (tok - nx.b * p.S)] =
             l2 * 0.6931471805599453f;
     }
 }
@@ -612,20 +740,13 @@ int encode(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, in
                : PGQA_ERR_CUDA;
 }
 
-/* Key ranges per (sequence, KV head, tile pair).  One as soon as the pairs fill the SMs;
- * else enough to fill them, of at least four key tiles (512 keys) each by the table's
- * capacity, so that an item's fixed cost (its Q tiles, its output) stays below its stream. */
-int splits_for(int64_t T, int64_t B, int64_t Hkv, int64_t g, int64_t cap_tokens, int sms) {
-    const int64_t per = 2 * (kTile / g);
-    int64_t pairs = (T + per - 1) / per;
-    if (pairs < B) pairs = B < T ? B : T;  // each sequence with a token has one
-    const int64_t items = pairs * Hkv;
-    if (items <= 0 || items * 2 > sms) return 1;
-    int64_t s = sms / items;
-    const int64_t most = cap_tokens / (4 * kTile);
-    if (s > most) s = most;
-    if (s > kMaxSplits) s = kMaxSplits;
-    return s < 1 ? 1 : (int)s;
+/* CTAs of the first launch: one per SM, or fewer where the key tiles are fewer (by the
+ * table's capacity). */
+int grid_for(int64_t T, int64_t B, int64_t Hkv, int64_t g, int64_t cap_tokens, int sms) {
+    const int64_t items = (T / (2 * (kTile / g)) + B) * Hkv;  // at least as many as there are
+    const int64_t tiles = (cap_tokens + kTile - 1) / kTile;
+    return items >= sms || tiles >= sms ? sms : (int)(items * tiles / kMinTiles < 1 ? 1 :
+           (items * tiles / kMinTiles < sms ? items * tiles / kMinTiles : sms));
 }
 
 int shape_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t bt_stride) {
@@ -636,9 +757,7 @@ int shape_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t P
     return PGQA_OK;
 }
 
-size_t workspace_bytes(int64_t T, int64_t Hq, int splits) {
-    return splits > 1 ? (size_t)splits * (size_t)T * (size_t)Hq * (128 + 1) * 4 : 0;
-}
+size_t workspace_bytes(int grid) { return (size_t)2 * grid * kRows * (128 + 1) * 4; }
 
 int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (a == nullptr) return PGQA_ERR_NULL_POINTER;
@@ -664,17 +783,14 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if ((st = host_error_word(dev, &p.err)) != PGQA_OK) return st;
     if (a->tokens == 0) return PGQA_OK;
     // items are counted in 32 bits
-    if ((a->tokens / (kTile / (a->num_heads / a->num_heads_k)) + a->batch_size) * a->num_heads_k * kMaxSplits > INT32_MAX)
+    if ((a->tokens / (kTile / (a->num_heads / a->num_heads_k)) + a->batch_size) * a->num_heads_k > INT32_MAX)
         return PGQA_ERR_UNSUPPORTED;
     p.g = (int32_t)(a->num_heads / a->num_heads_k);
     p.cap_tokens = a->bt_stride * a->page_size;
-    p.splits = splits_for(a->tokens, a->batch_size, a->num_heads_k, p.g, p.cap_tokens, sms);
-    if (p.splits > 1) {
-        const size_t need = workspace_bytes(a->tokens, a->num_heads, p.splits);
-        if (a->workspace == nullptr || a->workspace_bytes < need) return PGQA_ERR_WORKSPACE;
-        p.part_o = static_cast<float*>(a->workspace);
-        p.part_lse = p.part_o + (size_t)p.splits * a->tokens * a->num_heads * 128;
-    }
+    p.grid = grid_for(a->tokens, a->batch_size, a->num_heads_k, p.g, p.cap_tokens, sms);
+    if (a->workspace == nullptr || a->workspace_bytes < workspace_bytes(p.grid)) return PGQA_ERR_WORKSPACE;
+    p.rec_o = static_cast<float*>(a->workspace);
+    p.rec_lse = p.rec_o + (size_t)2 * p.grid * kRows * 128;
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.lse = a->softmax_lse;
     p.seq_lens = a->seq_lens;
@@ -704,12 +820,9 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
         return st;
     static int done[kHostMaxDevices] = {0};
     if ((st = host_smem_limit(cross_kernel, dev, kSmem, done)) != PGQA_OK) return st;
-    const int64_t per = 2 * p.tile_tokens;
-    int64_t ctas = (a->tokens / per + a->batch_size) * a->num_heads_k * p.splits;  // at least the items
-    if (ctas > sms) ctas = sms;
-    st = host_launch(cross_kernel, dim3((unsigned)ctas), kThreads, kSmem, stream, 1, qm, km, vm, p);
-    if (st != PGQA_OK || p.splits == 1) return st;
-    return host_launch(join_kernel, dim3((unsigned)((a->tokens * a->num_heads + 7) / 8)), 256, 0, stream, 1, p);
+    st = host_launch(cross_kernel, dim3((unsigned)p.grid), kThreads, kSmem, stream, 1, qm, km, vm, p);
+    if (st != PGQA_OK || p.grid == 1) return st;
+    return host_launch(join_kernel, dim3((unsigned)(p.grid - 1), kRows / 32), kJoinThreads, 0, stream, 1, p);
 }
 
 }  // namespace cross
@@ -723,9 +836,8 @@ extern "C" size_t pgqa_cross_workspace_size(int64_t tokens, int64_t batch_size, 
     int dev, sms = 0, optin;
     if (st == PGQA_OK) st = host_device(&dev, &sms, &optin);
     if (host_set_status(st) != PGQA_OK || tokens == 0) return 0;
-    return cross::workspace_bytes(tokens, num_heads,
-                                  cross::splits_for(tokens, batch_size, num_heads_k, num_heads / num_heads_k,
-                                                    bt_stride * page_size, sms));
+    return cross::workspace_bytes(cross::grid_for(tokens, batch_size, num_heads_k, num_heads / num_heads_k,
+                                                  bt_stride * page_size, sms));
 }
 
 extern "C" int pgqa_cross_attention(const pgqa_cross_args* args, void* stream) {

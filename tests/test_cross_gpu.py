@@ -109,6 +109,14 @@ def test_few_tokens_over_long_keys(lens, cuda_device):
     run_and_check(make([3, 9], lens, 8, 2, 16, seed=4), cuda_device)
 
 
+@pytest.mark.parametrize("new,lens,Hq,Hkv", [
+    ([1], [100000], 2, 1),                 # one item over every SM
+    ([2], [37000], 8, 1), ([1, 1], [50000, 100], 4, 2), ([70, 3, 500], [9000, 20000, 700], 4, 1),
+    ([33] * 40, [300 + 97 * i for i in range(40)], 8, 2), ([200], [18944], 4, 1), ([260, 5], [129, 40000], 6, 2)])
+def test_items_cut_between_ctas(new, lens, Hq, Hkv, cuda_device):
+    run_and_check(make(new, lens, Hq, Hkv, 16, seed=sum(lens)), cuda_device)
+
+
 def test_growing_scores_move_the_maximum(cuda_device):
     """Keys that grow along the sequence: the running maximum moves in every tile."""
     case = list(make([100], [1500], 4, 1, 16, seed=5))
