@@ -16,21 +16,23 @@
  * that is cut all the same leaves its parts' normalised O (fp32) and log-sum-exps in the
  * workspace, and a second launch joins them.  Every role of a CTA walks the same items:
  *
- *   warps 0-3, 4-7  softmax and output of tile 0 and tile 1: thread = row = TMEM lane, 64
- *                   keys at a time.  The running maximum is moved only when a score exceeds
- *                   it by 2^8 (O is then rescaled in TMEM), so the O accumulator is touched
- *                   once per item in the usual case; sums and statistics are fp32, P is
- *                   rounded to bf16 (2^-8 relative at most, of weights that are summed in
- *                   fp32) and goes back to TMEM over the scores it came from.
+ *   warps 0-3, 4-7  softmax and output of tile 0 and tile 1: thread = row = TMEM lane, a
+ *                   step of 64 keys at a time.  The running maximum is moved only when a
+ *                   score exceeds it by 2^8 (O is then rescaled in TMEM), so the O
+ *                   accumulator is touched once per item in the usual case; sums and
+ *                   statistics are fp32, P is rounded to bf16 (2^-8 relative at most, of
+ *                   weights that are summed in fp32) and goes back to TMEM over the scores it
+ *                   came from.
  *   warp 8          TMA: Q tiles, and 128-key tiles of K and V by page boxes through one
  *                   ring of five 32 KB slots; it zeroes V rows behind the last key, so that
  *                   a weight of 0 never meets a NaN left in a page.
- *   warp 9          issues the MMAs (one thread): S_w = Q_w K^T (both from shared memory),
- *                   O_w += P_w V (P from TMEM), the latter 64 keys at a time, as soon as
- *                   their weights are there.  The score tile of the next keys is issued
- *                   right behind the PV of the present ones, and the two tiles alternate,
- *                   so the tensor core works for one while the other's softmax runs.
- * TMEM: S and P of the tiles at columns 0 and 128, O at 256 and 384.
+ *   warps 9, 10     issue the MMAs of tile 0 and of tile 1: S = Q K^T (both from shared
+ *                   memory), O += P V (P from TMEM).
+ * TMEM: two score buffers of 64 columns for each tile (from columns 0 and 128), O at 256 and
+ * 384.  The scores of step i + 2 are issued right behind the PV of step i, which frees their
+ * buffer, so while a warpgroup works on step i + 1 its next scores are computed and neither
+ * waits for the other.  The price is QK^T with N = 64, which re-reads Q from shared memory
+ * twice as often: 48 clocks an MMA instead of 32.
  *
  * Every wait is bounded: one that expires sets the device error word and the CTA's abort
  * flag, every role leaves its loop, loads and MMAs in flight are drained and TMEM is freed.
@@ -49,13 +51,14 @@
 namespace pgqa {
 namespace cross {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;
 constexpr int kTile = 128;                 // rows of a tile, and keys of a K / V tile
 constexpr int kHalf = kTile * 128;         // one 64-dimension half of a tile, bf16
 constexpr int kSlot = 2 * kHalf;
 constexpr int kSlots = 5;
 constexpr int kQOff = 0, kRingOff = 2 * kSlot, kBarOff = kRingOff + kSlots * kSlot;
-constexpr int kBars = 2 * kSlots + 14;
+constexpr int kStep = 64;                  // keys of a softmax step
+constexpr int kBars = 2 * kSlots + 16;
 constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
 constexpr int kRows = 2 * kTile;           // rows of a work item
 constexpr int kMinTiles = 2;               // key tiles of a slice, at least
@@ -82,9 +85,13 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t 
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
            ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-/* fp32 accumulator, bf16 A and B, M = N = 128; B major: 0 = K, 1 = N */
-__host__ __device__ constexpr uint32_t idesc(uint32_t b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+/* fp32 accumulator, bf16 A and B, M = 128; B major: 0 = K, 1 = N */
+__host__ __device__ constexpr uint32_t idesc(uint32_t b_mn, uint32_t n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+/* Steps of an item's key tiles [t0, t1): the last one may have a single one. */
+__device__ __forceinline__ int steps_of(int32_t L, int32_t t0, int32_t t1) {
+    return t1 == t0 ? 0 : 2 * (t1 - t0) - (L - (t1 - 1) * kTile <= kStep ? 1 : 0);
 }
 
 /* A sequence's prompt tokens [tok0, tok1), keys L, key tiles n (at least 1), items. */
@@ -250,35 +257,38 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     const uint32_t bars = sb + kBarOff;
     auto FULL = [&](int s) { return bars + 8u * s; };
     auto EMPTY = [&](int s) { return bars + 8u * (kSlots + s); };
-    auto SFULL = [&](int w) { return bars + 8u * (2 * kSlots + w); };
-    // of tile w and keys [0, 64) or [64, 128) of a key tile
-    auto PFULL = [&](int w, int h) { return bars + 8u * (2 * kSlots + 2 + 2 * w + h); };
-    auto PVDONE = [&](int w, int h) { return bars + 8u * (2 * kSlots + 6 + 2 * w + h); };
-    const uint32_t QFULL = bars + 8u * (2 * kSlots + 10), QEMPTY = bars + 8u * (2 * kSlots + 11);
-    const uint32_t TAIL = bars + 8u * (2 * kSlots + 12), MMADONE = bars + 8u * (2 * kSlots + 13);
+    // score buffer u of tile w
+    auto SFULL = [&](int w, int u) { return bars + 8u * (2 * kSlots + 2 * w + u); };
+    auto PFULL = [&](int w, int u) { return bars + 8u * (2 * kSlots + 4 + 2 * w + u); };
+    // one per buffer: when the scores in a buffer are there, the PV before the last is done,
+    // so a wait for the last one cannot take an earlier phase for it
+    auto PVDONE = [&](int w, int u) { return bars + 8u * (2 * kSlots + 8 + 2 * w + u); };
+    const uint32_t QFULL = bars + 8u * (2 * kSlots + 12), QEMPTY = bars + 8u * (2 * kSlots + 13);
+    const uint32_t TAIL = bars + 8u * (2 * kSlots + 14), MMADONE = bars + 8u * (2 * kSlots + 15);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarOff + kBars * 8);
     volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
     if (tid == 0) {
         ptx::prefetch_tensormap(&qmap);
         ptx::prefetch_tensormap(&kmap);
         ptx::prefetch_tensormap(&vmap);
         for (int s = 0; s < kSlots; ++s) {
             ptx::mbar_init(FULL(s), 1);
-            ptx::mbar_init(EMPTY(s), 1);
+            ptx::mbar_init(EMPTY(s), 2);  // both tiles are done with it
         }
         for (int w = 0; w < 2; ++w) {
-            ptx::mbar_init(SFULL(w), 1);
-            for (int h = 0; h < 2; ++h) {
-                ptx::mbar_init(PFULL(w, h), 4);  // one arrival per warp
-                ptx::mbar_init(PVDONE(w, h), 1);
+            for (int u = 0; u < 2; ++u) {
+                ptx::mbar_init(SFULL(w, u), 1);
+                ptx::mbar_init(PFULL(w, u), 4);  // one arrival per warp
+                ptx::mbar_init(PVDONE(w, u), 1);
             }
         }
         ptx::mbar_init(QFULL, 1);
-        ptx::mbar_init(QEMPTY, 1);
+        ptx::mbar_init(QEMPTY, 2);
         ptx::mbar_init(TAIL, 1);
-        ptx::mbar_init(MMADONE, 1);
+        ptx::mbar_init(MMADONE, 2);
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -289,7 +299,12 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    // all 512 columns: the allocation starts at column 0, so every TMEM address is a constant
+    constexpr uint32_t tmem = 0;
+    if (tid == 0 && *tmem_slot != tmem) {
+        *abort_flag = 1;
+        atomicOr(p.err, kDevErrTimeout);
+    }
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
 
@@ -434,82 +449,88 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if (n_q > 0) drain_bar(QFULL, (n_q - 1) & 1);
         }
         __syncwarp();
-    } else if (warp == 9) {
-        /* ================= MMA issuer ================= */
-        int n_kv = 0, n_q = 0, n_s[2] = {0, 0};
+    } else if (warp >= 9) {
+        /* ================= MMA issuers: warp 9 tile 0, warp 10 tile 1 ================= */
+        const int w = warp - 9;
+        const uint32_t tS = tmem + (uint32_t)w * 128u, tO = tmem + 256u + (uint32_t)w * 128u;
+        const uint64_t qd = sdesc(sb + kQOff + (uint32_t)w * kSlot, 16, 1024);
+        const uint64_t kd = sdesc(sb + kRingOff, 16, 1024), vd = sdesc(sb + kRingOff, kHalf, 1024);
+        // ring places of the next K and V tile (loads alternate: K, V, K, V ...), their phases
+        int ks = 0, vs = 1, n_q = 0, n = 0;  // Q loads, steps so far
+        uint32_t kph = 0, vph = 0;
         bool ok = true;
-        auto qk = [&](int w, int slot) {
-            const uint32_t qb = sb + kQOff + (uint32_t)w * kSlot, kb = sb + kRingOff + (uint32_t)slot * kSlot;
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                const uint32_t o = (uint32_t)((ks >> 2) * kHalf + (ks & 3) * 32);
-                ptx::tc_mma_f16(tmem + (uint32_t)w * 128u, sdesc(qb + o, 16, 1024), sdesc(kb + o, 16, 1024), idesc(0),
-                                ks > 0 ? 1u : 0u);
+        auto advance = [&](int& slot, uint32_t& phase) {
+            slot += 2;
+            if (slot >= kSlots) {
+                slot -= kSlots;
+                phase ^= 1u;
             }
-        };
-        // 16-key steps [k0, k1) of a tile
-        auto pv = [&](int w, int slot, int k0, int k1, bool first) {
-            const uint32_t vb = sb + kRingOff + (uint32_t)slot * kSlot;
-            for (int ks = k0; ks < k1; ++ks)
-                ptx::tc_mma_f16_ts(tmem + 256u + (uint32_t)w * 128u, tmem + (uint32_t)(w * 128 + ks * 8),
-                                   sdesc(vb + (uint32_t)ks * 2048u, kHalf, 1024), idesc(1), (first && ks == 0) ? 0u : 1u);
         };
         while (ok && wk.next(p, lane, it)) {
-            const int n = it.t1 - it.t0;
-            if (n == 0) continue;
-            if (lane == 0) {
-                const int last = it.tok0 + p.tile_tokens < it.tok_end ? 1 : 0;  // last active tile
-                do {
-                    ok = wait_bar(QFULL, n_q & 1) && wait_bar(FULL(n_kv % kSlots), (n_kv / kSlots) & 1);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
-                    for (int w = 0; w <= last; ++w) {
-                        qk(w, n_kv % kSlots);
-                        ptx::tc_commit(SFULL(w));
-                    }
-                    ptx::tc_commit(EMPTY(n_kv % kSlots));
-                    if (n == 1) ptx::tc_commit(QEMPTY);
-                    for (int j = 0; j < n && ok; ++j) {
-                        const int kv_v = n_kv + 2 * j + 1, kv_k = kv_v + 1;
-                        const int nvalid = min(kTile, it.L - (it.t0 + j) * kTile);
-                        for (int w = 0; w <= last; ++w) {
-                            const int steps = (nvalid + 15) >> 4;
-                            ok = wait_bar(PFULL(w, 0), n_s[w] & 1) &&
-                                 (w > 0 || wait_bar(FULL(kv_v % kSlots), (kv_v / kSlots) & 1));
-                            if (!ok) break;
-                            ptx::tc_fence_after();
-                            pv(w, kv_v % kSlots, 0, min(4, steps), j == 0);
-                            ptx::tc_commit(PVDONE(w, 0));
-                            ok = wait_bar(PFULL(w, 1), n_s[w] & 1);
-                            if (!ok) break;
-                            ++n_s[w];
-                            ptx::tc_fence_after();
-                            pv(w, kv_v % kSlots, 4, steps, false);
-                            ptx::tc_commit(PVDONE(w, 1));
-                            if (w == last) ptx::tc_commit(EMPTY(kv_v % kSlots));
-                            if (j + 1 < n) {
-                                ok = w > 0 || wait_bar(FULL(kv_k % kSlots), (kv_k / kSlots) & 1);
-                                if (!ok) break;
-                                ptx::tc_fence_after();
-                                qk(w, kv_k % kSlots);
-                                ptx::tc_commit(SFULL(w));
-                                if (w == last) {
-                                    ptx::tc_commit(EMPTY(kv_k % kSlots));
-                                    if (j + 2 == n) ptx::tc_commit(QEMPTY);
-                                }
-                            }
-                        }
-                    }
-                } while (false);
-            }
-            n_kv += 2 * n;
+            const int m = __shfl_sync(0xffffffffu, steps_of(it.L, it.t0, it.t1), 0);
+            if (m == 0) continue;
+            const bool active = __shfl_sync(0xffffffffu, it.tok0 + w * p.tile_tokens < it.tok_end ? 1 : 0, 0) != 0;
+            const int keys = __shfl_sync(0xffffffffu, it.L - it.t0 * kTile, 0);
+            ok = wait_all(QFULL, n_q & 1);
             ++n_q;
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (!active) {  // nothing but the releases
+                for (int i = 0; i < m && ok; i += 2) {
+                    ok = wait_all(FULL(ks), kph);
+                    if (ok && lane == 0) ptx::mbar_arrive(EMPTY(ks));
+                    ok = ok && wait_all(FULL(vs), vph);
+                    if (ok && lane == 0) ptx::mbar_arrive(EMPTY(vs));
+                    advance(ks, kph);
+                    advance(vs, vph);
+                }
+                if (ok && lane == 0) ptx::mbar_arrive(QEMPTY);
+                continue;
+            }
+            // step i of the item: scores of keys [64 i, 64 i + 64) into buffer (n + i) & 1
+            auto qk = [&](int i) -> bool {
+                const int h = i & 1, u = (n + i) & 1;
+                if (h == 0 && !wait_all(FULL(ks), kph)) return false;
+                ptx::tc_fence_after();
+                const uint64_t k = kd + (uint64_t)((ks * kSlot + h * (kStep * 128)) >> 4);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const uint64_t o = (uint64_t)((x >> 2) * kHalf + (x & 3) * 32) >> 4;
+                    ptx::tc_mma_f16_elect(tS + (uint32_t)(u * kStep), qd + o, k + o, idesc(0, kStep), x > 0 ? 1u : 0u);
+                }
+                ptx::tc_commit_elect(SFULL(w, u));
+                if (h == 1 || i + 1 == m) {
+                    ptx::tc_commit_elect(EMPTY(ks));
+                    advance(ks, kph);
+                    if (i + 1 == m) ptx::tc_commit_elect(QEMPTY);
+                }
+                return true;
+            };
+            ok = ok && qk(0);
+            if (m > 1) ok = ok && qk(1);
+#pragma unroll 1
+            for (int i = 0; i < m && ok; ++i) {
+                const int h = i & 1, u = (n + i) & 1;
+                ok = (h == 1 || wait_all(FULL(vs), vph)) && wait_all(PFULL(w, u), ((n + i) >> 1) & 1);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                const uint64_t v = vd + (uint64_t)((vs * kSlot + h * (kStep * 128)) >> 4);
+                const int left = keys - i * kStep, k16 = left >= kStep ? kStep / 16 : (left + 15) >> 4;
+#pragma unroll
+                for (int x = 0; x < kStep / 16; ++x)
+                    if (x < k16)
+                        ptx::tc_mma_f16_ts_elect(tO, tS + (uint32_t)(u * kStep + x * 8), v + (uint64_t)(x * 128),
+                                                 idesc(1, 128), (i == 0 && x == 0) ? 0u : 1u);
+                ptx::tc_commit_elect(PVDONE(w, u));
+                if (h == 1 || i + 1 == m) {
+                    ptx::tc_commit_elect(EMPTY(vs));
+                    advance(vs, vph);
+                }
+                if (i + 2 < m) ok = qk(i + 2);
+            }
+            n += m;
         }
-        if (lane == 0) {  // every MMA issued is complete before TMEM is freed
-            ptx::tc_commit(MMADONE);
-            drain_bar(MMADONE, 0);
-        }
+        // every MMA issued is complete before TMEM is freed
+        ptx::tc_commit_elect(MMADONE);
+        if (lane == 0) drain_bar(MMADONE, 0);
         __syncwarp();
     } else {
         /* ================= softmax and output ================= */
@@ -518,7 +539,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = (tmem + (uint32_t)w * 128u) | lanes, tO = (tmem + 256u + (uint32_t)w * 128u) | lanes;
         const int my_tok = row / p.g, my_head = row - my_tok * p.g;
-        int n_s = 0;  // key tiles seen by this tile so far
+        int n_s = 0;  // steps of this tile so far
         bool ok = true;
         while (ok && wk.next(p, lane, it)) {
             const int32_t first = it.tok0 + w * p.tile_tokens;
@@ -527,78 +548,84 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const bool valid = row < p.tile_tokens * p.g && tok < it.tok_end;
             const int head = it.kvh * p.g + my_head;
             float m_ref = -INFINITY, l = 0.f;
-            for (int32_t tile = it.t0; tile < it.t1; ++tile, ++n_s) {
-                if (!wait_all(SFULL(w), n_s & 1)) {
+            const int m = steps_of(it.L, it.t0, it.t1);
+#pragma unroll 1
+            for (int i = 0; i < m; ++i, ++n_s) {
+                const uint32_t tB = tS + (uint32_t)((n_s & 1) * kStep);
+                if (!wait_all(SFULL(w, n_s & 1), (n_s >> 1) & 1)) {
                     ok = false;
                     break;
                 }
                 ptx::tc_fence_after();
-                const int32_t nvalid = it.L - tile * kTile;
-                float s[64];
+                float s[kStep];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int c = 0; c < 2; ++c)
+                    ptx::tc_ld32(tB + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                ptx::tc_wait_ld();
+                const int32_t nvalid = it.L - (it.t0 * kTile + i * kStep);
+                if (nvalid < kStep) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        ptx::tc_ld32(tS + 64u * h + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-                    ptx::tc_wait_ld();
-                    if (nvalid < kTile) {
+                    for (int k = 0; k < kStep; ++k) s[k] = k < nvalid ? s[k] : -INFINITY;
+                }
+                // eight chains of three-operand maxima
+                float m8[8];
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) s[i] = 64 * h + i < nvalid ? s[i] : -INFINITY;
-                    }
-                    float m4[4] = {s[0], s[1], s[2], s[3]};
+                for (int e = 0; e < 8; ++e) m8[e] = fmaxf(fmaxf(s[e], s[8 + e]), s[16 + e]);
 #pragma unroll
-                    for (int i = 4; i < 64; ++i) m4[i & 3] = fmaxf(m4[i & 3], s[i]);
-                    const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
-                    const bool raise = mx > m_ref + kLazyLog2;
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float m_new = raise ? mx : m_ref;
-                        const float alpha = raise ? ptx::ex2(m_ref - m_new) : 1.f;
-                        m_ref = m_new;
-                        l *= alpha;
-                        if (tile > it.t0 || h > 0) {
-                            // the products so far: of the 64 keys before these
-                            if (!wait_all(PVDONE(w, h ^ 1), (h ? n_s : n_s - 1) & 1)) {
-                                ok = false;
-                                break;
-                            }
-                            ptx::tc_fence_after();
+                for (int k = 24; k < 56; k += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m8[e] = fmaxf(fmaxf(m8[e], s[k + e]), s[k + 8 + e]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m8[e] = fmaxf(m8[e], s[56 + e]);
+                const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
+                const bool raise = mx > m_ref + kLazyLog2;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float m_new = raise ? mx : m_ref;
+                    const float alpha = raise ? ptx::ex2(m_ref - m_new) : 1.f;
+                    m_ref = m_new;
+                    l *= alpha;
+                    if (i > 0) {  // the products so far
+                        if (!wait_all(PVDONE(w, (n_s - 1) & 1), ((n_s - 1) >> 1) & 1)) {
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < 8; ++c) {
-                                float o[16];
-                                ptx::tc_ld16(tO + 16u * c, o);
-                                ptx::tc_wait_ld();
+                        for (int c = 0; c < 8; ++c) {
+                            float o[16];
+                            ptx::tc_ld16(tO + 16u * c, o);
+                            ptx::tc_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) o[i] *= alpha;
-                                ptx::tc_st16(tO + 16u * c, o);
-                            }
+                            for (int k = 0; k < 16; ++k) o[k] *= alpha;
+                            ptx::tc_st16(tO + 16u * c, o);
                         }
                     }
-                    const float base = m_ref == -INFINITY ? 0.f : m_ref;
-                    const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
-                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float2 x = ptx::fma2(make_float2(s[2 * i], s[2 * i + 1]), mul2, sub2);
-                        x.x = ptx::ex2(x.x);
-                        x.y = ptx::ex2(x.y);
-                        sum[i & 1] = ptx::add2(sum[i & 1], x);
-                        pk[i] = ptx::pack_bf16x2(x.x, x.y);
-                    }
-                    ptx::tc_st32(tS + 32u * h, pk);
-                    sum[0] = ptx::add2(sum[0], sum[1]);
-                    l += sum[0].x + sum[0].y;
-                    ptx::tc_wait_st();
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(PFULL(w, h));
                 }
-                if (!ok) break;
+                const float base = m_ref == -INFINITY ? 0.f : m_ref;
+                const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                uint32_t pk[kStep / 2];
+#pragma unroll
+                for (int k = 0; k < kStep / 2; ++k) {
+                    float2 x = ptx::fma2(make_float2(s[2 * k], s[2 * k + 1]), mul2, sub2);
+                    x.x = ptx::ex2(x.x);
+                    x.y = ptx::ex2(x.y);
+                    sum[k & 1] = ptx::add2(sum[k & 1], x);
+                    pk[k] = ptx::pack_bf16x2(x.x, x.y);
+                }
+                ptx::tc_st32(tB, pk);
+                sum[0] = ptx::add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
+                ptx::tc_wait_st();
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(PFULL(w, n_s & 1));
             }
             if (!ok) break;
             const bool none = !(it.t1 > it.t0);
             if (!none) {
-                if (!wait_all(PVDONE(w, 1), (n_s - 1) & 1)) {
+                if (!wait_all(PVDONE(w, (n_s - 1) & 1), ((n_s - 1) >> 1) & 1)) {
                     ok = false;
                     break;
                 }
@@ -653,7 +680,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     __syncthreads();
     if (warp == 9) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem, 512);
+        ptx::tmem_dealloc(*tmem_slot, 512);
     }
 }
 

@@ -398,14 +398,32 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32])
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-/* D[tmem] (+)= A[tmem] x B[smem desc], 16-bit inputs: lane m of A holds row m, each 32-bit
- * column two consecutive K elements (the lower one in the low half). */
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                              uint32_t acc) {
+/* Forms for a converged warp, of which one elected lane issues: the operands are the same in
+ * all lanes and stay in uniform registers.  Issued so, MMAs follow each other at the tensor
+ * core's rate (M = N = 128, K = 16: 64 clocks); behind a branch on the lane number, or with
+ * such a predicate in a rolled loop, 81 to 87 clocks. */
+__device__ __forceinline__ void tc_mma_f16_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                                 uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+/* A from TMEM: lane m of A holds row m, each 32-bit column two consecutive K elements (the
+ * lower one in the low half). */
+__device__ __forceinline__ void tc_mma_f16_ts_elect(uint32_t d, uint32_t a, uint64_t b,
+                                                    uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_elect(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
