@@ -11,10 +11,11 @@
  * that all rows of a KV head share.  The g query heads of a KV head are rows of one tile
  * (row = token * g + head), so a 128-row tile holds 128 / g tokens and K and V are read
  * once per 256 rows.  A work item is (sequence, KV head, two such tiles).  The items' key
- * tiles, one after the other, are cut into equal slices, one per persistent CTA (one CTA per
- * SM); a cut that would fall within 1/24 of a slice of an item's end is moved there.  An item
- * that is cut all the same leaves its parts' normalised O (fp32) and log-sum-exps in the
- * workspace, and a second launch joins them.  Every role of a CTA walks the same items:
+ * tiles, one after the other, each item's with kItemCost more for its Q tiles and its output,
+ * are cut into equal slices, one per persistent CTA (one CTA per SM); a cut that would fall
+ * within 1/24 of a slice of an item's end is moved there.  An item that is cut all the same
+ * leaves its parts' normalised O (fp32) and log-sum-exps in the workspace, and a second
+ * launch joins them.  Every role of a CTA walks the same items:
  *
  *   warps 0-3, 4-7  softmax and output of tile 0 and tile 1: thread = row = TMEM lane, a
  *                   step of 64 keys at a time.  The running maximum is moved only when a
@@ -61,7 +62,9 @@ constexpr int kStep = 64;                  // keys of a softmax step
 constexpr int kBars = 2 * kSlots + 16;
 constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
 constexpr int kRows = 2 * kTile;           // rows of a work item
-constexpr int kMinTiles = 2;               // key tiles of a slice, at least
+// What an item costs beside its key tiles, in key tiles (1 to 4 measured: 175, 159, 167, 166 us
+// for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys), and the least length of a slice.
+constexpr int kItemCost = 2, kMinSlice = 3;
 constexpr int kSnap = 24;
 constexpr float kLazyLog2 = 8.f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
@@ -71,6 +74,7 @@ struct Params {
     float* lse;              // optional: [Hq, T] packed, [B, Hq, S] padded
     float *rec_o, *rec_lse;  // parts of cut items: [2 * grid][256 rows][128], [2 * grid][256] (log2 units)
     const int32_t *seq_lens, *block_table, *cu;
+    struct Cut* cuts;        // [grid]
     int32_t* err;
     int64_t bt_stride, cap_tokens;
     int32_t B, S, T, Hq, Hkv, g, P, page_shift, num_pages;
@@ -94,10 +98,12 @@ __device__ __forceinline__ int steps_of(int32_t L, int32_t t0, int32_t t1) {
     return t1 == t0 ? 0 : 2 * (t1 - t0) - (L - (t1 - 1) * kTile <= kStep ? 1 : 0);
 }
 
-/* A sequence's prompt tokens [tok0, tok1), keys L, key tiles n (at least 1), items. */
+/* A sequence's prompt tokens [tok0, tok1), keys L, key tiles n (at least 1), items (all tile
+ * pairs of a KV head, then of the next). */
 struct Seq {
     int32_t tok0, tok1, L, n, pairs, items;
-    __device__ int64_t tiles() const { return (int64_t)items * n; }
+    __device__ int32_t len() const { return n + kItemCost; }  // of an item
+    __device__ int64_t size() const { return (int64_t)items * len(); }
 };
 
 __device__ __forceinline__ Seq load_seq(const Params& p, int32_t b, bool report) {
@@ -121,30 +127,30 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int32_t b, bool report)
     return q;
 }
 
-/* Slice [lo, hi) of CTA c of the n active ones, and the item at each end. */
+/* Slice [lo, hi) of CTA c of the n active ones, and the item at its start. */
 struct Slice {
     int64_t lo, hi;
-    int64_t base;            // first tile of sequence b, which holds tile lo
+    int64_t base;               // start of sequence b, which holds lo
+    int64_t item_lo, item_len;  // the item that holds lo: its start, its length
+    int64_t n, total;           // active CTAs, length of all slices
     int32_t b;
-    int64_t item_lo, item_len;  // the item that holds tile lo: its first tile, its length
-    int64_t n, total;        // active CTAs, tiles of all slices
 };
 
-/* A cut at most 1/kSnap of a slice away from an item's end is moved there. */
+/* A cut at most 1/kSnap of a slice away from an item's end is moved there, as is one before
+ * the item's first key tile. */
 __device__ __forceinline__ int64_t snap_range(int64_t n, int64_t total) { return total / n / kSnap; }
 __device__ __forceinline__ int64_t snapped(int64_t off, int64_t len, int64_t tol) {
-    return off <= tol ? 0 : (len - off <= tol ? len : off);
+    return off <= max(tol, (int64_t)kItemCost) ? 0 : (len - off <= tol ? len : off);
 }
 
 /* By all threads of a block (a multiple of 32, at most 1024); the result in shared memory. */
-template <int kT>
 __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
-    __shared__ int64_t wsum[kT / 32];
+    __shared__ int64_t wsum[kThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (p.B + kT - 1) / kT;
+    const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
     int64_t local = 0;
-    for (int b = b0; b < b1; ++b) local += load_seq(p, b, blockIdx.x == 0).tiles();
+    for (int b = b0; b < b1; ++b) local += load_seq(p, b, blockIdx.x == 0).size();
     int64_t incl = local;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -154,11 +160,11 @@ __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
     if (lane == 31) wsum[warp] = incl;
     __syncthreads();
     int64_t run = incl - local, total = 0;
-    for (int w = 0; w < kT / 32; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) run += wsum[w];
         total += wsum[w];
     }
-    int64_t n = total / kMinTiles;
+    int64_t n = total / kMinSlice;
     n = n < 1 ? 1 : (n > p.grid ? p.grid : n);
     if (tid == 0) {
         out.n = n;
@@ -171,18 +177,18 @@ __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
         if (tid == 0 && c + 1 == n) out.hi = total;
         for (int b = b0; b < b1; ++b) {
             const Seq q = load_seq(p, b, false);
-            const int64_t end = run + q.tiles();
+            const int64_t end = run + q.size();
             auto snap = [&](int64_t x) {
-                const int64_t off = (x - run) % q.n;
-                return x - off + snapped(off, q.n, tol);
+                const int64_t off = (x - run) % q.len();
+                return x - off + snapped(off, q.len(), tol);
             };
             if (run <= x0 && x0 < end) {
                 const int64_t lo = snap(x0);
                 out.lo = lo;
                 out.base = run;
                 out.b = b;
-                out.item_lo = lo - (lo - run) % q.n;
-                out.item_len = q.n;
+                out.item_lo = lo - (lo - run) % q.len();
+                out.item_len = q.len();
             }
             if (c + 1 < n && run <= x1 && x1 < end) out.hi = snap(x1);
             run = end;
@@ -198,9 +204,9 @@ struct Item {
 
 /* Walks a slice's items; called by whole warps, every role with a copy of its own. */
 struct Walker {
-    int64_t pos, hi, base;
-    int32_t b;
-    Seq mine, cur;  // this lane's of the 32 sequences from b - cur_lane, and the one at work
+    int64_t left;             // of the slice
+    int32_t b, kvh, pair, off;  // the next item, and where in it the slice goes on
+    Seq mine, cur;            // this lane's of the 32 sequences from b - cur_lane, and the one at work
     int cur_lane;
     __device__ void pick() {
         cur.tok0 = __shfl_sync(0xffffffffu, mine.tok0, cur_lane);
@@ -211,42 +217,86 @@ struct Walker {
         cur.items = __shfl_sync(0xffffffffu, mine.items, cur_lane);
     }
     __device__ void init(const Params& p, const Slice& s, int lane) {
-        pos = s.lo;
-        hi = s.hi;
-        base = s.base;
+        left = s.hi - s.lo;
         b = s.b;
         cur_lane = 0;
-        if (pos < hi) {
+        kvh = pair = off = 0;
+        if (left > 0) {
             mine = load_seq(p, b + lane, false);
             pick();
+            const int64_t in = s.lo - s.base;  // a cut moved to the sequence's end: kvh = Hkv
+            const int32_t unit = (int32_t)(in / cur.len());
+            off = (int32_t)(in - (int64_t)unit * cur.len());
+            kvh = unit / cur.pairs;
+            pair = unit - kvh * cur.pairs;
         }
     }
     __device__ bool next(const Params& p, int lane, Item& it) {
-        if (pos >= hi) return false;
-        while (pos >= base + cur.tiles()) {
-            base += cur.tiles();
-            ++b;
-            if (++cur_lane == 32) {
-                cur_lane = 0;
-                mine = load_seq(p, b + lane, false);
-            }
-            pick();
+        if (left <= 0) return false;
+        if (pair == cur.pairs) {
+            pair = 0;
+            ++kvh;
         }
-        const int64_t in = pos - base;
-        const int32_t unit = (int32_t)(in / cur.n);
+        if (kvh == p.Hkv) {
+            kvh = 0;
+            do {
+                ++b;
+                if (++cur_lane == 32) {
+                    cur_lane = 0;
+                    mine = load_seq(p, b + lane, false);
+                }
+                pick();
+            } while (cur.items == 0);  // some is left, so another sequence has items
+        }
         it.b = b;
-        it.kvh = unit / cur.pairs;
-        it.tok0 = cur.tok0 + (unit - it.kvh * cur.pairs) * 2 * p.tile_tokens;
+        it.kvh = kvh;
+        it.tok0 = cur.tok0 + pair * 2 * p.tile_tokens;
         it.tok_end = cur.tok1;
         it.L = cur.L;
-        it.t0 = (int32_t)(in - (int64_t)unit * cur.n);
-        it.t1 = hi - pos < cur.n - it.t0 ? it.t0 + (int32_t)(hi - pos) : cur.n;
-        it.cut = it.t0 > 0 || it.t1 < cur.n;
-        pos += it.t1 - it.t0;
-        if (it.L == 0) it.t1 = it.t0;  // a sequence without keys: one item length, no tiles
+        it.t0 = max(0, off - kItemCost);
+        const bool ends = left >= cur.len() - off;
+        it.t1 = ends ? cur.n : off + (int32_t)left - kItemCost;
+        it.cut = off > 0 || !ends;
+        left -= ends ? cur.len() - off : (int32_t)left;
+        off = 0;
+        ++pair;
+        if (it.L == 0) it.t1 = it.t0;  // a sequence without keys: nothing to read
         return true;
     }
 };
+
+/* What the second launch needs to know of the item that slice c cuts first (is not set where
+ * the slice begins with a whole item, or where an earlier cut is the item's first). */
+struct Cut {
+    int32_t is, last, b, kvh, tok0, tok_end, pad[2];  // its parts are of CTAs c - 1 .. last
+};
+__device__ Cut cut_of(const Params& p, int32_t c, const Slice& s) {
+    Cut k = {};
+    if (s.lo >= s.hi || s.item_lo == s.lo) return k;
+    const int64_t tol = snap_range(s.n, s.total);
+    const int64_t before = slice_begin(c - 1, s.n, s.total) - s.item_lo;
+    if (before > 0 && snapped(before, s.item_len, tol) != 0) return k;
+    // the slice that holds the item's last tile, unless its start was moved behind that
+    int32_t last = (int32_t)slice_owner(s.item_lo + s.item_len - 1, s.n, s.total);
+    const int64_t off = slice_begin(last, s.n, s.total) - s.item_lo;
+    if (off > 0 && snapped(off, s.item_len, tol) == s.item_len) --last;
+    const Seq q = load_seq(p, s.b, false);
+    const int32_t unit = (int32_t)((s.item_lo - s.base) / s.item_len);
+    k.is = 1;
+    k.last = last;
+    k.b = s.b;
+    k.kvh = unit / q.pairs;
+    k.tok0 = q.tok0 + (unit - k.kvh * q.pairs) * 2 * p.tile_tokens;
+    k.tok_end = q.tok1;
+    return k;
+}
+
+/* 32 bytes to global memory in one instruction. */
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 
 __global__ void __launch_bounds__(kThreads, 1)
 cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -338,7 +388,8 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     };
 
     __shared__ Slice slice;
-    find_slice<kThreads>(p, blockIdx.x, slice);
+    find_slice(p, blockIdx.x, slice);
+    if (tid == 0) p.cuts[blockIdx.x] = cut_of(p, blockIdx.x, slice);
     Walker wk;
     wk.init(p, slice, lane);
     Item it;
@@ -648,22 +699,25 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 }
                 if (!valid) continue;
                 if (!it.cut) {
-                    uint4* dst = reinterpret_cast<uint4*>(p.out + at * 128 + 32 * c);
+                    __nv_bfloat16* dst = p.out + at * 128 + 32 * c;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t h[4];
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t h[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            h[e] = l == 0.f ? 0u : ptx::pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv,
-                                                                    __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                        dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
+                        for (int e = 0; e < 8; ++e)
+                            h[e] = l == 0.f ? 0u : ptx::pack_bf16x2(__uint_as_float(o[16 * i + 2 * e]) * inv,
+                                                                    __uint_as_float(o[16 * i + 2 * e + 1]) * inv);
+                        st_global_32(dst + 16 * i, h);
                     }
                 } else if (l != 0.f) {
-                    float4* dst = reinterpret_cast<float4*>(p.rec_o + rec * 128 + 32 * c);
+                    float* dst = p.rec_o + rec * 128 + 32 * c;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                             __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) h[e] = __float_as_uint(__uint_as_float(o[8 * i + e]) * inv);
+                        st_global_32(dst + 8 * i, h);
+                    }
                 }
             }
             ptx::tc_fence_before();
@@ -685,31 +739,22 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 }
 
 /* Joins the parts of cut items: out = sum_s 2^(l_s - l) O_s with 2^l = sum_s 2^(l_s); a
- * part without weight has l_s = -inf and no O.  Block (j, y) looks at the cut before slice
- * j + 1: where it is the first inside its item, the block joins 32 of the item's rows, each
- * thread 16 dimensions of one. */
+ * part without weight has l_s = -inf and no O.  Block (j, y): 32 rows of the item that slice
+ * j + 1 cuts first, each thread 16 dimensions of one. */
 constexpr int kJoinThreads = 256;
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
-    __shared__ Slice a, nx;
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int32_t j = blockIdx.x;
-    find_slice<kJoinThreads>(p, j + 1, nx);
-    // (uniform) no such slice, or it begins with a whole item
-    if (nx.lo >= nx.hi || nx.item_lo == nx.lo) return;
-    find_slice<kJoinThreads>(p, j, a);
-    if (nx.item_lo < a.lo) return;  // an earlier cut is the item's first
-    // the item's parts: of slices j, j + 1, ... up to the one that holds its last tile
-    int32_t last = (int32_t)slice_owner(nx.item_lo + nx.item_len - 1, nx.n, nx.total);
-    const int64_t off = slice_begin(last, nx.n, nx.total) - nx.item_lo;
-    if (off > 0 && snapped(off, nx.item_len, snap_range(nx.n, nx.total)) == nx.item_len) --last;
-    const Seq q = load_seq(p, nx.b, false);
-    const int32_t unit = (int32_t)((nx.item_lo - nx.base) / q.n);
-    const int32_t kvh = unit / q.pairs, tok0 = q.tok0 + (unit - kvh * q.pairs) * 2 * p.tile_tokens;
+    const int4* k4 = reinterpret_cast<const int4*>(p.cuts + j + 1);
+    const int4 k0 = __ldcg(k4);
+    const int4 k1 = __ldcg(k4 + 1);
+    if (k0.x == 0) return;
+    const int32_t last = k0.y, b = k0.z, kvh = k0.w, tok0 = k1.x, tok_end = k1.y;
     const int32_t r = blockIdx.y * 32 + (threadIdx.x >> 3), d = (threadIdx.x & 7) * 16;
     const int32_t w = r >> 7, row = r & (kTile - 1), t = row / p.g;
     const int32_t tok = tok0 + w * p.tile_tokens + t, head = kvh * p.g + (row - t * p.g);
-    if (t >= p.tile_tokens || tok >= q.tok1) return;
+    if (t >= p.tile_tokens || tok >= tok_end) return;
     auto rec_of = [&](int32_t c) { return (int64_t)(2 * c + (c == j ? 1 : 0)) * kRows + r; };
     float m = -INFINITY;
     for (int32_t c = j; c <= last; ++c) m = fmaxf(m, __ldcg(p.rec_lse + rec_of(c)));
@@ -742,7 +787,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
                             ptx::pack_bf16x2(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
     if (d == 0 && p.lse != nullptr) {
         const float l2 = sum == 0.f ? -INFINITY : m + log2f(sum);
-        p.lse[p.cu ? (int64_t)head * p.T + tok : ((int64_t)nx.b * p.Hq + head) * p.S + (tok - nx.b * p.S)] =
+        p.lse[p.cu ? (int64_t)head * p.T + tok : ((int64_t)b * p.Hq + head) * p.S + (tok - b * p.S)] =
             l2 * 0.6931471805599453f;
     }
 }
@@ -772,8 +817,9 @@ int encode(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, in
 int grid_for(int64_t T, int64_t B, int64_t Hkv, int64_t g, int64_t cap_tokens, int sms) {
     const int64_t items = (T / (2 * (kTile / g)) + B) * Hkv;  // at least as many as there are
     const int64_t tiles = (cap_tokens + kTile - 1) / kTile;
-    return items >= sms || tiles >= sms ? sms : (int)(items * tiles / kMinTiles < 1 ? 1 :
-           (items * tiles / kMinTiles < sms ? items * tiles / kMinTiles : sms));
+    if (items >= sms || tiles >= sms) return sms;
+    const int64_t n = items * (tiles + kItemCost) / kMinSlice;
+    return (int)(n < 1 ? 1 : (n < sms ? n : sms));
 }
 
 int shape_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t P, int64_t bt_stride) {
@@ -784,7 +830,7 @@ int shape_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t P
     return PGQA_OK;
 }
 
-size_t workspace_bytes(int grid) { return (size_t)2 * grid * kRows * (128 + 1) * 4; }
+size_t workspace_bytes(int grid) { return (size_t)grid * (2 * kRows * (128 + 1) * 4 + sizeof(Cut)); }
 
 int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (a == nullptr) return PGQA_ERR_NULL_POINTER;
@@ -818,6 +864,7 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (a->workspace == nullptr || a->workspace_bytes < workspace_bytes(p.grid)) return PGQA_ERR_WORKSPACE;
     p.rec_o = static_cast<float*>(a->workspace);
     p.rec_lse = p.rec_o + (size_t)2 * p.grid * kRows * 128;
+    p.cuts = reinterpret_cast<Cut*>(p.rec_lse + (size_t)2 * p.grid * kRows);
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.lse = a->softmax_lse;
     p.seq_lens = a->seq_lens;

@@ -249,13 +249,19 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     positions [cache_seqlens[b], cache_seqlens[b] + S_new) first, and the end-aligned
     causal mask.  q is [B, Sq, Hq, D]; returns out of q's shape, or (out, softmax_lse
     [B, Hq, Sq] fp32) with `return_softmax_lse`, as flash-attn does.  `num_splits` is accepted
-    and ignored (the split follows the real lengths on the device); `rotary_interleaved`
-    only matters with rotary inputs.  Every other option raises NotImplementedError
-    instead of being ignored.
+    and ignored (the split follows the real lengths on the device).
+
+    With `rotary_cos` / `rotary_sin` [rows, rotary_dim / 2] (rotary_dim a multiple of 16) and
+    new tokens, k turns by the table rows of its places, cache_seqlens[b] + s, on its way into
+    the cache, and q by rows cache_seqlens[b] + i if `causal`, else all of it by row
+    cache_seqlens[b]; `rotary_interleaved` pairs elements (2i, 2i + 1), else (i, i +
+    rotary_dim / 2).  Places behind the tables' last row are a device error.  Every other
+    option raises NotImplementedError instead of being ignored.
     """
     unsupported = []
-    if rotary_cos is not None or rotary_sin is not None:
-        unsupported.append("rotary embedding (rotary_cos / rotary_sin)")
+    rotary = rotary_cos is not None or rotary_sin is not None
+    if rotary and (rotary_cos is None or rotary_sin is None or k is None or v is None):
+        unsupported.append("rotary_cos / rotary_sin without each other or without k and v")
     if cache_batch_idx is not None:
         unsupported.append("cache_batch_idx")
     if cache_leftpad is not None:
@@ -282,6 +288,20 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         cache_seqlens = torch.full((B,), cache_seqlens, dtype=torch.int32, device=q.device)
     elif cache_seqlens.dtype != torch.int32:
         cache_seqlens = cache_seqlens.to(torch.int32)
+    if rotary:
+        from .serving import _turn
+        what, S = "flash_attn_with_kvcache", k.shape[1]
+        # q has places of its own where it is not one token per new token, or where it has one
+        # place for all of its tokens
+        together = q.shape[1] == S and (causal or S == 1)
+        turned = _turn(what, q if together else None, k, v, k_cache, v_cache, block_table, cache_seqlens,
+                       rotary_cos, rotary_sin, None, None, rotary_interleaved, None, None, None, None, None)
+        if not together:
+            places = None if causal else cache_seqlens[:, None].expand(B, q.shape[1]).contiguous()
+            turned = _turn(what, q, None, None, None, None, None, cache_seqlens, rotary_cos, rotary_sin,
+                           places, None, rotary_interleaved, None, None, None, None, None)
+        return decode(turned, k_cache, v_cache, block_table, cache_seqlens + S, scale=softmax_scale,
+                      causal=bool(causal), return_lse=bool(return_softmax_lse))
     return decode(q, k_cache, v_cache, block_table, cache_seqlens, scale=softmax_scale,
                   causal=bool(causal), k_new=k, v_new=v, return_lse=bool(return_softmax_lse))
 

@@ -13,6 +13,7 @@ on torch's current stream of the tensors' device, allocates nothing but its outp
 be captured into a CUDA graph after one eager call.  Errors that only the device sees (a
 page id, length or position out of range) are read with `check_device_error()`.
 """
+import functools
 import math
 import struct
 
@@ -28,6 +29,11 @@ _ROPE = struct.Struct("N15P21q4i64s")
 _WEIGHTS = struct.Struct("N7P9qfi")
 _EVICT = struct.Struct("N8P9q2i")
 _CROSS = struct.Struct("N8P10qfiPN")
+
+
+# The handle of torch's current stream (a Stream object takes twenty times as long to make).
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _ptr(what, name, t, dtype, dev):
@@ -83,10 +89,10 @@ def _scales(x, Hkv, dev):
 def _call(fn, args, dev, what):
     """Launches on torch's current stream of the device, with that device current."""
     if dev == torch.cuda.current_device():
-        st = fn(args, torch.cuda.current_stream(dev).cuda_stream)
+        st = fn(args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            st = fn(args, torch.cuda.current_stream(dev).cuda_stream)
+            st = fn(args, _stream(dev))
     check(st, what)
 
 
@@ -297,6 +303,12 @@ def evict_kv(k_cache, v_cache, weights, block_table, seq_lens, keep, *, sinks=0,
     return kept, new_lens
 
 
+@functools.lru_cache(maxsize=4096)
+def _cross_workspace(dev, *shape):
+    with torch.cuda.device(dev):
+        return lib().pgqa_cross_workspace_size(*shape)
+
+
 def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=None, scale=None,
                     out=None, return_lse=False):
     """Attention of query tokens over each sequence's encoder states, held in pages:
@@ -354,15 +366,10 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     if return_lse:
         lse = seq_lens.new_empty((Hq, tokens) if cup else (B, Hq, Sq), dtype=_F32)
     if tokens:
-        L = lib()
-        if dev == torch.cuda.current_device():
-            need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, width)
-        else:
-            with torch.cuda.device(dev):
-                need = L.pgqa_cross_workspace_size(tokens, B, Hq, Hkv, D, P, width)
+        need = _cross_workspace(dev, tokens, B, Hq, Hkv, D, P, width)
         # a buffer of this call's own: calls on two streams or in two graphs share none
         ws = seq_lens.new_empty((need,), dtype=torch.uint8) if need else None
-        _call(L.pgqa_cross_attention, _CROSS.pack(
+        _call(lib().pgqa_cross_attention, _CROSS.pack(
             _CROSS.size, q.data_ptr(), kp, vp, op, 0 if lse is None else lse.data_ptr(), lp, tp, cup, B,
             Sq, tokens, stride, Hq, Hkv, D, P, num_pages, width,
             1.0 / math.sqrt(D) if scale is None else scale, 0, 0 if ws is None else ws.data_ptr(), need),
