@@ -313,7 +313,8 @@ int pgqa_rope_append(const pgqa_rope_args* args, void* stream);
  * [num_pages, Hkv, P].  A row whose log-sum-exp is -inf adds nothing; entries from a
  * sequence's length on are not touched.  Each entry gets one addition per call, in one
  * order, unless sequences share a page: then their sums are added in any order.
- * seqlen_q is at most 4096 and batch_size at most about 28,000 (PGQA_ERR_UNSUPPORTED).
+ * seqlen_q is at most 4096 and batch_size at most about 11,000 (28,000 with up to 8 query
+ * rows per KV head; PGQA_ERR_UNSUPPORTED).
  */
 typedef struct pgqa_weights_args {
     size_t struct_size;

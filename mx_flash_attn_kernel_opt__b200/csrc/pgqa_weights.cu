@@ -20,11 +20,10 @@
  * red.add: no other warp of the call adds to it (unless sequences share a page), so the
  * result does not depend on any order.
  *
- * e4m3 keys become 16-bit numbers in registers, exactly (4 significant bits).  With q held
- * over a unit they become f16, one conversion per pair, and q is turned into f16 once: each
- * row times the power of two that brings its largest element to [2^14, 2^15), undone in
- * fp32 (8 significant bits fit f16's 11; an element 2^28 times smaller than its row's largest
- * is rounded to 2^-25).  With q re-read for every chunk the keys become bf16 instead.
+ * e4m3 keys become f16 in registers, exactly (4 significant bits), and q is turned into f16
+ * once per unit: each row times the power of two that brings its largest element to [2^14,
+ * 2^15), undone in fp32 (8 significant bits fit f16's 11; an element 2^28 times smaller than
+ * its row's largest is rounded to 2^-25).
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -61,8 +60,6 @@ struct Chunk {
     uint4 lo[kPieces], hi[kPieces];
 };
 
-__device__ __forceinline__ uint32_t bf16x2_of(float2 f) { return ptx::pack_bf16x2(f.x, f.y); }
-
 /* q fragments of one group of 8 rows, in the dimension order of the chunk's pieces. */
 struct QFrag {
     uint4 v[4];
@@ -85,7 +82,7 @@ __device__ __forceinline__ void row_of(const Params& p, int32_t b, int32_t kvh, 
 /* Per lane: the q pieces of row 8 j + g, and for rows 8 j + 2 t, 8 j + 2 t + 1 (its two
  * columns of the score tile) the score's factor in log2 units, the negated log2-sum-exp and
  * the number of tokens seen. */
-template <bool KV8, bool F16>
+template <bool KV8>
 __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t kvh, int32_t L, float mul, int j,
                                            int lane, QFrag& f, float (&ml)[2], float (&nl)[2], int32_t (&lim)[2]) {
     const int g = lane >> 2, t = lane & 3;
@@ -104,7 +101,7 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
         for (int i = 0; i < 4; ++i) f.v[i] = make_uint4(0, 0, 0, 0);
     }
     float down = 1.f;
-    if (F16) {
+    if (KV8) {
         uint32_t mx = 0;  // largest magnitude of the row, as its bits
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -126,7 +123,7 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
     for (int e = 0; e < 2; ++e) {
         const int c = 8 * j + 2 * t + e;
         ml[e] = mul;
-        if (F16) ml[e] *= __shfl_sync(0xffffffffu, down, 4 * (2 * t + e));
+        if (KV8) ml[e] *= __shfl_sync(0xffffffffu, down, 4 * (2 * t + e));
         nl[e] = 0.f;
         lim[e] = 0;
         if (c < p.rows) {
@@ -163,7 +160,7 @@ struct AFrag {
 
 /* e4m3 is converted once per chunk, not per group of rows: the conversions are what the SM
  * does fewest of per clock here. */
-template <bool KV8, bool F16>
+template <bool KV8>
 __device__ __forceinline__ void fragments(const Chunk<KV8>& c, AFrag& f) {
 #pragma unroll
     for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
@@ -182,22 +179,15 @@ __device__ __forceinline__ void fragments(const Chunk<KV8>& c, AFrag& f) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 uint32_t(&a)[4] = f.a[(4 * i + s) & 7];
-                if (F16) {
-                    ptx::e4m3x4_to_f16(lo[s], a[0], a[2]);
-                    ptx::e4m3x4_to_f16(hi[s], a[1], a[3]);
-                } else {
-                    a[0] = bf16x2_of(ptx::e4m3x2_to_f32x2(lo[s] & 0xffffu));
-                    a[2] = bf16x2_of(ptx::e4m3x2_to_f32x2(lo[s] >> 16));
-                    a[1] = bf16x2_of(ptx::e4m3x2_to_f32x2(hi[s] & 0xffffu));
-                    a[3] = bf16x2_of(ptx::e4m3x2_to_f32x2(hi[s] >> 16));
-                }
+                ptx::e4m3x4_to_f16(lo[s], a[0], a[2]);
+                ptx::e4m3x4_to_f16(hi[s], a[1], a[3]);
             }
         }
     }
 }
 
 /* Scores of the chunk's 16 tokens against 8 rows: two chains of four products each. */
-template <bool F16>
+template <bool KV8>
 __device__ __forceinline__ void scores(const AFrag& f, const QFrag& q, float (&s)[4]) {
     float u[4] = {0.f, 0.f, 0.f, 0.f};
     s[0] = s[1] = s[2] = s[3] = 0.f;
@@ -206,24 +196,31 @@ __device__ __forceinline__ void scores(const AFrag& f, const QFrag& q, float (&s
         const uint4 v = q.v[i >> 1];
         const uint32_t b0 = (i & 1) ? v.z : v.x, b1 = (i & 1) ? v.w : v.y;
         float(&d)[4] = (i & 1) ? u : s;
-        if (F16) ptx::mma_f16_16816(d, f.a[i][0], f.a[i][1], f.a[i][2], f.a[i][3], b0, b1);
+        if (KV8) ptx::mma_f16_16816(d, f.a[i][0], f.a[i][1], f.a[i][2], f.a[i][3], b0, b1);
         else ptx::mma_bf16_16816(d, f.a[i][0], f.a[i][1], f.a[i][2], f.a[i][3], b0, b1);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += u[e];
 }
 
-/* CTAs of 8 warps on an SM: one where the q fragments of more than 8 rows (32 registers per
- * 16 rows) would not leave room for the chunks in flight otherwise. */
-__host__ __device__ constexpr int ctas_per_sm(int NT) { return NT >= 2 ? 1 : 2; }
 /* Chunks held by a warp: the one at work and those in flight. */
-__host__ __device__ constexpr int depth(bool KV8, int NT) { return NT >= 2 ? (KV8 ? 4 : 3) : (NT == 1 && KV8 ? 3 : 2); }
+__host__ __device__ constexpr int depth(bool KV8, int NT) { return KV8 && NT == 1 ? 3 : 2; }
+/* Shared memory of a warp for the q fragments of NT >= 2 groups, which would leave the
+ * registers no room for the chunks in flight, and for their columns' factors and bounds. */
+struct Cols {
+    float ml[2], nl[2];
+    int32_t lim[2];
+    int32_t pad[2];
+};
+__host__ __device__ constexpr int warp_smem(int NT) { return NT >= 2 ? NT * (4 * 32 * 16 + 4 * (int)sizeof(Cols)) : 0; }
 
-/* NT > 0: that many groups of 8 rows, their q fragments held in registers over a unit;
- * NT = 0: any number, the fragments re-read (from L1) for every chunk. */
+/* NT groups of 8 rows at a time, their q fragments held over a unit: in registers for one, in
+ * the warp's shared memory for two or four.  More than 32 rows take several turns over the
+ * warp's chunks; a token's additions then come from the same lane, in the turns' order. */
 template <bool KV8, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(const Params p) {
-    extern __shared__ uint32_t pre[];  // chunks of the sequences before b, [B + 1]
+__global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
+    extern __shared__ uint4 smem[];  // the warps' q fragments, then pre
+    uint32_t* pre = reinterpret_cast<uint32_t*>(smem) + kWarps * warp_smem(NT) / 4;  // chunks of the sequences before b, [B + 1]
     __shared__ uint32_t wsum[kWarps];
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
@@ -272,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(cons
     const int64_t in = cur - (int64_t)pre[b] * p.Hkv;
     int32_t kvh = (int32_t)(in / n), c = (int32_t)(in - (int64_t)kvh * n);
     const int t = lane & 3, g = lane >> 2;
-    constexpr int kHeld = NT > 0 ? NT : 1;
-    constexpr bool F16 = KV8 && NT > 0;
+    uint4* const my_q = smem + warp * (warp_smem(NT) / 16) + lane;
+    Cols* const my_cols = reinterpret_cast<Cols*>(smem + warp * (warp_smem(NT) / 16) + NT * 128) + t;
     constexpr int D = depth(KV8, NT);
     const int groups = (p.rows + 7) / 8;
 
@@ -284,13 +281,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(cons
         const int32_t L = (int32_t)(L64 > p.cap_tokens ? p.cap_tokens : L64);
         const float ks = (KV8 && p.k_scale) ? __ldg(p.k_scale + kvh) : 1.f;
         const float mul = p.scale_log2 * ks;
-        QFrag qf[kHeld];
-        float ml[kHeld][2], nl[kHeld][2];
-        int32_t lim[kHeld][2];
-        if (NT > 0) {
-#pragma unroll
-            for (int j = 0; j < kHeld; ++j) load_group<KV8, F16>(p, b, kvh, L, mul, j, lane, qf[j], ml[j], nl[j], lim[j]);
-        }
         const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
         auto page_of = [&](int32_t chunk, int32_t& pid, int32_t& slot) {
             const int32_t tok = chunk * kChunkTokens;
@@ -304,63 +294,85 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(cons
             pid = 0;  // read, not added to
             return false;
         };
-        Chunk<KV8> ring[D];
-        int32_t pid[D], slot[D];
-        bool ok[D];
-#pragma unroll
-        for (int u = 0; u < D; ++u) {
-            if (c + u < ce) {
-                page_of(c + u, pid[u], slot[u]);
-                ok[u] = check(pid[u]);
-                load_chunk<KV8>(p, pid[u], slot[u], kvh, lane, ring[u]);
-            }
-        }
-        int32_t npid = 0, nslot = 0;  // of the chunk to be loaded next
-        if (c + D < ce) page_of(c + D, npid, nslot);
-        auto work = [&](const Chunk<KV8>& k, int32_t pid, int32_t slot, bool ok, int32_t c) {
-            const int32_t tok = c * kChunkTokens + g;
-            AFrag fr;
-            fragments<KV8, F16>(k, fr);
-            float w0 = 0.f, w1 = 0.f;  // weights of tokens g and g + 8 over this lane's rows
-            auto add = [&](const QFrag& f, const float (&m)[2], const float (&nlj)[2], const int32_t (&limj)[2]) {
-                float s[4];
-                scores<F16>(fr, f, s);
-                // selected, never multiplied: a masked score may be infinite or NaN
-                w0 += tok < limj[0] ? ptx::ex2(fmaf(s[0], m[0], nlj[0])) : 0.f;
-                w0 += tok < limj[1] ? ptx::ex2(fmaf(s[1], m[1], nlj[1])) : 0.f;
-                w1 += tok + 8 < limj[0] ? ptx::ex2(fmaf(s[2], m[0], nlj[0])) : 0.f;
-                w1 += tok + 8 < limj[1] ? ptx::ex2(fmaf(s[3], m[1], nlj[1])) : 0.f;
-            };
-            if (NT > 0) {
-#pragma unroll
-                for (int j = 0; j < kHeld; ++j) add(qf[j], ml[j], nl[j], lim[j]);
+        const int32_t c_first = c;
+#pragma unroll 1
+        for (int j0 = 0; j0 < groups; j0 += NT) {
+            c = c_first;
+            QFrag qf;
+            Cols cl;
+            if (NT == 1) {
+                load_group<KV8>(p, b, kvh, L, mul, 0, lane, qf, cl.ml, cl.nl, cl.lim);
             } else {
-                for (int j = 0; j < groups; ++j) {
-                    load_group<KV8, F16>(p, b, kvh, L, mul, j, lane, qf[0], ml[0], nl[0], lim[0]);
-                    add(qf[0], ml[0], nl[0], lim[0]);
+                __syncwarp();  // the last rows' are no longer read
+#pragma unroll 1
+                for (int j = 0; j < NT; ++j) {
+                    load_group<KV8>(p, b, kvh, L, mul, j0 + j, lane, qf, cl.ml, cl.nl, cl.lim);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) my_q[(4 * j + i) * 32] = qf.v[i];
+                    if (g == 0) my_cols[4 * j] = cl;
                 }
+                __syncwarp();
             }
-            w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
-            w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
-            w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
-            w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
-            if (ok && t < 2) {
-                const int i = g + 8 * t;
-                if (c * kChunkTokens + i < L)
-                    atomicAdd(p.weights + ((int64_t)pid * p.Hkv + kvh) * p.P + slot + i, t == 0 ? w0 : w1);
-            }
-        };
-        for (; c < ce; c += D) {
+            Chunk<KV8> ring[D];
+            int32_t pid[D], slot[D];
+            bool ok[D];
 #pragma unroll
             for (int u = 0; u < D; ++u) {
-                if (c + u >= ce) break;
-                work(ring[u], pid[u], slot[u], ok[u], c + u);
-                if (c + u + D < ce) {
-                    pid[u] = npid;
-                    slot[u] = nslot;
+                if (c + u < ce) {
+                    page_of(c + u, pid[u], slot[u]);
                     ok[u] = check(pid[u]);
                     load_chunk<KV8>(p, pid[u], slot[u], kvh, lane, ring[u]);
-                    if (c + u + D + 1 < ce) page_of(c + u + D + 1, npid, nslot);
+                }
+            }
+            int32_t npid = 0, nslot = 0;  // of the chunk to be loaded next
+            if (c + D < ce) page_of(c + D, npid, nslot);
+            auto work = [&](const Chunk<KV8>& k, int32_t pid, int32_t slot, bool ok, int32_t c) {
+                const int32_t tok = c * kChunkTokens + g;
+                AFrag fr;
+                fragments<KV8>(k, fr);
+                float w0 = 0.f, w1 = 0.f;  // weights of tokens g and g + 8 over this lane's rows
+                auto add = [&](const QFrag& f, const Cols& c) {
+                    float s[4];
+                    scores<KV8>(fr, f, s);
+                    // selected, never multiplied: a masked score may be infinite or NaN
+                    w0 += tok < c.lim[0] ? ptx::ex2(fmaf(s[0], c.ml[0], c.nl[0])) : 0.f;
+                    w0 += tok < c.lim[1] ? ptx::ex2(fmaf(s[1], c.ml[1], c.nl[1])) : 0.f;
+                    w1 += tok + 8 < c.lim[0] ? ptx::ex2(fmaf(s[2], c.ml[0], c.nl[0])) : 0.f;
+                    w1 += tok + 8 < c.lim[1] ? ptx::ex2(fmaf(s[3], c.ml[1], c.nl[1])) : 0.f;
+                };
+                if (NT == 1) {
+                    add(qf, cl);
+                } else {
+#pragma unroll 2
+                    for (int j = 0; j < NT; ++j) {
+                        QFrag f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.v[i] = my_q[(4 * j + i) * 32];
+                        add(f, my_cols[4 * j]);
+                    }
+                }
+                w0 += __shfl_xor_sync(0xffffffffu, w0, 1);
+                w1 += __shfl_xor_sync(0xffffffffu, w1, 1);
+                w0 += __shfl_xor_sync(0xffffffffu, w0, 2);
+                w1 += __shfl_xor_sync(0xffffffffu, w1, 2);
+                if (ok && t < 2) {
+                    const int i = g + 8 * t;
+                    if (c * kChunkTokens + i < L)
+                        atomicAdd(p.weights + ((int64_t)pid * p.Hkv + kvh) * p.P + slot + i, t == 0 ? w0 : w1);
+                }
+            };
+            for (; c < ce; c += D) {
+#pragma unroll
+                for (int u = 0; u < D; ++u) {
+                    if (c + u >= ce) break;
+                    work(ring[u], pid[u], slot[u], ok[u], c + u);
+                    if (c + u + D < ce) {
+                        pid[u] = npid;
+                        slot[u] = nslot;
+                        ok[u] = check(pid[u]);
+                        load_chunk<KV8>(p, pid[u], slot[u], kvh, lane, ring[u]);
+                        if (c + u + D + 1 < ce) page_of(c + u + D + 1, npid, nslot);
+                    }
                 }
             }
         }
@@ -375,20 +387,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) weights_kernel(cons
 }
 
 template <bool KV8, int NT>
-int launch(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
+int launch(const Params& p, int dev, int sms, int optin, cudaStream_t stream) {
+    const int smem = kWarps * warp_smem(NT) + (p.B + 1) * 4;
+    // the chunk counts before each sequence live in shared memory; two CTAs per SM
+    if (smem > optin / 2 - 1024) return PGQA_ERR_UNSUPPORTED;
     static int done[kHostMaxDevices] = {0};
     auto kern = weights_kernel<KV8, NT>;
     int st = PGQA_OK;
     if (smem > 48 * 1024 && (st = host_smem_limit(kern, dev, smem, done)) != PGQA_OK) return st;
-    return host_launch(kern, dim3((unsigned)(ctas_per_sm(NT) * sms)), kThreads, (size_t)smem, stream, 1, p);
+    return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, 1, p);
 }
 
 template <bool KV8>
-int launch_nt(const Params& p, int dev, int sms, int smem, cudaStream_t stream) {
-    if (p.rows <= 8) return launch<KV8, 1>(p, dev, sms, smem, stream);
-    if (p.rows <= 16) return launch<KV8, 2>(p, dev, sms, smem, stream);
-    if (p.rows <= 32) return launch<KV8, 4>(p, dev, sms, smem, stream);
-    return launch<KV8, 0>(p, dev, sms, smem, stream);
+int launch_nt(const Params& p, int dev, int sms, int optin, cudaStream_t stream) {
+    if (p.rows <= 8) return launch<KV8, 1>(p, dev, sms, optin, stream);
+    if (p.rows <= 16) return launch<KV8, 2>(p, dev, sms, optin, stream);
+    return launch<KV8, 4>(p, dev, sms, optin, stream);
 }
 
 int entry(const pgqa_weights_args* a, cudaStream_t stream) {
@@ -411,8 +425,7 @@ int entry(const pgqa_weights_args* a, cudaStream_t stream) {
         return PGQA_ERR_MISALIGNED;
     int dev, sms, optin;
     if ((st = host_device(&dev, &sms, &optin)) != PGQA_OK) return st;
-    // the table of chunk counts before each sequence lives in shared memory (two CTAs per SM)
-    if ((a->batch_size + 1) * 4 > optin / 2 - 2048) return PGQA_ERR_UNSUPPORTED;
+    if (a->batch_size > optin / 8) return PGQA_ERR_UNSUPPORTED;  // (see launch)
     Params p = {};
     if ((st = host_error_word(dev, &p.err)) != PGQA_OK) return st;
     p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -435,9 +448,8 @@ int entry(const pgqa_weights_args* a, cudaStream_t stream) {
     p.num_pages = (int32_t)a->num_pages;
     p.causal = (int32_t)a->causal;
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    const int smem = (int)(a->batch_size + 1) * 4;
-    return a->kv_format == 1 ? launch_nt<true>(p, dev, sms, smem, stream)
-                             : launch_nt<false>(p, dev, sms, smem, stream);
+    return a->kv_format == 1 ? launch_nt<true>(p, dev, sms, optin, stream)
+                             : launch_nt<false>(p, dev, sms, optin, stream);
 }
 
 }  // namespace weights

@@ -146,3 +146,10 @@ def test_bad_pages_and_lengths_are_reported(cuda_device):
         with pytest.raises(PgqaError) as e:
             pgqa.check_device_error()
         assert e.value.status == status, what
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_more_rows_than_one_turn_takes(kv, cuda_device):
+    """g * Sq of 66 and of 35: several turns over a warp's chunks, the last one partly empty."""
+    run_and_check(make([50, 3, 0], 22, 2, 16, 6, kv, True, seed=20), True, cuda_device)
+    run_and_check(make([90], 5, 1, 32, 7, kv, False, seed=21), False, cuda_device)
