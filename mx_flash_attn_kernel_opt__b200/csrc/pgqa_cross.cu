@@ -83,6 +83,7 @@ struct Params {
     int32_t grid;            // CTAs of the first launch
     float scale_log2;
     uint64_t wait_limit_ns;
+    int32_t debug_stuck;     // test hook: > 0 makes CTA 0's first load expect 16 bytes too many
 };
 
 __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -111,9 +112,9 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int32_t b, bool report)
     q.tok0 = q.tok1 = q.L = q.pairs = q.items = 0;
     q.n = 1;
     if (b >= p.B) return q;
-    q.tok0 = p.cu ? __ldg(p.cu + b) : b * p.S;
-    q.tok1 = p.cu ? __ldg(p.cu + b + 1) : q.tok0 + p.S;
-    int64_t L = __ldg(p.seq_lens + b);
+    q.tok0 = p.cu ? ptx::ld(p.cu + b) : b * p.S;
+    q.tok1 = p.cu ? ptx::ld(p.cu + b + 1) : q.tok0 + p.S;
+    int64_t L = ptx::ld(p.seq_lens + b);
     if (q.tok0 < 0 || q.tok1 < q.tok0 || q.tok1 > p.T || L < 0 || L > p.cap_tokens) {
         if (report) atomicOr(p.err, kDevErrBadSeqlen);
         q.tok0 = max(0, min(q.tok0, p.T));
@@ -406,7 +407,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             auto page_id = [&](int32_t tile) -> int32_t {
                 const int32_t tok = tile * kTile + lane * box;
                 if (lane * box >= kTile || tok >= it.L || tile >= it.t1) return 0;
-                return __ldg(bt + (p.page_shift >= 0 ? tok >> p.page_shift : tok / P));
+                return ptx::ld(bt + (p.page_shift >= 0 ? tok >> p.page_shift : tok / P));
             };
             int32_t pid = page_id(it.t0);
             for (int32_t tile = it.t0; ok && tile < it.t1; ++tile) {
@@ -431,7 +432,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     // a V tile that ends inside a 16-key step is finished here before its release
                     const bool tail = kv == 1 && (nvalid & 15) != 0;
                     const uint32_t bar = tail ? TAIL : FULL(slot);
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * 256));
+                    if (lane == 0) {
+                        const bool stuck = p.debug_stuck > 0 && blockIdx.x == 0 && n_kv == 0;
+                        ptx::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * 256) + (stuck ? 16u : 0u));
+                    }
                     __syncwarp();
                     if (mine) {
                         const CUtensorMap* map = kv ? &vmap : &kmap;
@@ -886,6 +890,8 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     const char* lim = getenv("PGQA_WAIT_LIMIT_NS");
     p.wait_limit_ns = (lim && *lim) ? strtoull(lim, nullptr, 10) : kWaitLimitNs;
     if (p.wait_limit_ns == 0 || p.wait_limit_ns > 10 * kWaitLimitNs) p.wait_limit_ns = kWaitLimitNs;
+    const char* stuck = getenv("PGQA_DEBUG_STUCK_BARRIER");
+    p.debug_stuck = (stuck && *stuck) ? atoi(stuck) : 0;
     CUtensorMap qm, km, vm;
     const int64_t slots = a->num_pages * a->page_size;
     if ((st = encode(&qm, a->q, a->num_heads, a->tokens, a->q_stride * 2, p.g, p.tile_tokens)) != PGQA_OK ||

@@ -70,7 +70,7 @@ __device__ __forceinline__ int32_t page_of(const Params& p, int32_t tok) {
 }
 
 __device__ __forceinline__ int32_t length_of(const Params& p, int32_t b) {
-    const int32_t L = __ldg(p.seq_lens + b);
+    const int32_t L = ptx::ld(p.seq_lens + b);
     return L < 0 ? 0 : (L > p.cap_tokens ? (int32_t)p.cap_tokens : L);
 }
 
@@ -129,7 +129,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int l
 /* Slot of token `tok` in the pool's token order, or -1 for a bad page. */
 __device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, int32_t tok, int32_t& pid) {
     const int32_t page = page_of(p, tok);
-    pid = __ldg(bt + page);
+    pid = ptx::ld(bt + page);
     if ((uint32_t)pid >= (uint32_t)p.num_pages) {
         atomicOr(p.err, kDevErrBadPage);
         return -1;
@@ -158,12 +158,12 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
     bool bad = false;
     auto load_group = [&](int32_t g) -> uint4 {
         const int32_t tok = 4 * g, page = page_of(p, tok);
-        const int32_t pid = __ldg(bt + page);
+        const int32_t pid = ptx::ld(bt + page);
         if ((uint32_t)pid >= (uint32_t)p.num_pages) {
             bad = true;
             return make_uint4(0, 0, 0, 0);
         }
-        const float4 w = __ldg(reinterpret_cast<const float4*>(p.weights + ((int64_t)pid * p.Hkv + h) * p.P +
+        const float4 w = ptx::ld(reinterpret_cast<const float4*>(p.weights + ((int64_t)pid * p.Hkv + h) * p.P +
                                                                (tok - page * p.P)));
         return make_uint4(key_of(w.x), key_of(w.y), key_of(w.z), key_of(w.w));
     };
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
     const int tid = threadIdx.x;
     const int32_t C = p.cluster, item = blockIdx.x / C, rank = blockIdx.x - item * C;
     const int32_t b = item / p.Hkv, h = item - b * p.Hkv;
-    const int32_t L0 = __ldg(p.seq_lens + b);
+    const int32_t L0 = ptx::ld(p.seq_lens + b);
     const int32_t L = length_of(p, b);
     const int32_t n = min(L, p.keep);
     if (h == 0 && tid == 0 && rank == 0) {

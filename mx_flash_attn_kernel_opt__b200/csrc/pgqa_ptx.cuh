@@ -157,6 +157,12 @@ __device__ __forceinline__ void griddep_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+/* Ordinary global load.  A kernel that starts before its predecessor has ended reads what that
+ * one wrote through this, after griddepcontrol.wait, and not through the read-only path
+ * (ld.global.nc), whose data may not change while the kernel runs. */
+template <typename T>
+__device__ __forceinline__ T ld(const T* p) { return *p; }
+
 /* Explicit shared-memory accesses by 32-bit shared-window address. */
 __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
     float4 v;

@@ -56,7 +56,7 @@ __device__ __forceinline__ int32_t find_sequence(const int32_t* cu, int32_t B, i
     while (hi - lo > 1) {
         const int32_t step = (hi - lo + 31) / 32;
         const int32_t at = lo + (lane + 1) * step;
-        const bool le = at < hi && (int64_t)__ldg(cu + at) <= x;
+        const bool le = at < hi && (int64_t)ptx::ld(cu + at) <= x;
         const int32_t n = __popc(__ballot_sync(0xffffffffu, le));
         lo += n * step;
         hi = min(hi, lo + step);
@@ -125,28 +125,28 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
             else if (r < p.Hq + p.Hk) src = p.k + b_pad * p.ks[0] + sx * p.ks[1] + (r - p.Hq) * p.ks[2];
             else src = p.v + b_pad * p.vs[0] + sx * p.vs[1] + (r - p.Hq - p.Hk) * p.vs[2];
             const uint4* s4 = reinterpret_cast<const uint4*>(src);
-            a[i] = __ldg(s4 + c0);
-            e[i] = __ldg(s4 + c1);
+            a[i] = ptx::ld(s4 + c0);
+            e[i] = ptx::ld(s4 + c1);
         }
     }
     // positions of this lane's pairs [8 t, 8 t + 8): one, or one per pair
     int32_t pos[8];
     if (t < turned && p.positions != nullptr) {
-        pos[0] = __ldg(p.positions + (int64_t)p.axis[8 * t] * p.T + x);
+        pos[0] = ptx::ld(p.positions + (int64_t)p.axis[8 * t] * p.T + x);
         if (!p.runs8) {
 #pragma unroll
-            for (int j = 1; j < 8; ++j) pos[j] = __ldg(p.positions + (int64_t)p.axis[8 * t + j] * p.T + x);
+            for (int j = 1; j < 8; ++j) pos[j] = ptx::ld(p.positions + (int64_t)p.axis[8 * t + j] * p.T + x);
         }
     }
     int32_t b = b_pad;
     int64_t s = sx;
     if (p.cu != nullptr) {
         b = find_sequence(p.cu, p.B, x, lane);
-        s = x - __ldg(p.cu + b);
+        s = x - ptx::ld(p.cu + b);
         // in front of the first sequence or behind the last: left as it was
-        if (s < 0 || x >= __ldg(p.cu + b + 1)) return;
+        if (s < 0 || x >= ptx::ld(p.cu + b + 1)) return;
     }
-    const int64_t tok = (p.seq_lens != nullptr ? (int64_t)__ldg(p.seq_lens + b) : 0) + s;
+    const int64_t tok = (p.seq_lens != nullptr ? (int64_t)ptx::ld(p.seq_lens + b) : 0) + s;
     // cosines and sines
     float c[8], n[8];
     bool bad = false;
@@ -161,12 +161,12 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
         if (p.runs8 || p.positions == nullptr) {  // the eight pairs turn about one axis
             const int64_t at = row_of(p.positions ? (int64_t)pos[0] : tok) + 8 * t;
             if (p.table_bf16) {
-                unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + at)), c);
-                unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.sin) + at)), n);
+                unpack8(ptx::ld(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + at)), c);
+                unpack8(ptx::ld(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.sin) + at)), n);
             } else {
                 const float4* cp = reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at);
                 const float4* np = reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at);
-                const float4 u0 = __ldg(cp), u1 = __ldg(cp + 1), w0 = __ldg(np), w1 = __ldg(np + 1);
+                const float4 u0 = ptx::ld(cp), u1 = ptx::ld(cp + 1), w0 = ptx::ld(np), w1 = ptx::ld(np + 1);
                 c[0] = u0.x; c[1] = u0.y; c[2] = u0.z; c[3] = u0.w; c[4] = u1.x; c[5] = u1.y; c[6] = u1.z; c[7] = u1.w;
                 n[0] = w0.x; n[1] = w0.y; n[2] = w0.z; n[3] = w0.w; n[4] = w1.x; n[5] = w1.y; n[6] = w1.z; n[7] = w1.w;
             }
@@ -175,11 +175,11 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
             for (int j = 0; j < 8; ++j) {
                 const int64_t at = row_of(pos[j]) + 8 * t + j;
                 if (p.table_bf16) {
-                    c[j] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.cos) + at));
-                    n[j] = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.sin) + at));
+                    c[j] = __bfloat162float(ptx::ld(static_cast<const __nv_bfloat16*>(p.cos) + at));
+                    n[j] = __bfloat162float(ptx::ld(static_cast<const __nv_bfloat16*>(p.sin) + at));
                 } else {
-                    c[j] = __ldg(static_cast<const float*>(p.cos) + at);
-                    n[j] = __ldg(static_cast<const float*>(p.sin) + at);
+                    c[j] = ptx::ld(static_cast<const float*>(p.cos) + at);
+                    n[j] = ptx::ld(static_cast<const float*>(p.sin) + at);
                 }
             }
         }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
         }
         const int32_t page = p.page_shift >= 0 ? (int32_t)(tok >> p.page_shift) : (int32_t)(tok / p.P);
         slot = (int32_t)(tok - (int64_t)page * p.P);
-        pid = __ldg(p.block_table + (int64_t)b * p.bt_stride + page);
+        pid = ptx::ld(p.block_table + (int64_t)b * p.bt_stride + page);
         if ((uint32_t)pid >= (uint32_t)p.num_pages) {
             if (lane == 0) atomicOr(p.err, kDevErrBadPage);
             return;
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
                 a[i] = pack8_bf16(y0);
                 e[i] = pack8_bf16(y1);
             } else {
-                const float sc = p.k_scale ? __ldg(p.k_scale + (r - p.Hq)) : 1.f;
+                const float sc = p.k_scale ? ptx::ld(p.k_scale + (r - p.Hq)) : 1.f;
                 const uint2 u0 = pack8_e4m3(y0, sc), u1 = pack8_e4m3(y1, sc);
                 a[i].x = u0.x; a[i].y = u0.y;
                 e[i].x = u1.x; e[i].y = u1.y;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p
             unpack8(a[i], f);
             unpack8(e[i], g);
             const float* scale = is_v ? p.v_scale : p.k_scale;
-            const float sc = scale ? __ldg(scale + (r - p.Hq - (is_v ? p.Hk : 0))) : 1.f;
+            const float sc = scale ? ptx::ld(scale + (r - p.Hq - (is_v ? p.Hk : 0))) : 1.f;
             const uint2 u0 = pack8_e4m3(f, sc), u1 = pack8_e4m3(g, sc);
             a[i].x = u0.x; a[i].y = u0.y;
             e[i].x = u1.x; e[i].y = u1.y;

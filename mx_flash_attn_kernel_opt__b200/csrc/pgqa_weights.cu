@@ -95,7 +95,7 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             // e4m3: a 16-byte piece of K covers two consecutive pieces of q
-            f.v[i] = __ldg(src + (KV8 ? 8 * (i >> 1) + 2 * t + (i & 1) : 4 * i + t));
+            f.v[i] = ptx::ld(src + (KV8 ? 8 * (i >> 1) + 2 * t + (i & 1) : 4 * i + t));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.v[i] = make_uint4(0, 0, 0, 0);
@@ -128,7 +128,7 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
         lim[e] = 0;
         if (c < p.rows) {
             row_of(p, b, kvh, c, qo, lo, tok);
-            const float l = __ldg(p.lse + lo);
+            const float l = ptx::ld(p.lse + lo);
             // a row that saw nothing (-inf) has no weight to give
             if (l != -INFINITY) {
                 nl[e] = -l * 1.4426950408889634f;
@@ -148,8 +148,8 @@ __device__ __forceinline__ void load_chunk(const Params& p, int32_t pid, int32_t
     const uint4* d = a + (int64_t)8 * p.Hkv * kRow;
 #pragma unroll
     for (int i = 0; i < Chunk<KV8>::kPieces; ++i) {
-        c.lo[i] = __ldg(a + 4 * i);
-        c.hi[i] = __ldg(d + 4 * i);
+        c.lo[i] = __ldcg(a + 4 * i);  // read once: no line in L1
+        c.hi[i] = __ldcg(d + 4 * i);
     }
 }
 
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
         uint32_t local = 0;
         bool bad = false;
         for (int b = s0; b < s1; ++b) {
-            const int32_t L = __ldg(p.seq_lens + b);
+            const int32_t L = ptx::ld(p.seq_lens + b);
             bad = bad || L < 0 || L > p.cap_tokens;
             local += (uint32_t)seq_chunks(L, p.cap_tokens);
         }
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
         for (int w = 0; w < warp; ++w) run += wsum[w];
         for (int b = s0; b < s1; ++b) {
             pre[b] = run;
-            run += (uint32_t)seq_chunks(__ldg(p.seq_lens + b), p.cap_tokens);
+            run += (uint32_t)seq_chunks(ptx::ld(p.seq_lens + b), p.cap_tokens);
         }
         if (s1 == p.B) pre[p.B] = run;  // every thread past the last sequence writes the same total
         __syncthreads();
@@ -277,16 +277,16 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
     while (cur < end) {
         // the slice's part of the unit (b, kvh): chunks [c, ce)
         const int32_t ce = (int32_t)((end - cur < n - c) ? c + (end - cur) : n);
-        const int64_t L64 = __ldg(p.seq_lens + b);
+        const int64_t L64 = ptx::ld(p.seq_lens + b);
         const int32_t L = (int32_t)(L64 > p.cap_tokens ? p.cap_tokens : L64);
-        const float ks = (KV8 && p.k_scale) ? __ldg(p.k_scale + kvh) : 1.f;
+        const float ks = (KV8 && p.k_scale) ? ptx::ld(p.k_scale + kvh) : 1.f;
         const float mul = p.scale_log2 * ks;
         const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
         auto page_of = [&](int32_t chunk, int32_t& pid, int32_t& slot) {
             const int32_t tok = chunk * kChunkTokens;
             const int32_t page = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.P;
             slot = tok - page * p.P;
-            pid = __ldg(bt + page);
+            pid = ptx::ld(bt + page);
         };
         auto check = [&](int32_t& pid) -> bool {
             if ((uint32_t)pid < (uint32_t)p.num_pages) return true;

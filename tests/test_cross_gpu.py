@@ -243,3 +243,19 @@ def test_bad_pages_and_lengths_are_reported(cuda_device):
             pgqa.check_device_error()
         assert e.value.status == status, what
         pgqa.check_device_error()
+
+
+def test_an_expired_wait_is_reported_and_leaves_the_context_usable(cuda_device, monkeypatch):
+    """A load that waits for 16 bytes that are never sent: every role gives up at its (short)
+    limit, the call ends and the next one is right."""
+    case = make([70, 9], [900, 333], 8, 2, 16, seed=30)
+    args = [x.to(cuda_device) for x in case]
+    monkeypatch.setenv("PGQA_DEBUG_STUCK_BARRIER", "1")
+    monkeypatch.setenv("PGQA_WAIT_LIMIT_NS", "3000000")
+    pgqa.cross_attention(*args[:5], cu_seqlens_q=args[5])
+    with pytest.raises(PgqaError) as e:
+        pgqa.check_device_error()
+    assert e.value.status == 8
+    monkeypatch.delenv("PGQA_DEBUG_STUCK_BARRIER")
+    monkeypatch.delenv("PGQA_WAIT_LIMIT_NS")
+    run_and_check(case, cuda_device)
