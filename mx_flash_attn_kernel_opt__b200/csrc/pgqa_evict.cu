@@ -49,8 +49,9 @@ constexpr int kRows = 2048;            // rows looked up at a time by a CTA
 constexpr int kRingBytes = kStages * kStagePieces * 16;
 constexpr int kSmem = kRingBytes + 2 * kRows * 4;  // so many that kCtasPerSm fit
 constexpr int kCtasPerSm = 1024 / kThreads;
-constexpr int kMaxGroups = kRingBytes / 16;        // groups of four keys held in the ring before the move
-static_assert(2 * kRows >= kBins, "the select's histogram lies in the rows' places");
+constexpr int kHistBytes = kBins * 4;
+constexpr int kMaxGroups = (kRingBytes - kHistBytes) / 16;  // groups of four keys held in the ring before the move
+static_assert(2 * kRows >= 2 * kBins, "two of the select's histograms lie in the rows' places, one in the ring");
 
 struct Params {
     void *k_cache, *v_cache;
@@ -138,9 +139,12 @@ __device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, i
 }
 
 /* Writes kept[0, keep) of a sequence of L > keep tokens: C CTAs of a cluster together, each
- * with the keys of its range in `keys`, or (C = 1) one CTA alone. */
+ * with the keys of its range in `keys`, or (C = 1) one CTA alone, which leaves the first kRows
+ * of them in `places` too.  The three passes have a histogram each (at `places` and at the
+ * end of the ring), so one cluster barrier per pass will do; and nothing is stored to global
+ * memory before the last pass, since a releasing barrier waits for such stores. */
 __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32_t h, int32_t* kept, int C, int rank,
-                            uint4* keys, uint32_t* hist) {
+                            uint4* keys, uint32_t* places) {
     __shared__ uint32_t wsum[32];
     __shared__ uint32_t found[2];   // the digit of the last kept key, and how many lie above it
     __shared__ __align__(16) uint32_t counts[4];  // this CTA's tokens above the last kept key, and equal to it
@@ -148,9 +152,6 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
     const int t_all = rank * kThreads + tid, n_all = C * kThreads;
     const int32_t lo = p.sinks, hi = L - p.recent;       // candidates [lo, hi)
     const int32_t m = p.keep - p.sinks - p.recent;       // of which m < hi - lo stay
-    for (int j = t_all; j < p.sinks; j += n_all) kept[j] = j;
-    for (int j = t_all; j < p.recent; j += n_all) kept[p.sinks + m + j] = L - p.recent + j;
-    if (m == 0) return;
     // this CTA's groups of four tokens (a group never crosses a page): [g0, g1)
     const int32_t ga = lo >> 2, gn = ((hi + 3) >> 2) - ga, per = (gn + C - 1) / C;
     const int32_t g0 = ga + min(gn, rank * per), g1 = ga + min(gn, (rank + 1) * per);
@@ -178,12 +179,15 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
 
     uint32_t prefix = 0, mask = 0;  // digits fixed so far
     uint32_t need = (uint32_t)m;    // tokens still to take among those that match them
+    uint32_t* const third = reinterpret_cast<uint32_t*>(keys + kMaxGroups);
+    for (int i = tid; i < 2 * kBins; i += kThreads) places[i] = 0;
+    for (int i = tid; i < kBins; i += kThreads) third[i] = 0;
+    __syncthreads();
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
+    for (int pass = 0; pass < 3 && m > 0; ++pass) {
+        uint32_t* const hist = pass < 2 ? places + pass * kBins : third;
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
         const uint32_t digits = pass == 2 ? 1023u : 2047u;
-        for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-        __syncthreads();
         auto count = [&](int32_t g, const uint4& k) {
             each(g, k, [&](uint32_t key, int) {
                 if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digits], 1u);
@@ -236,25 +240,46 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
         }
 #pragma unroll
         for (int i = 0; i < kBinsPerThread; ++i) sum += c[i];
-        uint32_t total;
-        uint32_t above = block_scan(sum, wsum, lane, warp, total);
+        // the warp whose bins hold the `need`-th key from the top, then the thread and the bin
+        const uint32_t mine = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) wsum[warp] = mine;
+        __syncthreads();
+        uint32_t above = lane < warp ? wsum[lane] : 0;  // kThreads / 32 warps, at most 32
+        above = __reduce_add_sync(0xffffffffu, above);
+        if (above < need && need <= above + mine) {
+            uint32_t incl = sum;
 #pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) {
-            if (above < need && need <= above + c[i]) {
-                found[0] = (uint32_t)(top - i);
-                found[1] = above | (c[i] == need - above ? 0x80000000u : 0u);
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
             }
-            above += c[i];
+            above += incl - sum;
+#pragma unroll
+            for (int i = 0; i < kBinsPerThread; ++i) {
+                if (above < need && need <= above + c[i]) {
+                    found[0] = (uint32_t)(top - i);
+                    found[1] = above | (c[i] == need - above ? 0x80000000u : 0u);
+                }
+                above += c[i];
+            }
         }
-        if (C > 1) cluster_sync();  // the other CTAs have read this one's histogram
-        else __syncthreads();
+        __syncthreads();
         const uint32_t digit = found[0], over = found[1];
         need -= over & 0x7fffffffu;
         prefix |= digit << shift;
         mask |= digits << shift;
         if (over >> 31) break;  // every token that matches the prefix stays
     }
-    // kept: keys above the prefix (under its mask), and the first `need` that match it
+    // kept: keys above the prefix (under its mask), and the first `need` that match it; none
+    // of the middle (m = 0) is above an all-ones prefix
+    if (m == 0) {
+        prefix = mask = 0xffffffffu;
+        need = 0;
+    }
+    auto put = [&](int32_t at, int32_t tok) {
+        kept[at] = tok;
+        if (C == 1 && at < kRows) places[at] = (uint32_t)tok;
+    };
     uint32_t gt_before = 0, eq_before = 0;  // in the tokens before
     if (C > 1) {
         uint32_t gt = 0, eq = 0;
@@ -302,17 +327,16 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const uint32_t at = (uint32_t)p.sinks + gt + (eq < need ? eq : need);
-            if (flags & (1u << u)) {
-                kept[at] = 4 * g + u;
-                ++gt;
-            } else if (flags & (16u << u)) {
-                if (eq < need) kept[at] = 4 * g + u;
-                ++eq;
-            }
+            const bool above = (flags & (1u << u)) != 0, equal = (flags & (16u << u)) != 0;
+            if (above || (equal && eq < need)) put((int32_t)at, 4 * g + u);
+            gt += above;
+            eq += equal;
         }
         gt_before += total & 0xffffu;
         eq_before += total >> 16;
     }
+    for (int j = t_all; j < p.sinks; j += n_all) put(j, j);
+    for (int j = t_all; j < p.recent; j += n_all) put(p.sinks + m + j, L - p.recent + j);
     if (bad) atomicOr(p.err, kDevErrBadPage);
 }
 
@@ -333,16 +357,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
     int32_t* kept = p.kept + (int64_t)item * p.keep;
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
     const bool cut = L > p.keep;  // the same in all of the cluster, as is every count of a loop with a barrier
+    int32_t* src_slot = reinterpret_cast<int32_t*>(ring + kRingBytes / 16);
+    int32_t* dst_slot = src_slot + kRows;
+    const bool solo = C == 2;
     if (cut) {
         // a pair of CTAs: each selects for itself (and writes the same indices), which costs
         // less than meeting at every step; more of them divide the tokens
-        select_kept(p, bt, L, h, kept, C == 2 ? 1 : C, C == 2 ? 0 : rank, ring,
-                    reinterpret_cast<uint32_t*>(ring + kRingBytes / 16));
-        // kept is complete, every weight has been read, and nobody reads another's shared memory
-        cluster_sync();
+        select_kept(p, bt, L, h, kept, solo ? 1 : C, solo ? 0 : rank, ring, reinterpret_cast<uint32_t*>(src_slot));
+        // kept is complete; every weight has been read, and nobody reads another's shared
+        // memory (a pair shares none, and meets before it overwrites a weight)
+        if (solo) __syncthreads();
+        else cluster_sync();
     } else {
         for (int j = rank * kThreads + tid; j < p.keep; j += C * kThreads) kept[j] = j < L ? j : -1;
     }
+    // the j-th kept token; a CTA that selected alone has the first ones at hand until the first
+    // rows' places are looked up
+    bool at_hand = solo;
+    auto kept_at = [&](int32_t j) { return at_hand && j < kRows ? src_slot[j] : __ldcg(kept + j); };
+
     // the weights, one 4-byte element per token
     const bool in_place = p.weights_out == p.weights;
     if (cut || !in_place) {
@@ -355,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
                 const int32_t j = j0 + (u * C + rank) * kThreads + tid;
                 dst[u] = -1;
                 if (j < n) {
-                    const int32_t src = cut ? __ldcg(kept + j) : j;
+                    const int32_t src = cut ? kept_at(j) : j;
                     int32_t sp, dp;
                     const int32_t ss = slot_of(p, bt, src, sp), ds = slot_of(p, bt, j, dp);
                     if (ss >= 0 && ds >= 0 && !(in_place && src == j)) {
@@ -378,11 +411,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
     const int32_t batch = rows * kPieces;            // and in a batch
     pool += (int64_t)h * p.row_pieces + tid % p.row_pieces;
     const int64_t pitch = (int64_t)p.Hkv * p.row_pieces;
-    int32_t* src_slot = reinterpret_cast<int32_t*>(ring + kRingBytes / 16);
-    int32_t* dst_slot = src_slot + kRows;
     // rows that stay where they are form a prefix; skip whole strides of it
     const int32_t stride = (n + kThreads - 1) / kThreads;
-    const bool still = tid * stride < n && __ldcg(kept + tid * stride) == tid * stride;
+    const bool still = tid * stride < n && kept_at(tid * stride) == tid * stride;
     const int32_t fixed = __syncthreads_count(still);
     for (int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0; j0 < n; j0 += kRows * S) {
         const int32_t here = min(kRows * S, n - j0);
@@ -393,8 +424,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
 #pragma unroll
         for (int u = 0; u < kRows / kThreads; ++u) {
             const int32_t r = row_of(u * kThreads + tid);
-            from[u] = r < here ? __ldcg(kept + j0 + r) : -1;
+            from[u] = r < here ? kept_at(j0 + r) : -1;
         }
+        if (at_hand) __syncthreads();  // they are overwritten now
+        at_hand = false;
 #pragma unroll
         for (int u = 0; u < kRows / kThreads; ++u) {
             const int32_t i = u * kThreads + tid, r = row_of(i);

@@ -63,6 +63,14 @@ def test_pairs_cut_by_clusters_and_pairs_left_alone(cuda_device):
     run_and_check((k, v, w, bt, lens), 37, 30, 7, cuda_device)
 
 
+def test_more_kept_than_places_looked_up_at_a_time(cuda_device):
+    """More than 2048 kept rows, by a pair of CTAs and by more, in place and apart."""
+    for pairs, P in ((90, 16), (1, 64)):
+        case = make([5300] + [0] * (pairs - 1), 4 if pairs > 1 else 1, P, "e4m3", seed=30 + pairs)
+        run_and_check(case, 5000, 7, 100, cuda_device)
+        run_and_check(case, 2600, 0, 2600, cuda_device, apart=True)
+
+
 def test_longer_than_shared_memory_holds(cuda_device):
     """More candidates than the select keeps in shared memory: keys are re-read."""
     g = torch.Generator().manual_seed(1)
