@@ -40,7 +40,6 @@ namespace evict {
 
 constexpr int kThreads = 512;
 constexpr int kBins = 2048;
-constexpr int kBinsPerThread = kBins / kThreads;
 constexpr int kMaxCluster = 8;
 constexpr int kPieces = 2;             // 16-byte pieces of a thread per batch
 constexpr int kStages = 5;             // batches in the ring
@@ -93,17 +92,15 @@ __device__ __forceinline__ void cluster_arrive_relaxed() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint4 ld_cluster(uint32_t addr, uint32_t rank) {
-    uint4 v;
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t v;
     asm volatile(
-        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\t"
-        "ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a];\n\t}"
-        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+        : "=r"(v)
         : "r"(addr), "r"(rank)
         : "memory");
     return v;
 }
-
 /* Sum of v over the threads before this one, and over all, of a block; two
  * 16-bit counts packed in a word pass through as long as neither total reaches 2^16. */
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int lane, int warp, uint32_t& total) {
@@ -127,15 +124,19 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* wsum, int l
     return incl - v + __shfl_sync(0xffffffffu, ws - own, warp);
 }
 
-/* Slot of token `tok` in the pool's token order, or -1 for a bad page. */
-__device__ __forceinline__ int32_t slot_of(const Params& p, const int32_t* bt, int32_t tok, int32_t& pid) {
-    const int32_t page = page_of(p, tok);
-    pid = ptx::ld(bt + page);
+/* Place of token `tok` in the pool's token order, given its page's id, or -1 for a bad one
+ * (`bad` is then set).  The ids are loaded apart, many at a time. */
+__device__ __forceinline__ int32_t place_of(const Params& p, int32_t tok, int32_t pid, bool& bad) {
     if ((uint32_t)pid >= (uint32_t)p.num_pages) {
-        atomicOr(p.err, kDevErrBadPage);
+        bad = true;
         return -1;
     }
-    return tok - page * p.P;
+    return pid * p.P + (tok - page_of(p, tok) * p.P);
+}
+/* Entry of the weight pool at a place. */
+__device__ __forceinline__ int64_t weight_at(const Params& p, int32_t place, int32_t h) {
+    const int32_t pid = page_of(p, place);
+    return ((int64_t)pid * p.Hkv + h) * p.P + (place - pid * p.P);
 }
 
 /* Writes kept[0, keep) of a sequence of L > keep tokens: C CTAs of a cluster together, each
@@ -147,7 +148,8 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
                             uint4* keys, uint32_t* places) {
     __shared__ uint32_t wsum[32];
     __shared__ uint32_t found[2];   // the digit of the last kept key, and how many lie above it
-    __shared__ __align__(16) uint32_t counts[4];  // this CTA's tokens above the last kept key, and equal to it
+    __shared__ uint32_t counts[2];  // the CTAs before: tokens above the digit, and with it
+    __shared__ uint32_t coarse[3][kBins / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int t_all = rank * kThreads + tid, n_all = C * kThreads;
     const int32_t lo = p.sinks, hi = L - p.recent;       // candidates [lo, hi)
@@ -179,6 +181,7 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
 
     uint32_t prefix = 0, mask = 0;  // digits fixed so far
     uint32_t need = (uint32_t)m;    // tokens still to take among those that match them
+    uint32_t gt_before = 0, eq_before = 0;  // kept for sure, and equal to the last, in the CTAs before
     uint32_t* const third = reinterpret_cast<uint32_t*>(keys + kMaxGroups);
     for (int i = tid; i < 2 * kBins; i += kThreads) places[i] = 0;
     for (int i = tid; i < kBins; i += kThreads) third[i] = 0;
@@ -211,59 +214,105 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
         } else {
             for (int32_t g = g0 + tid; g < g1; g += kThreads) count(g, group_at(g));
         }
-        // counts of all CTAs from the top: thread t owns the bins from top down to
-        // top - kBinsPerThread + 1
-        const int top = kBins - 1 - kBinsPerThread * tid;
-        uint32_t c[kBinsPerThread], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) c[i] = 0;
-        if (C > 1) cluster_sync();
-        else __syncthreads();
-#pragma unroll
-        for (int q = 0; q < kBinsPerThread; q += 4) {
-            const uint32_t at = ptx::smem_u32(hist + top - q - 3);
-            auto take = [&](const uint4& v) {
-                c[q] += v.w;
-                c[q + 1] += v.z;
-                c[q + 2] += v.y;
-                c[q + 3] += v.x;
-            };
-            if (C > 1) {
-                uint4 v[kMaxCluster];
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r) v[r] = r < C ? ld_cluster(at, (uint32_t)r) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r) take(v[r]);
-            } else {
-                take(ptx::lds_u4(at));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kBinsPerThread; ++i) sum += c[i];
-        // the warp whose bins hold the `need`-th key from the top, then the thread and the bin
-        const uint32_t mine = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0) wsum[warp] = mine;
         __syncthreads();
-        uint32_t above = lane < warp ? wsum[lane] : 0;  // kThreads / 32 warps, at most 32
-        above = __reduce_add_sync(0xffffffffu, above);
-        if (above < need && need <= above + mine) {
-            uint32_t incl = sum;
+        if (C == 1) {
+            // alone: all bins at once, from the top; thread t owns those from `top` down.  The
+            // warp whose bins hold the `need`-th key of those left, then the thread and the bin
+            // (three levels by one warp, as below: evict-step 16.4 us instead of 13.9)
+            constexpr int kOwn = kBins / kThreads;
+            const int top = kBins - 1 - kOwn * tid;
+            uint32_t c[kOwn], sum = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
+            for (int i = 0; i < kOwn; ++i) {
+                c[i] = hist[top - i];
+                sum += c[i];
             }
-            above += incl - sum;
+            const uint32_t mine = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) wsum[warp] = mine;
+            __syncthreads();
+            uint32_t above = __reduce_add_sync(0xffffffffu, lane < warp ? wsum[lane] : 0);
+            if (above < need && need <= above + mine) {
+                uint32_t incl = sum;
 #pragma unroll
-            for (int i = 0; i < kBinsPerThread; ++i) {
-                if (above < need && need <= above + c[i]) {
-                    found[0] = (uint32_t)(top - i);
-                    found[1] = above | (c[i] == need - above ? 0x80000000u : 0u);
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
                 }
-                above += c[i];
+                above += incl - sum;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) {
+                    if (above < need && need <= above + c[i]) {
+                        found[0] = (uint32_t)(top - i);
+                        found[1] = above | (c[i] == need - above ? 0x80000000u : 0u);
+                    }
+                    above += c[i];
+                }
+            }
+            if (tid < 2) counts[tid] = 0;
+        } else {
+            // together: sums of 32 bins each, so that the others read these and one group of
+            // 32 of this CTA's histogram instead of all of it (evict-long-e4m3: 37 us instead of 44)
+            for (int i = warp; i < kBins / 32; i += kThreads / 32) {
+                const uint32_t v = __reduce_add_sync(0xffffffffu, hist[32 * i + lane]);
+                if (lane == 0) coarse[pass][i] = v;
+            }
+            cluster_sync();
+        }
+        if (C > 1 && warp == 0) {
+            // the group of bins, then the bin, that hold the `need`-th key from the top (of those
+            // left); and how many keys above it, and in it, the CTAs before this one have
+            uint32_t whole = 0;         // keys in the bin found
+            uint32_t over = 0, gt = 0;  // keys above so far, of all CTAs and of those before
+            const uint32_t at_coarse = ptx::smem_u32(&coarse[pass][0]);
+            int group = 0;
+            auto search = [&](uint32_t at, int top, uint32_t& eq) -> int {  // 32 words down from `top`
+                uint32_t sum = 0, low = 0, v[kMaxCluster];
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) v[r] = r < C ? ld_cluster(at + 4u * (top - lane), (uint32_t)r) : 0;
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {
+                    sum += v[r];
+                    if (r < rank) low += v[r];
+                }
+                uint32_t incl = sum, lincl = low;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t a = __shfl_up_sync(0xffffffffu, incl, o), b = __shfl_up_sync(0xffffffffu, lincl, o);
+                    if (lane >= o) {
+                        incl += a;
+                        lincl += b;
+                    }
+                }
+                const uint32_t hit = __ballot_sync(0xffffffffu, over + incl >= need);
+                const int f = hit ? __ffs(hit) - 1 : 32;  // lanes before f lie above
+                const int prev = f > 0 ? f - 1 : 0;
+                const uint32_t a = __shfl_sync(0xffffffffu, incl, prev), b = __shfl_sync(0xffffffffu, lincl, prev);
+                if (f > 0) {
+                    over += a;
+                    gt += b;
+                }
+                eq = f < 32 ? __shfl_sync(0xffffffffu, low, f) : 0;
+                whole = f < 32 ? __shfl_sync(0xffffffffu, sum, f) : 0;
+                return f;
+            };
+            uint32_t eq = 0;
+            int f = search(at_coarse, kBins / 32 - 1, eq);
+            group = kBins / 32 - 1 - f;
+            if (f == 32) {
+                f = search(at_coarse, kBins / 32 - 33, eq);
+                group = kBins / 32 - 33 - f;
+            }
+            f = search(ptx::smem_u32(hist), 32 * group + 31, eq);
+            if (lane == 0) {
+                found[0] = (uint32_t)(32 * group + 31 - f);
+                found[1] = over | (whole == need - over ? 0x80000000u : 0u);
+                counts[0] = gt;
+                counts[1] = eq;
             }
         }
         __syncthreads();
+        gt_before += counts[0];
+        eq_before = counts[1];
         const uint32_t digit = found[0], over = found[1];
         need -= over & 0x7fffffffu;
         prefix |= digit << shift;
@@ -280,33 +329,6 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
         kept[at] = tok;
         if (C == 1 && at < kRows) places[at] = (uint32_t)tok;
     };
-    uint32_t gt_before = 0, eq_before = 0;  // in the tokens before
-    if (C > 1) {
-        uint32_t gt = 0, eq = 0;
-        for (int32_t g = g0 + tid; g < g1; g += kThreads)
-            each(g, group_at(g), [&](uint32_t key, int) {
-                gt += (key & mask) > prefix;
-                eq += (key & mask) == prefix;
-            });
-        if (tid < 2) counts[tid] = 0;
-        __syncthreads();
-        gt = __reduce_add_sync(0xffffffffu, gt);
-        eq = __reduce_add_sync(0xffffffffu, eq);
-        if (lane == 0) {
-            atomicAdd(&counts[0], gt);
-            atomicAdd(&counts[1], eq);
-        }
-        cluster_sync();
-        uint4 v[kMaxCluster];
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r)
-            v[r] = r < rank ? ld_cluster(ptx::smem_u32(counts), (uint32_t)r) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            gt_before += v[r].x;
-            eq_before += v[r].y;
-        }
-    }
     for (int32_t gb = g0; gb < g1; gb += kThreads) {
         const int32_t g = gb + tid;
         uint32_t cnt = 0, flags = 0;  // (above | equal << 16) of this thread's four tokens
@@ -378,47 +400,63 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
 
     // the weights, one 4-byte element per token
     const bool in_place = p.weights_out == p.weights;
-    if (cut || !in_place) {
+    auto move_weights = [&]() {
+        bool bad = false;
         constexpr int kU = 4;
+#pragma unroll 1
         for (int32_t j0 = 0; j0 < n; j0 += kU * C * kThreads) {
             float v[kU];
-            int64_t dst[kU];
+            int32_t from[kU], to[kU], sp[kU], dp[kU];
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                const int32_t j = j0 + (u * C + rank) * kThreads + tid;
-                dst[u] = -1;
-                if (j < n) {
-                    const int32_t src = cut ? kept_at(j) : j;
-                    int32_t sp, dp;
-                    const int32_t ss = slot_of(p, bt, src, sp), ds = slot_of(p, bt, j, dp);
-                    if (ss >= 0 && ds >= 0 && !(in_place && src == j)) {
-                        v[u] = __ldcg(p.weights + ((int64_t)sp * p.Hkv + h) * p.P + ss);
-                        dst[u] = ((int64_t)dp * p.Hkv + h) * p.P + ds;
-                    }
+                to[u] = j0 + (u * C + rank) * kThreads + tid;
+                from[u] = to[u] < n ? (cut ? __ldcg(kept + to[u]) : to[u]) : -1;
+                if (in_place && from[u] == to[u]) from[u] = -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                sp[u] = dp[u] = 0;
+                if (from[u] >= 0) {
+                    sp[u] = ptx::ld(bt + page_of(p, from[u]));
+                    dp[u] = ptx::ld(bt + page_of(p, to[u]));
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                if (from[u] < 0) continue;
+                from[u] = place_of(p, from[u], sp[u], bad);
+                to[u] = place_of(p, to[u], dp[u], bad);
+                if (to[u] < 0) from[u] = -1;
+                if (from[u] >= 0) v[u] = __ldcg(p.weights + weight_at(p, from[u], h));
             }
             if (in_place) cluster_sync();
 #pragma unroll
             for (int u = 0; u < kU; ++u)
-                if (dst[u] >= 0) p.weights_out[dst[u]] = v[u];
+                if (from[u] >= 0) p.weights_out[weight_at(p, to[u], h)] = v[u];
         }
+        if (bad) atomicOr(p.err, kDevErrBadPage);
+    };
+    if (!cut) {
+        if (!in_place) move_weights();
+        return;
     }
-    if (!cut) return;
     const int32_t S = C / 2, part = rank >> 1;  // CTAs that share the rows of K, or of V
     uint4* pool = static_cast<uint4*>((rank & 1) == 0 ? p.k_cache : p.v_cache);
     const int r0 = tid / p.row_pieces;
     const int rows = kThreads / p.row_pieces;        // rows that the CTA covers at a time
-    const int32_t batch = rows * kPieces;            // and in a batch
+    const int32_t batch = rows * kPieces;            // and in a batch: a power of two
+    const int lb = __ffs(batch) - 1;
     pool += (int64_t)h * p.row_pieces + tid % p.row_pieces;
     const int64_t pitch = (int64_t)p.Hkv * p.row_pieces;
     // rows that stay where they are form a prefix; skip whole strides of it
     const int32_t stride = (n + kThreads - 1) / kThreads;
     const bool still = tid * stride < n && kept_at(tid * stride) == tid * stride;
     const int32_t fixed = __syncthreads_count(still);
+    bool weights_done = false;
     for (int32_t j0 = fixed > 0 ? (fixed - 1) * stride : 0; j0 < n; j0 += kRows * S) {
         const int32_t here = min(kRows * S, n - j0);
         // this CTA's i-th row is row (i / batch * S + part) * batch + i % batch of them
-        auto row_of = [&](int32_t i) { return (i / batch * S + part) * batch + i % batch; };
+        auto row_of = [&](int32_t i) { return ((i >> lb) * S + part) * batch + (i & (batch - 1)); };
         __syncthreads();
         int32_t from[kRows / kThreads];
 #pragma unroll
@@ -428,24 +466,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
         }
         if (at_hand) __syncthreads();  // they are overwritten now
         at_hand = false;
+        bool bad = false;
+        int32_t sp[kRows / kThreads], dp[kRows / kThreads];
 #pragma unroll
         for (int u = 0; u < kRows / kThreads; ++u) {
-            const int32_t i = u * kThreads + tid, r = row_of(i);
+            const int32_t to = j0 + row_of(u * kThreads + tid);
+            if (from[u] == to) from[u] = -1;
+            sp[u] = dp[u] = 0;
+            if (from[u] >= 0) {
+                sp[u] = ptx::ld(bt + page_of(p, from[u]));
+                dp[u] = ptx::ld(bt + page_of(p, to));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRows / kThreads; ++u) {
+            const int32_t i = u * kThreads + tid;
             int32_t s = -1, d = -1;
-            if (from[u] >= 0 && from[u] != j0 + r) {
-                int32_t sp, dp;
-                s = slot_of(p, bt, from[u], sp);
-                d = slot_of(p, bt, j0 + r, dp);
-                if (s >= 0 && d >= 0) {
-                    s += sp * p.P;
-                    d += dp * p.P;
-                } else {
-                    s = -1;
-                }
+            if (from[u] >= 0) {
+                s = place_of(p, from[u], sp[u], bad);
+                d = place_of(p, j0 + row_of(i), dp[u], bad);
+                if (d < 0) s = -1;
             }
             src_slot[i] = s;
             dst_slot[i] = d;
         }
+        if (bad) atomicOr(p.err, kDevErrBadPage);
         __syncthreads();
         const int32_t batches = (here + batch * S - 1) / (batch * S);  // at most kRows / batch
         auto fetch = [&](int32_t k) {
@@ -464,6 +509,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) evict_kernel(const Param
         };
 #pragma unroll
         for (int k = 0; k < kStages; ++k) fetch(k);
+        if (!weights_done) {  // while the first rows are on their way
+            move_weights();
+            weights_done = true;
+        }
         // Every load of a batch, by all who share the rows, is back before any of its rows is
         // overwritten; a thread stores what it loaded itself.  The stores come one batch
         // later, so the wait for the others has a batch's time to pass.
