@@ -15,10 +15,10 @@
  * of its Hq + 2 Hkv rows, 8 lanes per row with two 16-byte pieces each.  A lane's 8 pairs are
  * the same in every row it visits, so cosines and sines are read once per warp into
  * registers.  What a warp waits for is a chain of small loads (sequence, length, page), so
- * the loads that depend on the token's number alone, rows and positions, go first, and 64
- * registers a thread let 32 warps of an SM wait at once.  Prompts of 18,000 tokens with 28 + 8
- * heads: 63.7 us (4.8 TB/s); with 16 rows per warp and 80 registers 69.0 us, with 8 rows per
- * warp 75.7 us.
+ * the loads that depend on the token's number alone, rows and positions, go first, a warp is a
+ * CTA (it leaves its place to the next as soon as it is done), and 72 registers a thread let
+ * 26 of them wait on an SM at once.  Prompts of 18,000 tokens with 28 + 8 heads: 56.3 us (5.4
+ * TB/s, 0.83 of a copy's rate); with four warps per CTA 62.2 us, with 8 rows per warp 86.7 us.
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -30,7 +30,7 @@
 namespace pgqa {
 namespace rope {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 32;
 constexpr int kRowsPerLane = 3;  // rows a lane visits: 12 rows of a token per warp
 
 struct Params {
@@ -88,7 +88,7 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
 }
 
 template <bool KV8>
-__global__ void __launch_bounds__(kThreads, 8) rope_append_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 26) rope_append_kernel(const Params p) {
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int lane = threadIdx.x & 31;

@@ -23,6 +23,7 @@ from ._lib import PgqaError, check, lib
 from .ops import FP8, _scale_array
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+_AXES = bytes(range(64))
 
 # include/pgqa.h's argument structs, field by field
 _ROPE = struct.Struct("N15P21q4i64s")
@@ -38,13 +39,13 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 def _ptr(what, name, t, dtype, dev):
     """Address of a contiguous tensor of `dtype` on CUDA device number `dev`."""
+    if t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
     if t.get_device() != dev:
         raise ValueError(f"{what}: {name} must be on cuda:{dev}, got {t.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{what}: {name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{what}: {name} must be contiguous")
 
 
 def _cache(what, k_cache, block_table, seq_lens):
@@ -196,10 +197,13 @@ def _turn(what, q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos, s
                                    "or without the first dimension for one axis")
             num_axes = ps[0]
     if axes is not None:
-        if len(axes) != pairs or pairs > 64 or min(axes) < 0 or max(axes) >= num_axes:
+        try:
+            axes = bytes(axes)
+        except ValueError:  # an entry below 0 or above 255
+            axes = b""
+        if len(axes) != pairs or axes.translate(None, _AXES[:num_axes]):
             raise PgqaError(2, f"{what}: axes must name one of the {num_axes} axes for each of "
                                f"the {pairs} pairs")
-        axes = bytes(axes)
     elif num_axes > 1:
         raise ValueError(f"{what}: positions on several axes need axes, the axis of each pair")
     if tokens:  # torch gives empty tensors no address
