@@ -33,7 +33,11 @@
  * 384.  The scores of step i + 2 are issued right behind the PV of step i, which frees their
  * buffer, so while a warpgroup works on step i + 1 its next scores are computed and neither
  * waits for the other.  The price is QK^T with N = 64, which re-reads Q from shared memory
- * twice as often: 48 clocks an MMA instead of 32.
+ * twice as often: 48 clocks an MMA instead of 32.  Measured: 2 x 4096 tokens, 32 + 8 heads, over
+ * 8192 keys each 1.01 to 1.04 ms back to back (1060 TFLOP/s, at the power cap) and 859 us in
+ * single calls; with one buffer of 128 columns per tile, where the softmax waits for PV and
+ * QK^T of every step, 1.19 ms back to back.  Prompts of 17 to 1024 tokens over 197 to 4097 keys,
+ * 28 + 4 heads: 160 us (930 TFLOP/s).
  *
  * Every wait is bounded: one that expires sets the device error word and the CTA's abort
  * flag, every role leaves its loop, loads and MMAs in flight are drained and TMEM is freed.

@@ -27,6 +27,11 @@
  * is then the cluster's.  The rows' places are looked up 2048 at a time, so no load waits
  * for an index.  Rows before the first evicted one are not touched.  Bound by reading and
  * writing the moved rows.
+ *
+ * Measured: 16 sequences of 1025 tokens cut to 1024, 8 heads, bf16 14.5 us (0.9 of a copy's
+ * rate over the rows that move); 64 sequences of up to 8192 tokens cut to 2048, 4 heads 92 us
+ * (4.2 TB/s over all of the call, of which the first selects take 12 us); 2 of 32,000 cut to
+ * 8192, 8 heads, e4m3 37 us, of which the select 14.
  */
 #include <cuda_runtime.h>
 #include <math.h>
@@ -86,8 +91,8 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 /* Arrival that orders no memory: for a barrier that only says that loads have returned.  A
- * releasing arrival waits for the thread's stores to reach L2 as well (evict-long-e4m3: the
- * first stall reason). */
+ * releasing arrival waits for the thread's stores to reach L2 as well (2 sequences of 32,000
+ * tokens cut to 8192, 8 heads, e4m3: 55.4 us instead of 45.7). */
 __device__ __forceinline__ void cluster_arrive_relaxed() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
@@ -218,7 +223,8 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
         if (C == 1) {
             // alone: all bins at once, from the top; thread t owns those from `top` down.  The
             // warp whose bins hold the `need`-th key of those left, then the thread and the bin
-            // (three levels by one warp, as below: evict-step 16.4 us instead of 13.9)
+            // (three levels by one warp, as below: 16.4 us instead of 13.9 for 16 sequences of 1025
+            // tokens cut to 1024, 8 heads)
             constexpr int kOwn = kBins / kThreads;
             const int top = kBins - 1 - kOwn * tid;
             uint32_t c[kOwn], sum = 0;
@@ -251,7 +257,8 @@ __device__ void select_kept(const Params& p, const int32_t* bt, int32_t L, int32
             if (tid < 2) counts[tid] = 0;
         } else {
             // together: sums of 32 bins each, so that the others read these and one group of
-            // 32 of this CTA's histogram instead of all of it (evict-long-e4m3: 37 us instead of 44)
+            // 32 of this CTA's histogram instead of all of it (37 us instead of 44 for 2 sequences
+            // of 32,000 tokens cut to 8192, 8 heads, e4m3)
             for (int i = warp; i < kBins / 32; i += kThreads / 32) {
                 const uint32_t v = __reduce_add_sync(0xffffffffu, hist[32 * i + lane]);
                 if (lane == 0) coarse[pass][i] = v;

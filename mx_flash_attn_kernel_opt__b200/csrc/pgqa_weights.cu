@@ -14,7 +14,7 @@
  * mma.sync A fragments: the order of the 128 dimensions inside the dot product is free as
  * long as q uses the same one, so lane (g, t) takes 16-byte pieces t, t + 4, ... of token
  * rows g and g + 8, whole 64-byte runs per row, and q rows are loaded by the same
- * addresses as B fragments.  Two to four chunks
+ * addresses as B fragments.  Two or three chunks
  * are held, one at work and the others in flight.  The four lanes
  * that share a token add their partial sums by shuffles, and the token's weight gets one
  * red.add: no other warp of the call adds to it (unless sequences share a page), so the
@@ -24,6 +24,11 @@
  * once per unit: each row times the power of two that brings its largest element to [2^14,
  * 2^15), undone in fp32 (8 significant bits fit f16's 11; an element 2^28 times smaller than
  * its row's largest is rounded to 2^-25).
+ *
+ * Measured: 290,000 tokens in 256 sequences, 8 KV heads, 4 rows each, bf16 101 us (6.1 TB/s,
+ * 0.93 of a copy's rate); 2 sequences of 32,768 tokens, e4m3: 20 us with 8 rows per KV head
+ * (start and end of the call, about 8 us, included), 34 us with 32 and 59 us with 64, where
+ * the products and exponentials of a chunk take longer than its load.
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
