@@ -244,14 +244,19 @@ struct Walker {
         }
         if (kvh == p.Hkv) {
             kvh = 0;
-            do {
-                ++b;
-                if (++cur_lane == 32) {
-                    cur_lane = 0;
-                    mine = load_seq(p, b + lane, false);
-                }
-                pick();
-            } while (cur.items == 0);  // some is left, so another sequence has items
+            // the next sequence with items; some is left, so there is one
+            int32_t from = cur_lane + 1;
+            uint32_t some = __ballot_sync(0xffffffffu, mine.items > 0 && lane >= from);
+            b += 1;
+            while (some == 0) {
+                b += 32 - from;
+                from = 0;
+                mine = load_seq(p, b + lane, false);
+                some = __ballot_sync(0xffffffffu, mine.items > 0);
+            }
+            cur_lane = __ffs(some) - 1;
+            b += cur_lane - from;
+            pick();
         }
         it.b = b;
         it.kvh = kvh;

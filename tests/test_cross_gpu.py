@@ -99,6 +99,16 @@ def test_many_sequences(cuda_device):
     run_and_check(make(new, lens, 8, 4, 16, seed=2), cuda_device)
 
 
+def test_few_sequences_with_tokens_among_many(cuda_device):
+    """Long runs of sequences without prompt tokens between those with some, and keys of 0."""
+    new, lens = [0] * 333, [30 + i % 50 for i in range(333)]
+    for at, n, L in ((0, 5, 100), (31, 3, 0), (32, 70, 300), (95, 1, 16), (96, 2, 129), (200, 40, 513), (332, 9, 77)):
+        new[at], lens[at] = n, L
+    run_and_check(make(new, lens, 8, 2, 16, seed=40), cuda_device)
+    new[332] = 0
+    run_and_check(make(new, lens, 4, 4, 16, seed=41), cuda_device)
+
+
 def test_more_items_than_sms_and_long_keys(cuda_device):
     run_and_check(make([600, 900], [3000, 1111], 32, 8, 16, seed=3), cuda_device)
 

@@ -201,3 +201,22 @@ def test_cross_attention_refuses_bad_tensors(cuda_device):
         with pytest.raises(error):
             pgqa.cross_attention(*args, bt, lens, **kw)
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_batches_past_the_shared_memory_table_are_refused(cuda_device):
+    """accumulate_weights keeps the chunk counts of all sequences in shared memory."""
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=cuda_device)  # noqa: E731
+    k, w = z(1, 16, 1, 128, dtype=torch.bfloat16), z(1, 1, 16)
+    for B, Sq, ok in ((20000, 1, True), (40000, 1, False), (40000, 9, False), (20000, 17, False), (9000, 17, True)):
+        call = lambda: pgqa.accumulate_weights(  # noqa: E731
+            z(B, Sq, 1, 128, dtype=torch.bfloat16), k, z(B, 1, dtype=torch.int32), z(B, dtype=torch.int32),
+            z(B, 1, Sq), w)
+        if ok:
+            call()
+        else:
+            with pytest.raises(pgqa.PgqaError) as e:
+                call()
+            assert e.value.status == 3
+    pgqa.check_device_error()
+    assert (w == 0).all()
