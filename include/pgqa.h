@@ -370,14 +370,15 @@ int pgqa_evict(const pgqa_evict_args* args, void* stream);
  * Cross attention: out[x, h] = softmax(scale * q[x, h] . K^T) . V over the first seq_lens[b]
  * tokens of sequence b's pages, for every query token x of sequence b.  No causal mask; the
  * number of query tokens and of keys are unrelated.  A sequence without keys gives zeros
- * (and a log-sum-exp of -inf).  bf16 in and out, fp32 scores, sums and accumulators.
+ * (and a log-sum-exp of -inf).  q and out bf16, fp32 scores, sums and accumulators.
  *   q            [tokens, Hq, 128], token stride q_stride elements (a multiple of 8, at
  *                least Hq * 128), heads contiguous
  *   out          [tokens, Hq, 128], contiguous
  *   cu_seqlens   NULL: [batch_size, seqlen_q] tokens, tokens = batch_size * seqlen_q.
  *                Else int32 [batch_size + 1], ascending from 0; rows of out and softmax_lse
  *                from cu[batch_size] on are left as they are
- *   k, v pools   [num_pages, P, Hkv, 128] bf16, as in the decode; g = Hq / Hkv <= 128
+ *   k, v pools   [num_pages, P, Hkv, 128] bf16 (kv_format 0) or e4m3 (1, with k_scale and
+ *                v_scale), as in the decode; g = Hq / Hkv <= 128
  *   softmax_lse  NULL or fp32: [Hq, tokens] with cu_seqlens, else [B, Hq, seqlen_q]
  *   workspace    pgqa_cross_workspace_size(...) bytes (at most 40 MB on a B200), 256-byte
  *                aligned, any contents: parts of results that several CTAs share.  Calls
@@ -396,7 +397,9 @@ typedef struct pgqa_cross_args {
     int64_t batch_size, seqlen_q, tokens, q_stride, num_heads, num_heads_k, headdim;
     int64_t page_size, num_pages, bt_stride;
     float scale;
-    int32_t reserved;
+    int32_t kv_format;
+    const float* k_scale;
+    const float* v_scale;
     void* workspace;
     size_t workspace_bytes;
 } pgqa_cross_args;

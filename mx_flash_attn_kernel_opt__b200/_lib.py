@@ -113,7 +113,8 @@ class PgqaCrossArgs(ctypes.Structure):
         ("q_stride", c_int64), ("num_heads", c_int64), ("num_heads_k", c_int64),
         ("headdim", c_int64), ("page_size", c_int64), ("num_pages", c_int64),
         ("bt_stride", c_int64),
-        ("scale", c_float), ("reserved", c_int32),
+        ("scale", c_float), ("kv_format", c_int32),
+        ("k_scale", c_void_p), ("v_scale", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 

@@ -27,6 +27,11 @@
  *   warp 8          TMA: Q tiles, and 128-key tiles of K and V by page boxes through one
  *                   ring of five 32 KB slots; it zeroes V rows behind the last key, so that
  *                   a weight of 0 never meets a NaN left in a page.
+ *   warps 12-15     (e4m3 pages) turn the tiles that TMA brings as they are into bf16, exactly,
+ *                   in the ring that the MMAs read (four slots then); the scales go into the
+ *                   score's factor and the normaliser.  2 x 4096 tokens, 32 + 8 heads, over 8192
+ *                   keys: 1.03 ms, 0.92 ms from bf16 pages on the same GPU; two such
+ *                   warpgroups leave 96 registers a thread, and the spills cost more (1.12 ms).
  *   warps 9, 10     issue the MMAs of tile 0 and of tile 1: S = Q K^T (both from shared
  *                   memory), O += P V (P from TMEM).
  * TMEM: two score buffers of 64 columns for each tile (from columns 0 and 128), O at 256 and
@@ -56,15 +61,24 @@
 namespace pgqa {
 namespace cross {
 
-constexpr int kThreads = 352;
+constexpr int kThreads = 352;              // bf16 pages; e4m3 pages: and a warpgroup that converts
 constexpr int kTile = 128;                 // rows of a tile, and keys of a K / V tile
 constexpr int kHalf = kTile * 128;         // one 64-dimension half of a tile, bf16
 constexpr int kSlot = 2 * kHalf;
-constexpr int kSlots = 5;
-constexpr int kQOff = 0, kRingOff = 2 * kSlot, kBarOff = kRingOff + kSlots * kSlot;
 constexpr int kStep = 64;                  // keys of a softmax step
-constexpr int kBars = 2 * kSlots + 16;
-constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
+constexpr int kQOff = 0, kRingOff = 2 * kSlot;
+/* Shared memory: Q tiles, the ring of bf16 K and V tiles, for e4m3 pages a ring of tiles as
+ * they come, barriers, then 16 bytes. */
+template <bool KV8>
+struct Geo {
+    static constexpr int kThreads = KV8 ? 512 : cross::kThreads;
+    static constexpr int kSlots = KV8 ? 4 : 5;
+    static constexpr int kRaw = KV8 ? 2 : 0;  // tiles of kHalf bytes
+    static constexpr int kRawOff = kRingOff + kSlots * kSlot;
+    static constexpr int kBarOff = kRawOff + kRaw * kHalf;
+    static constexpr int kBars = 2 * kSlots + 16 + 2 * kRaw;
+    static constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
+};
 constexpr int kRows = 2 * kTile;           // rows of a work item
 // What an item costs beside its key tiles, in key tiles (1 to 4 measured: 175, 159, 167, 166 us
 // for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys), and the least length of a slice.
@@ -78,6 +92,7 @@ struct Params {
     float* lse;              // optional: [Hq, T] packed, [B, Hq, S] padded
     float *rec_o, *rec_lse;  // parts of cut items: [2 * grid][256 rows][128], [2 * grid][256] (log2 units)
     const int32_t *seq_lens, *block_table, *cu;
+    const float *k_scale, *v_scale;  // e4m3 pools: factor per KV head (null = 1)
     struct Cut* cuts;        // [grid]
     int32_t* err;
     int64_t bt_stride, cap_tokens;
@@ -149,6 +164,7 @@ __device__ __forceinline__ int64_t snapped(int64_t off, int64_t len, int64_t tol
 }
 
 /* By all threads of a block (a multiple of 32, at most 1024); the result in shared memory. */
+template <int kThreads>
 __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
     __shared__ int64_t wsum[kThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -301,6 +317,20 @@ __device__ Cut cut_of(const Params& p, int32_t c, const Slice& s) {
     return k;
 }
 
+/* Four e4m3 numbers as bf16 pairs, NaN excepted (comes out as 480): the exponent and mantissa
+ * bits stand in the low bits of bf16's, which is the value times 2^(7 - 127), subnormals
+ * too, and the product with 2^120 is exact.  Shifts by multiplication, so that the integer
+ * and the FMA pipes share the work; the four converting warps are what bounds short prompts
+ * (16 x 3 tokens, 32 + 8 heads, over 16,000 keys: 262 us with conversion instructions, which
+ * leave at a fraction of the rate, 245 us with shifts and masks, 224 to 232 us so). */
+__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t b, uint32_t& lo, uint32_t& hi) {
+    // 16-bit lanes 0000 s eeee mmm 0000; the sign goes from bit 11 to bit 15: + 15 * 2^11
+    const uint32_t x = __byte_perm(b, 0, 0x4140) * 16u, y = __byte_perm(b, 0, 0x4342) * 16u;
+    const uint32_t mx = (x & 0x08000800u) * 15u + x, my = (y & 0x08000800u) * 15u + y;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(mx), "r"(0x7b807b80u));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(my), "r"(0x7b807b80u));
+}
+
 /* 32 bytes to global memory in one instruction. */
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
@@ -308,12 +338,23 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
                  : "memory");
 }
 
-__global__ void __launch_bounds__(kThreads, 1)
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+                                         int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <bool KV8>
+__global__ void __launch_bounds__(Geo<KV8>::kThreads, 1)
 cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
              const __grid_constant__ CUtensorMap vmap, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t sb = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (sb - ptx::smem_u32(smem_raw));
+    constexpr int kSlots = Geo<KV8>::kSlots, kRaw = Geo<KV8>::kRaw, kBarOff = Geo<KV8>::kBarOff;
     const uint32_t bars = sb + kBarOff;
     auto FULL = [&](int s) { return bars + 8u * s; };
     auto EMPTY = [&](int s) { return bars + 8u * (kSlots + s); };
@@ -325,7 +366,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     auto PVDONE = [&](int w, int u) { return bars + 8u * (2 * kSlots + 8 + 2 * w + u); };
     const uint32_t QFULL = bars + 8u * (2 * kSlots + 12), QEMPTY = bars + 8u * (2 * kSlots + 13);
     const uint32_t TAIL = bars + 8u * (2 * kSlots + 14), MMADONE = bars + 8u * (2 * kSlots + 15);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarOff + kBars * 8);
+    // e4m3 pages: a tile as it came is there, and has been converted
+    auto RFULL = [&](int s) { return bars + 8u * (2 * kSlots + 16 + s); };
+    auto REMPTY = [&](int s) { return bars + 8u * (2 * kSlots + 16 + kRaw + s); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarOff + Geo<KV8>::kBars * 8);
     volatile int32_t* abort_flag = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, lane = tid & 31;
@@ -335,7 +379,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         ptx::prefetch_tensormap(&kmap);
         ptx::prefetch_tensormap(&vmap);
         for (int s = 0; s < kSlots; ++s) {
-            ptx::mbar_init(FULL(s), 1);
+            ptx::mbar_init(FULL(s), KV8 ? 4 : 1);  // e4m3: one arrival per converting warp
             ptx::mbar_init(EMPTY(s), 2);  // both tiles are done with it
         }
         for (int w = 0; w < 2; ++w) {
@@ -347,6 +391,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         ptx::mbar_init(QFULL, 1);
         ptx::mbar_init(QEMPTY, 2);
+        for (int s = 0; s < kRaw; ++s) {
+            ptx::mbar_init(RFULL(s), 1);
+            ptx::mbar_init(REMPTY(s), 4);
+        }
         ptx::mbar_init(TAIL, 1);
         ptx::mbar_init(MMADONE, 2);
         *abort_flag = 0;
@@ -398,7 +446,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     };
 
     __shared__ Slice slice;
-    find_slice(p, blockIdx.x, slice);
+    find_slice<Geo<KV8>::kThreads>(p, blockIdx.x, slice);
     if (tid == 0) p.cuts[blockIdx.x] = cut_of(p, blockIdx.x, slice);
     Walker wk;
     wk.init(p, slice, lane);
@@ -432,33 +480,28 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 const int32_t nvalid = min(kTile, it.L - tile * kTile);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    const int slot = n_kv % kSlots;
-                    if (n_kv >= kSlots && !wait_all(EMPTY(slot), ((n_kv / kSlots) - 1) & 1)) {
+                    constexpr int kRing = KV8 ? kRaw : kSlots;
+                    const int slot = n_kv % kRing;
+                    if (n_kv >= kRing && !wait_all(KV8 ? REMPTY(slot) : EMPTY(slot), ((n_kv / kRing) - 1) & 1)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t dst = sb + kRingOff + (uint32_t)slot * kSlot;
-                    // a V tile that ends inside a 16-key step is finished here before its release
-                    const bool tail = kv == 1 && (nvalid & 15) != 0;
-                    const uint32_t bar = tail ? TAIL : FULL(slot);
+                    const uint32_t dst = KV8 ? sb + Geo<KV8>::kRawOff + (uint32_t)slot * kHalf
+                                             : sb + kRingOff + (uint32_t)slot * kSlot;
+                    // a bf16 V tile that ends inside a 16-key step is finished here before its release
+                    const bool tail = !KV8 && kv == 1 && (nvalid & 15) != 0;
+                    const uint32_t bar = KV8 ? RFULL(slot) : (tail ? TAIL : FULL(slot));
                     if (lane == 0) {
                         const bool stuck = p.debug_stuck > 0 && blockIdx.x == 0 && n_kv == 0;
-                        ptx::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * 256) + (stuck ? 16u : 0u));
+                        ptx::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * (KV8 ? 128 : 256)) + (stuck ? 16u : 0u));
                     }
                     __syncwarp();
                     if (mine) {
                         const CUtensorMap* map = kv ? &vmap : &kmap;
-                        // K and V tiles are read again by the other q tiles of the sequence
-                        asm volatile(
-                            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-                            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst + (uint32_t)(lane * box) * 128u),
-                            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(0), "r"(it.kvh), "r"(z)
-                            : "memory");
-                        asm volatile(
-                            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-                            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst + kHalf + (uint32_t)(lane * box) * 128u),
-                            "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(64), "r"(it.kvh), "r"(z)
-                            : "memory");
+                        // K and V tiles are read again by the other q tiles of the sequence: no
+                        // eviction hint
+                        tma_load(dst + (uint32_t)(lane * box) * 128u, map, bar, 0, it.kvh, z);
+                        if (!KV8) tma_load(dst + kHalf + (uint32_t)(lane * box) * 128u, map, bar, 64, it.kvh, z);
                     }
                     ++n_kv;
                     if (tail) {
@@ -492,13 +535,8 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             ptx::mbar_arrive_expect_tx(QFULL, two ? 2 * bytes : bytes);
                             for (int w = 0; w < (two ? 2 : 1); ++w)
                                 for (int hf = 0; hf < 2; ++hf)
-                                    asm volatile(
-                                        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx"
-                                        "::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-                                            sb + kQOff + (uint32_t)(w * kSlot + hf * kHalf)),
-                                        "l"(reinterpret_cast<uint64_t>(&qmap)), "r"(QFULL), "r"(hf * 64),
-                                        "r"(it.kvh * p.g), "r"(it.tok0 + w * p.tile_tokens)
-                                        : "memory");
+                                    tma_load(sb + kQOff + (uint32_t)(w * kSlot + hf * kHalf), &qmap, QFULL, hf * 64,
+                                             it.kvh * p.g, it.tok0 + w * p.tile_tokens);
                         }
                         __syncwarp();
                         ++n_q;
@@ -509,11 +547,13 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         }
         // loads of the last slots may still be in flight (after an abort)
         if (lane == 0) {
-            for (int k = n_kv > kSlots ? n_kv - kSlots : 0; k < n_kv; ++k) drain_bar(FULL(k % kSlots), (k / kSlots) & 1);
+            constexpr int kRing = KV8 ? kRaw : kSlots;
+            for (int k = n_kv > kRing ? n_kv - kRing : 0; k < n_kv; ++k)
+                drain_bar(KV8 ? RFULL(k % kRing) : FULL(k % kRing), (k / kRing) & 1);
             if (n_q > 0) drain_bar(QFULL, (n_q - 1) & 1);
         }
         __syncwarp();
-    } else if (warp >= 9) {
+    } else if (warp == 9 || warp == 10) {
         /* ================= MMA issuers: warp 9 tile 0, warp 10 tile 1 ================= */
         const int w = warp - 9;
         const uint32_t tS = tmem + (uint32_t)w * 128u, tO = tmem + 256u + (uint32_t)w * 128u;
@@ -596,7 +636,72 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         ptx::tc_commit_elect(MMADONE);
         if (lane == 0) drain_bar(MMADONE, 0);
         __syncwarp();
-    } else {
+    } else if (warp >= 12) {
+        /* ================= e4m3 tiles to bf16 (KV8) ================= */
+        // thread = key: its 128 bytes become two 128-byte halves in the swizzle the MMAs read;
+        // V rows behind the last key, up to the end of their 16-key step, become zeros
+        const int row = tid - 384;
+        const uint32_t sw = (uint32_t)(row & 7);
+        int n = 0;
+        bool ok = KV8;
+        while (ok && wk.next(p, lane, it)) {
+            for (int32_t tile = it.t0; ok && tile < it.t1; ++tile) {
+                const int32_t nvalid = it.L - tile * kTile;
+#pragma unroll 1
+                for (int kv = 0; kv < 2; ++kv, ++n) {
+                    constexpr int kRing = KV8 ? kRaw : 1;
+                    const int raw = n % kRing, slot = n % kSlots;
+                    // both at once where neither is waited for
+                    const bool r = ptx::mbar_try_wait(RFULL(raw), (n / kRing) & 1);
+                    const bool e = n < kSlots || ptx::mbar_try_wait(EMPTY(slot), ((n / kSlots) - 1) & 1);
+                    if (!__all_sync(0xffffffffu, r && e)) {
+                        ok = wait_all(RFULL(raw), (n / kRing) & 1) &&
+                             (n < kSlots || wait_all(EMPTY(slot), ((n / kSlots) - 1) & 1));
+                        if (!ok) break;
+                    }
+                    const uint32_t src = sb + Geo<KV8>::kRawOff + (uint32_t)(raw * kHalf + row * 128);
+                    const uint32_t dst = sb + kRingOff + (uint32_t)(slot * kSlot + row * 128);
+                    if (row >= nvalid) {
+                        if (row < ((nvalid + 15) & ~15))
+                            for (uint32_t x = 0; x < 16; ++x)
+                                ptx::sts_u4(dst + (x >> 3) * kHalf + ((x & 7u) << 4), make_uint4(0, 0, 0, 0));
+                    } else {
+                        uint32_t nan = 0;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {  // 16 dimensions each
+                            const uint4 v = ptx::lds_u4(src + (((uint32_t)c ^ sw) << 4));
+                            const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+                            uint32_t h[8];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                e4m3x4_to_bf16(b[e], h[2 * e], h[2 * e + 1]);
+                                nan |= (b[e] & 0x7f7f7f7fu) + 0x01010101u;
+                            }
+                            const uint32_t half = dst + (uint32_t)((c >> 2) * kHalf), cc = (uint32_t)(2 * (c & 3));
+                            ptx::sts_u4(half + ((cc ^ sw) << 4), make_uint4(h[0], h[1], h[2], h[3]));
+                            ptx::sts_u4(half + (((cc + 1) ^ sw) << 4), make_uint4(h[4], h[5], h[6], h[7]));
+                        }
+                        if (nan & 0x80808080u) {  // some element is NaN: its bytes read again
+#pragma unroll 1
+                            for (uint32_t x = 0; x < 128; ++x) {
+                                const uint32_t at = ((x >> 4) ^ sw) * 16u + (x & 15u);
+                                const uint32_t to = (x >> 6) * kHalf + ((((x >> 3) & 7u) ^ sw) << 4) + (x & 7u) * 2u;
+                                if ((smem[src - sb + at] & 0x7fu) == 0x7fu)
+                                    *reinterpret_cast<uint16_t*>(smem + (dst - sb) + to) = 0x7fffu;
+                            }
+                        }
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive(FULL(slot));
+                        ptx::mbar_arrive(REMPTY(raw));
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8) {
         /* ================= softmax and output ================= */
         const int w = warp >> 2;
         const int row = (warp & 3) * 32 + lane;
@@ -612,6 +717,16 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const bool valid = row < p.tile_tokens * p.g && tok < it.tok_end;
             const int head = it.kvh * p.g + my_head;
             float m_ref = -INFINITY, l = 0.f;
+            float mul = p.scale_log2, sign = 1.f;
+            if (KV8 && p.k_scale) {
+                // the factor has to be positive for the masked -inf and the maximum: a scale of
+                // zero (a head quantised from zeros) or below goes into the scores instead
+                mul *= ptx::ld(p.k_scale + it.kvh);
+                if (mul <= 0.f) {
+                    sign = mul < 0.f ? -1.f : 0.f;
+                    mul = mul < 0.f ? -mul : 1.f;
+                }
+            }
             const int m = steps_of(it.L, it.t0, it.t1);
 #pragma unroll 1
             for (int i = 0; i < m; ++i, ++n_s) {
@@ -626,6 +741,10 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 for (int c = 0; c < 2; ++c)
                     ptx::tc_ld32(tB + 32u * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
                 ptx::tc_wait_ld();
+                if (KV8 && sign != 1.f) {
+#pragma unroll
+                    for (int k = 0; k < kStep; ++k) s[k] *= sign;
+                }
                 const int32_t nvalid = it.L - (it.t0 * kTile + i * kStep);
                 if (nvalid < kStep) {
 #pragma unroll
@@ -642,7 +761,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                 for (int e = 0; e < 8; ++e) m8[e] = fmaxf(m8[e], s[56 + e]);
                 const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
+                                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * mul;
                 const bool raise = mx > m_ref + kLazyLog2;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float m_new = raise ? mx : m_ref;
@@ -667,7 +786,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
                 }
                 const float base = m_ref == -INFINITY ? 0.f : m_ref;
-                const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                const float2 mul2 = make_float2(mul, mul), sub2 = make_float2(-base, -base);
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 uint32_t pk[kStep / 2];
 #pragma unroll
@@ -696,7 +815,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 ptx::tc_fence_after();
             }
             // a row whose scores are all -inf has no weight to normalise by
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = l == 0.f ? 0.f : (KV8 && p.v_scale ? ptx::ld(p.v_scale + it.kvh) : 1.f) / l;
             const int64_t at = (int64_t)tok * p.Hq + head;
             // part of a cut item: the slice's first one if it begins before the slice, else its last
             const int64_t rec = (int64_t)(2 * blockIdx.x + (it.t0 > 0 ? 0 : 1)) * kRows + w * kTile + row;
@@ -809,17 +928,19 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-/* (128 dims, heads, tokens) with 64-dimension boxes, 128-byte swizzle; boxes past the end read zeros. */
+/* (128 dims, heads, tokens) with boxes of 128 bytes of a row (64 bf16, 128 e4m3), 128-byte
+ * swizzle; boxes past the end read zeros. */
 int encode(CUtensorMap* map, const void* base, int64_t heads, int64_t tokens, int64_t token_stride_bytes,
-           int64_t box_heads, int64_t box_tokens) {
+           int64_t box_heads, int64_t box_tokens, bool e4m3 = false) {
     EncodeFn fn = reinterpret_cast<EncodeFn>(host_encode_tiled());
     if (fn == nullptr) return PGQA_ERR_CUDA;
     cuuint64_t dims[3] = {128, (cuuint64_t)heads, (cuuint64_t)tokens};
-    cuuint64_t strides[2] = {256, (cuuint64_t)token_stride_bytes};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
+    cuuint64_t strides[2] = {e4m3 ? 128u : 256u, (cuuint64_t)token_stride_bytes};
+    cuuint32_t box[3] = {e4m3 ? 128u : 64u, (cuuint32_t)box_heads, (cuuint32_t)box_tokens};
     cuuint32_t step[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return fn(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              e4m3 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? PGQA_OK
                : PGQA_ERR_CUDA;
@@ -845,6 +966,16 @@ int shape_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t P
 
 size_t workspace_bytes(int grid) { return (size_t)grid * (2 * kRows * (128 + 1) * 4 + sizeof(Cut)); }
 
+template <bool KV8>
+int launch(const Params& p, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int dev,
+           cudaStream_t stream) {
+    static int done[kHostMaxDevices] = {0};
+    using G = Geo<KV8>;
+    const int st = host_smem_limit(cross_kernel<KV8>, dev, G::kSmem, done);
+    if (st != PGQA_OK) return st;
+    return host_launch(cross_kernel<KV8>, dim3((unsigned)p.grid), G::kThreads, G::kSmem, stream, 1, qm, km, vm, p);
+}
+
 int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (a == nullptr) return PGQA_ERR_NULL_POINTER;
     if (a->struct_size != sizeof(pgqa_cross_args)) return PGQA_ERR_BAD_SHAPE;
@@ -852,6 +983,9 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
         return PGQA_ERR_NULL_POINTER;
     int st = shape_ok(a->tokens, a->batch_size, a->num_heads, a->num_heads_k, a->headdim, a->page_size, a->bt_stride);
     if (st != PGQA_OK) return st;
+    if (a->kv_format != 0 && a->kv_format != 1) return PGQA_ERR_UNSUPPORTED;
+    const bool kv8 = a->kv_format == 1;
+    if (!kv8 && (a->k_scale || a->v_scale)) return PGQA_ERR_BAD_SHAPE;
     if (a->num_pages <= 0) return PGQA_ERR_BAD_SHAPE;
     if (a->num_pages >= ((int64_t)1 << 31) / a->page_size) return PGQA_ERR_UNSUPPORTED;
     if (!a->cu_seqlens && (a->seqlen_q < 0 || a->tokens != a->batch_size * a->seqlen_q)) return PGQA_ERR_BAD_SHAPE;
@@ -860,7 +994,7 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (a->q_stride % 8 != 0 || !host_aligned(a->q, 16) || !host_aligned(a->k_cache, 16) ||
         !host_aligned(a->v_cache, 16) || !host_aligned(a->out, 16) || !host_aligned(a->softmax_lse, 4) ||
         !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) || !host_aligned(a->cu_seqlens, 4) ||
-        !host_aligned(a->workspace, 256))
+        !host_aligned(a->workspace, 256) || !host_aligned(a->k_scale, 4) || !host_aligned(a->v_scale, 4))
         return PGQA_ERR_MISALIGNED;
     if (a->q_stride >= ((int64_t)1 << 39)) return PGQA_ERR_UNSUPPORTED;  // a tensor map's stride is 40 bits
     int dev, sms, optin;
@@ -883,6 +1017,8 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     p.seq_lens = a->seq_lens;
     p.block_table = a->block_table;
     p.cu = a->cu_seqlens;
+    p.k_scale = a->k_scale;
+    p.v_scale = a->v_scale;
     p.bt_stride = a->bt_stride;
     p.B = (int32_t)a->batch_size;
     p.S = (int32_t)a->seqlen_q;
@@ -903,13 +1039,12 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     p.debug_stuck = (stuck && *stuck) ? atoi(stuck) : 0;
     CUtensorMap qm, km, vm;
     const int64_t slots = a->num_pages * a->page_size;
+    const int64_t row = kv8 ? 128 : 256;
     if ((st = encode(&qm, a->q, a->num_heads, a->tokens, a->q_stride * 2, p.g, p.tile_tokens)) != PGQA_OK ||
-        (st = encode(&km, a->k_cache, a->num_heads_k, slots, a->num_heads_k * 256, 1, p.box)) != PGQA_OK ||
-        (st = encode(&vm, a->v_cache, a->num_heads_k, slots, a->num_heads_k * 256, 1, p.box)) != PGQA_OK)
+        (st = encode(&km, a->k_cache, a->num_heads_k, slots, a->num_heads_k * row, 1, p.box, kv8)) != PGQA_OK ||
+        (st = encode(&vm, a->v_cache, a->num_heads_k, slots, a->num_heads_k * row, 1, p.box, kv8)) != PGQA_OK)
         return st;
-    static int done[kHostMaxDevices] = {0};
-    if ((st = host_smem_limit(cross_kernel, dev, kSmem, done)) != PGQA_OK) return st;
-    st = host_launch(cross_kernel, dim3((unsigned)p.grid), kThreads, kSmem, stream, 1, qm, km, vm, p);
+    st = kv8 ? launch<true>(p, qm, km, vm, dev, stream) : launch<false>(p, qm, km, vm, dev, stream);
     if (st != PGQA_OK || p.grid == 1) return st;
     return host_launch(join_kernel, dim3((unsigned)(p.grid - 1), kRows / 32), kJoinThreads, 0, stream, 1, p);
 }

@@ -29,7 +29,7 @@ _AXES = bytes(range(64))
 _ROPE = struct.Struct("N15P21q4i64s")
 _WEIGHTS = struct.Struct("N7P9qfi")
 _EVICT = struct.Struct("N8P9q2i")
-_CROSS = struct.Struct("N8P10qfiPN")
+_CROSS = struct.Struct("N8P10qfi3PN")
 
 
 # The handle of torch's current stream (a Stream object takes twenty times as long to make).
@@ -314,13 +314,14 @@ def _cross_workspace(dev, *shape):
 
 
 def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=None, scale=None,
-                    out=None, return_lse=False):
+                    k_scale=None, v_scale=None, out=None, return_lse=False):
     """Attention of query tokens over each sequence's encoder states, held in pages:
     softmax(scale * q K^T) V over the first seq_lens[b] tokens of sequence b, no causal mask.
 
     q [B, Sq, Hq, 128] bf16, or packed [tokens, Hq, 128] with `cu_seqlens_q` [B + 1] int32,
     ascending from 0; its token stride may be any multiple of 8 elements (a slice of a
-    projection), heads contiguous.  k_cache / v_cache [num_pages, P, Hkv, 128] bf16,
+    projection), heads contiguous.  k_cache / v_cache [num_pages, P, Hkv, 128] bf16 or
+    float8_e4m3fn (an element of KV head h is worth e4m3 * k_scale[h], v_scale for V),
     block_table [B, width] int32, seq_lens [B] int32 (0: the sequence's rows are zeros).
 
     Returns out (contiguous, q's shape) or (out, lse) with `return_lse`: fp32 [Hq, tokens]
@@ -329,9 +330,12 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     what = "cross_attention"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
     num_pages, P, Hkv, D = shape
-    if fp8:
-        raise NotImplementedError(f"{what}: float8_e4m3fn pools are not implemented here")
     vp = _v_pool(what, v_cache, k_cache, dev)
+    ks = vs = None
+    if fp8:
+        ks, vs = _scales(k_scale, Hkv, dev), _scales(v_scale, Hkv, dev)
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("k_scale / v_scale apply to float8_e4m3fn pools only")
     if q.dtype is not _BF16:
         raise TypeError(f"{what}: q must be {_BF16}, got {q.dtype}")
     if q.get_device() != dev:
@@ -376,6 +380,6 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
         _call(lib().pgqa_cross_attention, _CROSS.pack(
             _CROSS.size, q.data_ptr(), kp, vp, op, 0 if lse is None else lse.data_ptr(), lp, tp, cup, B,
             Sq, tokens, stride, Hq, Hkv, D, P, num_pages, width,
-            1.0 / math.sqrt(D) if scale is None else scale, 0, 0 if ws is None else ws.data_ptr(), need),
-            dev, "pgqa_cross_attention")
+            1.0 / math.sqrt(D) if scale is None else scale, 1 if fp8 else 0, 0 if ks is None else ks.data_ptr(),
+            0 if vs is None else vs.data_ptr(), 0 if ws is None else ws.data_ptr(), need), dev, "pgqa_cross_attention")
     return (out, lse) if return_lse else out

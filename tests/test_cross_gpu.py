@@ -17,16 +17,16 @@ from tests import _paged
 pytestmark = pytest.mark.gpu
 
 
-def make(new, lens, Hq, Hkv, P, seed=0, std=1.0):
+def make(new, lens, Hq, Hkv, P, seed=0, std=1.0, kv="bf16"):
     g = torch.Generator().manual_seed(seed)
     bt, pages = _paged.table(lens, P, g)
-    k, v = (_paged.poison_unused(_paged.pool(pages, P, Hkv, g, std=std), lens, bt, P) for _ in range(2))
+    k, v = (_paged.poison_unused(_paged.pool(pages, P, Hkv, g, kv, std), lens, bt, P) for _ in range(2))
     q = torch.randn(sum(new), Hq, 128, generator=g).to(torch.bfloat16)
     return q, k, v, bt, torch.tensor(lens, dtype=torch.int32), \
         torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32)
 
 
-def reference(q, k, v, bt, lens, cu, scale, dev):
+def reference(q, k, v, bt, lens, cu, scale, dev, ks=None, vs=None):
     """64 bits, on the device: out, lse [Hq, T], sum of |weight * v|, score bound."""
     T, Hq, _ = q.shape
     Hkv, P = k.shape[2], k.shape[1]
@@ -34,7 +34,10 @@ def reference(q, k, v, bt, lens, cu, scale, dev):
     mag = torch.zeros_like(out)
     lse = torch.full((Hq, T), -math.inf, dtype=torch.float64, device=dev)
     d = torch.zeros(Hq, T, dtype=torch.float64, device=dev)
-    kd, vd, qd = k.to(dev), v.to(dev), q.to(dev).double()
+    kd, vd, qd = k.to(dev).float(), v.to(dev).float(), q.to(dev).double()
+    if ks is not None:
+        kd = kd.double() * ks.to(dev).double().view(1, 1, Hkv, 1)
+        vd = vd.double() * vs.to(dev).double().view(1, 1, Hkv, 1)
     for b, L in enumerate(lens.tolist()):
         x0, x1 = int(cu[b]), int(cu[b + 1])
         if not L or x0 == x1:
@@ -269,3 +272,66 @@ def test_an_expired_wait_is_reported_and_leaves_the_context_usable(cuda_device, 
     monkeypatch.delenv("PGQA_DEBUG_STUCK_BARRIER")
     monkeypatch.delenv("PGQA_WAIT_LIMIT_NS")
     run_and_check(case, cuda_device)
+
+
+@pytest.mark.parametrize("Hq,Hkv,P", [(32, 8, 16), (28, 4, 64), (6, 2, 256), (16, 16, 48)])
+def test_e4m3_pages(Hq, Hkv, P, cuda_device):
+    """e4m3 K and V are exact in bf16 and their scales multiply in fp32: the bounds of bf16
+    pages, with one more fp32 rounding of the score's factor (2^-23 of the largest score)."""
+    dev = cuda_device
+    for new, lens in (([40, 0, 1, 150, 7, 300, 0], [700, 30, 0, 129, 1300, 256, 5]), ([2], [20000]),
+                      ([65, 64, 1], [1, 16, 17]), ([33] * 12, [64 * i + 1 for i in range(12)])):
+        q, k, v, bt, lens, cu = make(new, lens, Hq, Hkv, P, seed=Hq + len(new), std=4.0, kv="e4m3")
+        g = torch.Generator().manual_seed(1)
+        ks, vs = (torch.rand(Hkv, generator=g) * 0.2 + 0.15 for _ in range(2))
+        a = [x.to(dev) for x in (q, k, v, bt, lens)]
+        out, lse = pgqa.cross_attention(*a, cu_seqlens_q=cu.to(dev), k_scale=ks.to(dev), v_scale=vs.to(dev),
+                                        return_lse=True)
+        pgqa.check_device_error()
+        check(out, lse, reference(q, k, v, bt, lens, cu, 1 / math.sqrt(128), dev, ks, vs))
+    plain = pgqa.cross_attention(*a, cu_seqlens_q=cu.to(dev))
+    one = torch.ones(Hkv)
+    check(plain, None, reference(q, k, v, bt, lens, cu, 1 / math.sqrt(128), dev, one, one))
+    # a scale of zero gives every key the same weight, one below zero turns the scores around
+    ks = torch.tensor([0.0, -0.2] * (Hkv // 2))
+    out, lse = pgqa.cross_attention(*a, cu_seqlens_q=cu.to(dev), k_scale=ks.to(dev), v_scale=-0.3, return_lse=True)
+    check(out, lse, reference(q, k, v, bt, lens, cu, 1 / math.sqrt(128), dev, ks, torch.full((Hkv,), -0.3)))
+    with pytest.raises(ValueError):
+        pgqa.cross_attention(a[0], a[1].to(torch.bfloat16), a[2].to(torch.bfloat16), *a[3:], cu_seqlens_q=cu.to(dev),
+                             k_scale=1.0)
+
+
+def test_e4m3_every_value(cuda_device):
+    """One key: the output is its V, exactly, for all 256 codes (a NaN stays one and stays in
+    its place); a NaN in K makes its row's result NaN."""
+    dev = cuda_device
+    codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).view(2, 1, 1, 128)
+    k = torch.zeros(2, 16, 2, 128).to(torch.float8_e4m3fn)
+    v = torch.full((2, 16, 2, 128), float("nan")).to(torch.float8_e4m3fn)
+    v.view(torch.uint8)[:, :1] = codes.view(torch.uint8)
+    bt = torch.tensor([[0], [1], [0]], dtype=torch.int32)
+    lens = torch.ones(3, dtype=torch.int32)
+    k.view(torch.uint8)[1, 0, 1, 77] = 0x7F
+    q = torch.randn(6, 4, 128).to(torch.bfloat16)
+    out = pgqa.cross_attention(*[x.to(dev) for x in (q.view(3, 2, 4, 128), k, v, bt, lens)]).cpu()
+    want = codes.float().view(2, 128)
+    for b, page in enumerate((0, 1, 0)):
+        w = want[page].expand(2, 2, 128)
+        assert torch.equal(torch.nan_to_num(out[b, :, :2].float(), 1e9), torch.nan_to_num(w, 1e9))
+        assert out[b, :, 2:].isnan().all() if page else torch.equal(
+            torch.nan_to_num(out[b, :, 2:].float(), 1e9), torch.nan_to_num(w, 1e9))
+
+
+def test_e4m3_expired_wait(cuda_device, monkeypatch):
+    case = make([70, 9], [900, 333], 8, 2, 16, seed=30, kv="e4m3")
+    args = [x.to(cuda_device) for x in case]
+    want = pgqa.cross_attention(*args[:5], cu_seqlens_q=args[5])
+    monkeypatch.setenv("PGQA_DEBUG_STUCK_BARRIER", "1")
+    monkeypatch.setenv("PGQA_WAIT_LIMIT_NS", "3000000")
+    pgqa.cross_attention(*args[:5], cu_seqlens_q=args[5])
+    with pytest.raises(PgqaError) as e:
+        pgqa.check_device_error()
+    assert e.value.status == 8
+    monkeypatch.delenv("PGQA_DEBUG_STUCK_BARRIER")
+    monkeypatch.delenv("PGQA_WAIT_LIMIT_NS")
+    assert torch.equal(pgqa.cross_attention(*args[:5], cu_seqlens_q=args[5]), want)

@@ -170,6 +170,7 @@ def cross(**kw):
     (2, dict(scale=-1.0)), (2, dict(scale=float("nan"))), (2, dict(q_stride=1016)), (4, dict(q_stride=1028)),
     (4, dict(q=A + 8)), (4, dict(out=A + 8)), (4, dict(workspace=A + 128)), (4, dict(softmax_lse=A + 2)),
     (3, dict(q_stride=1 << 39)), (2, dict(batch_size=0)),
+    (3, dict(kv_format=2)), (2, dict(k_scale=A)), (4, dict(kv_format=1, v_scale=A + 2)),
 ])
 def test_cross_attention(status, kw):
     assert cross(**kw) == status
@@ -189,7 +190,8 @@ def test_cross_attention_refuses_bad_tensors(cuda_device):
     i32 = torch.int32
     k, bt, lens, q = z(4, 16, 2, 128), z(2, 2, dtype=i32), z(2, dtype=i32), z(2, 3, 8, 128)
     for error, args, kw in (
-            (NotImplementedError, (q, *[k.to(torch.float8_e4m3fn)] * 2), {}), (TypeError, (q.float(), k, k), {}),
+            (ValueError, (q, k, k), dict(v_scale=1.0)), (TypeError, (q, k.to(torch.float8_e4m3fn), k), {}),
+            (TypeError, (q.float(), k, k), {}),
             (ValueError, (q.cpu(), k, k), {}), (ValueError, (z(2, 4, 8, 128)[:, :3], k, k), {}),
             (ValueError, (z(2, 3, 128, 8).transpose(2, 3), k, k), {}),
             (ValueError, (z(2, 3, 16, 128)[:, :, ::2], k, k), {}),
