@@ -9,8 +9,8 @@ attention of prompt tokens over an encoder's states.
     out = cross_attention(q, enc_k, enc_v, enc_table, enc_lens, cu_seqlens_q=cu)
 
 `weights` is a float32 pool [num_pages, Hkv, P] beside the K and V pools.  Every call runs
-on torch's current stream of the tensors' device, allocates nothing but its outputs and can
-be captured into a CUDA graph after one eager call.  Errors that only the device sees (a
+on torch's current stream of the tensors' device, allocates its outputs (cross_attention: and
+a workspace) by torch and can be captured into a CUDA graph after one eager call.  Errors that only the device sees (a
 page id, length or position out of range) are read with `check_device_error()`.
 """
 import functools
@@ -84,7 +84,10 @@ def _scales(x, Hkv, dev):
     if torch.is_tensor(x) and x.dtype is _F32 and x.get_device() == dev and x.shape == (Hkv,) \
             and x.is_contiguous():
         return x
-    return _scale_array(x, Hkv, torch.device("cuda", dev))
+    at = torch.device("cuda", dev)
+    if x is not None and not torch.is_tensor(x):  # filled on the device: a copy from the host cannot be captured
+        return torch.full((Hkv,), float(x), dtype=_F32, device=at)
+    return _scale_array(x, Hkv, at)
 
 
 def _call(fn, args, dev, what):

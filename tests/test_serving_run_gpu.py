@@ -158,3 +158,40 @@ def test_flash_attn_rotary_arguments(cuda_device):
         ref = paged_decode_ref(qt.to(torch.bfloat16).reshape(q.shape), got_k, got_v, bt, seq + S, causal=causal)
         assert_parity(out, ref, edge=True, what=f"causal={causal} Sq={Sq} S={S}")
     pgqa.check_device_error()
+
+
+def test_captured_with_scalar_scales(cuda_device):
+    """e4m3 pages with one number as the scale of all heads: the calls can be captured, and the
+    replay equals the eager calls."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(3)
+    lens = [20, 33]
+    bt, pages = _paged.table([n + 1 for n in lens], P, g)
+    pools = [_paged.pool(pages, P, Hkv, g, "e4m3").to(dev) for _ in range(2)]
+    cos, sin = (x.to(dev) for x in tables(64, 128))
+    btd, before = bt.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev)
+    after = before + 1
+    x = torch.randn(2, Hq + 2 * Hkv, 128, generator=g).to(torch.bfloat16).to(dev)
+
+    def step(k, v, w):
+        q = pgqa.rope_append_kv(x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], k, v, btd, before, cos, sin, weights=w,
+                                k_scale=0.5, v_scale=0.25)
+        out, lse = pgqa.cross_attention(q.unsqueeze(1), k, v, btd, after, k_scale=0.5, v_scale=0.25, return_lse=True)
+        pgqa.accumulate_weights(q, k, btd, after, lse, w, k_scale=0.5)
+        return out
+
+    eager = [p.clone() for p in pools] + [torch.zeros(pages, Hkv, P, device=dev)]
+    want = step(*eager)
+    # one query token per sequence: the weights that each KV head's tokens received sum up to its rows
+    w = eager[2].cpu()
+    sums = torch.stack([w[bt[b, :-(-(n + 1) // P)].long()].sum((0, 2)) for b, n in enumerate(lens)])
+    assert torch.allclose(sums, torch.full_like(sums, Hq / Hkv), rtol=1e-4)
+    state = [p.clone() for p in pools] + [torch.zeros(pages, Hkv, P, device=dev)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*state)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(state[2], eager[2])
+    assert all(torch.equal(_paged.raw(a), _paged.raw(b)) for a, b in zip(state, eager))
+    pgqa.check_device_error()
