@@ -81,8 +81,9 @@ struct Geo {
 };
 constexpr int kRows = 2 * kTile;           // rows of a work item
 // What an item costs beside its key tiles, in key tiles (1 to 4 measured: 175, 159, 167, 166 us
-// for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys), and the least length of a slice.
-constexpr int kItemCost = 2, kMinSlice = 3;
+// for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys), and the least length of a slice
+// (1, 2 and 3: 17.7, 14.0, 16.7 us for 10 + 13 tokens over 1024 keys, 32 + 8 heads).
+constexpr int kItemCost = 2, kMinSlice = 2;
 constexpr int kSnap = 24;
 constexpr float kLazyLog2 = 8.f;
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
@@ -102,7 +103,7 @@ struct Params {
     int32_t grid;            // CTAs of the first launch
     float scale_log2;
     uint64_t wait_limit_ns;
-    int32_t debug_stuck;     // test hook: > 0 makes CTA 0's first load expect 16 bytes too many
+    int32_t debug_stuck;     // test hook: > 0 makes every CTA's first load expect 16 bytes too many
 };
 
 __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -492,7 +493,7 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     const bool tail = !KV8 && kv == 1 && (nvalid & 15) != 0;
                     const uint32_t bar = KV8 ? RFULL(slot) : (tail ? TAIL : FULL(slot));
                     if (lane == 0) {
-                        const bool stuck = p.debug_stuck > 0 && blockIdx.x == 0 && n_kv == 0;
+                        const bool stuck = p.debug_stuck > 0 && n_kv == 0;
                         ptx::mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * (KV8 ? 128 : 256)) + (stuck ? 16u : 0u));
                     }
                     __syncwarp();
@@ -872,8 +873,8 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 
 /* Joins the parts of cut items: out = sum_s 2^(l_s - l) O_s with 2^l = sum_s 2^(l_s); a
  * part without weight has l_s = -inf and no O.  Block (j, y): 32 rows of the item that slice
- * j + 1 cuts first, each thread 16 dimensions of one. */
-constexpr int kJoinThreads = 256;
+ * j + 1 cuts first, each thread 16 dimensions of one, with the maximum moved as the parts come. */
+constexpr int kJoinThreads = 256, kParts = 2;
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
@@ -888,25 +889,46 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     const int32_t tok = tok0 + w * p.tile_tokens + t, head = kvh * p.g + (row - t * p.g);
     if (t >= p.tile_tokens || tok >= tok_end) return;
     auto rec_of = [&](int32_t c) { return (int64_t)(2 * c + (c == j ? 1 : 0)) * kRows + r; };
-    float m = -INFINITY;
-    for (int32_t c = j; c <= last; ++c) m = fmaxf(m, __ldcg(p.rec_lse + rec_of(c)));
-    const float base = m == -INFINITY ? 0.f : m;
-    float sum = 0.f, acc[16];
+    float m = -INFINITY, sum = 0.f, acc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    for (int32_t c = j; c <= last; ++c) {
-        const float l2 = __ldcg(p.rec_lse + rec_of(c));
-        if (l2 == -INFINITY) continue;
-        const float wgt = exp2f(l2 - base);  // NaN parts reach the result through their weight
-        sum += wgt;
-        const float4* src = reinterpret_cast<const float4*>(p.rec_o + rec_of(c) * 128 + d);
+    // kParts parts in flight, with their log-sum-exps: one token over 8000 keys, 8 + 1 heads,
+    // 27 -> 19 us; with four in flight the registers cost more where whole tiles are joined (ragged
+    // prompts: 169 instead of 163 us)
+#pragma unroll 1
+    for (int32_t c0 = j; c0 <= last; c0 += kParts) {
+        float l2[kParts], top = m;
+        float4 o[kParts][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 o = __ldcg(src + i);
-            acc[4 * i] = fmaf(wgt, o.x, acc[4 * i]);
-            acc[4 * i + 1] = fmaf(wgt, o.y, acc[4 * i + 1]);
-            acc[4 * i + 2] = fmaf(wgt, o.z, acc[4 * i + 2]);
-            acc[4 * i + 3] = fmaf(wgt, o.w, acc[4 * i + 3]);
+        for (int u = 0; u < kParts; ++u) {
+            const int64_t rec = rec_of(min(c0 + u, last));
+            l2[u] = __ldcg(p.rec_lse + rec);
+            const float4* src = reinterpret_cast<const float4*>(p.rec_o + rec * 128 + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[u][i] = __ldcg(src + i);
+        }
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {
+            if (c0 + u > last) l2[u] = -INFINITY;
+            top = fmaxf(top, l2[u]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, alpha = exp2f(m - base);
+        m = top;
+        sum *= alpha;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] *= alpha;
+#pragma unroll
+        for (int u = 0; u < kParts; ++u) {
+            if (l2[u] == -INFINITY) continue;        // whose O was not written
+            const float wgt = exp2f(l2[u] - base);   // NaN parts reach the result through their weight
+            sum += wgt;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[4 * i] = fmaf(wgt, o[u][i].x, acc[4 * i]);
+                acc[4 * i + 1] = fmaf(wgt, o[u][i].y, acc[4 * i + 1]);
+                acc[4 * i + 2] = fmaf(wgt, o[u][i].z, acc[4 * i + 2]);
+                acc[4 * i + 3] = fmaf(wgt, o[u][i].w, acc[4 * i + 3]);
+            }
         }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
