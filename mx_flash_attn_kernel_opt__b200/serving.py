@@ -100,22 +100,25 @@ def _call(fn, args, dev, what):
     check(st, what)
 
 
-def _rows(what, name, x, lead, D, dev, step):
-    """Checks q / k_new / v_new [*lead, heads, D] (a head's elements contiguous, any other
-    strides); returns (address, heads, element strides of sequence, token, head).  step: the
-    one leading dimension counts sequences rather than tokens."""
+def _rows(what, name, x, want, dev, step):
+    """Checks q / k_new / v_new of shape `want` [..., heads, D] (a head's elements contiguous,
+    any other strides); returns (address, element strides of sequence, token, head).  step:
+    the one leading dimension counts sequences rather than tokens."""
     if x.dtype is not _BF16:
         raise TypeError(f"{what}: {name} must be {_BF16}, got {x.dtype}")
     if x.get_device() != dev:
         raise ValueError(f"{what}: {name} must be on cuda:{dev}, got {x.device}")
-    n = len(lead)
-    shape, s = x.shape, x.stride()
-    if len(shape) != n + 2 or shape[:n] != lead or shape[-1] != D:
-        raise PgqaError(2, f"{what}: {name} must be [{', '.join(map(str, lead))}, heads, {D}]")
+    if x.shape != want:
+        raise PgqaError(2, f"{what}: {name} must be {list(want)}, got {list(x.shape)}")
+    s = x.stride()
     if s[-1] != 1:
         raise ValueError(f"{what}: the elements of a head of {name} must be contiguous")
-    s = (s[0], s[1], s[2]) if n == 2 else ((s[0], 0, s[1]) if step else (0, s[0], s[1]))
-    return x.data_ptr(), shape[-2], s
+    return x.data_ptr(), s[:3] if len(s) == 4 else ((s[0], 0, s[1]) if step else (0, s[0], s[1]))
+
+
+def _like(x):
+    """An uninitialised contiguous tensor of x's shape and type."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _turn(what, q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos, sin, positions,
@@ -172,14 +175,14 @@ def _turn(what, q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos, s
     qs = kst = vst = none
     Hq = 0
     if k_new is not None:
-        knp, hk, kst = _rows(what, "k_new", k_new, lead, D, dev, step)
-        vnp, hv, vst = _rows(what, "v_new", v_new, lead, D, dev, step)
-        if hk != Hkv or hv != Hkv:
-            raise PgqaError(2, f"{what}: k_new / v_new must have the pools' {Hkv} heads")
+        want = (*lead, Hkv, D)
+        knp, kst = _rows(what, "k_new", k_new, want, dev, step)
+        vnp, vst = _rows(what, "v_new", v_new, want, dev, step)
     if q is not None:
-        qp, Hq, qs = _rows(what, "q", q, lead, D, dev, step)
+        Hq = full[-2]
+        qp, qs = _rows(what, "q", q, (*lead, Hq, D), dev, step)
         if q_out is None:
-            q_out = q.new_empty(full)
+            q_out = _like(q)
             qo = q_out.data_ptr()
         else:
             qo = _ptr(what, "q_out", q_out, _BF16, dev)
@@ -367,7 +370,7 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     if tokens <= 1:
         stride = Hq * D
     if out is None:
-        out = q.new_empty(qs)
+        out = _like(q)
         op = out.data_ptr()
     else:
         op = _ptr(what, "out", out, _BF16, dev)
