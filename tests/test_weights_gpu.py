@@ -153,3 +153,25 @@ def test_more_rows_than_one_turn_takes(kv, cuda_device):
     """g * Sq of 66 and of 35: several turns over a warp's chunks, the last one partly empty."""
     run_and_check(make([50, 3, 0], 22, 2, 16, 6, kv, True, seed=20), True, cuda_device)
     run_and_check(make([90], 5, 1, 32, 7, kv, False, seed=21), False, cuda_device)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("Hq,Sq", [(16, 4), (32, 4), (4, 8)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_whole_groups_of_rows_over_long_sequences(kv, Hq, Sq, causal, cuda_device):
+    """32, 64 and 16 rows per KV head without a padding row: chunks that every row sees, the
+    causal border and the ragged end are in one call."""
+    run_and_check(make([700, 33, 257, 16], Hq, 2, 16, Sq, kv, causal, seed=30 + Hq), causal, cuda_device)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_one_row_that_saw_nothing_among_many(kv, cuda_device):
+    """A log-sum-exp of -inf in a whole group of rows: that row adds nothing, the others theirs."""
+    q, k, bt, lens, lse, w, scale, ks = make([320, 40], 16, 2, 16, 4, kv, False, seed=41)
+    lse[0, 5, 2] = -math.inf
+    ref, bound = weights_ref(q, k, bt, lens, lse, w, scale, False, ks)
+    dev = cuda_device
+    wd = w.to(dev)
+    pgqa.accumulate_weights(q.to(dev), k.to(dev), bt.to(dev), lens.to(dev), lse.to(dev), wd, scale=scale,
+                            k_scale=None if ks is None else ks.to(dev))
+    assert ((wd.cpu().double() - ref).abs() <= bound).all()
