@@ -373,7 +373,7 @@ int pgqa_evict(const pgqa_evict_args* args, void* stream);
  * (and a log-sum-exp of -inf).  q and out bf16, fp32 scores, sums and accumulators.
  *   q            [tokens, Hq, 128], token stride q_stride elements (a multiple of 8, at
  *                least Hq * 128), heads contiguous
- *   out          [tokens, Hq, 128], contiguous
+ *   out          [tokens, Hq, 128], contiguous, 16-byte aligned
  *   cu_seqlens   NULL: [batch_size, seqlen_q] tokens, tokens = batch_size * seqlen_q.
  *                Else int32 [batch_size + 1], ascending from 0; rows of out and softmax_lse
  *                from cu[batch_size] on are left as they are

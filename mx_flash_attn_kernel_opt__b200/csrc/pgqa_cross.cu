@@ -104,6 +104,7 @@ struct Params {
     float scale_log2;
     uint64_t wait_limit_ns;
     int32_t debug_stuck;     // test hook: > 0 makes every CTA's first load expect 16 bytes too many
+    int32_t out_32;          // out is 32-byte aligned (torch gives a view any multiple of its element)
 };
 
 __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -332,11 +333,17 @@ __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t b, uint32_t& lo, uint32_
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(my), "r"(0x7b807b80u));
 }
 
-/* 32 bytes to global memory in one instruction. */
+/* 32 bytes to global memory in one instruction; the address must be a multiple of 32. */
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
+}
+/* The same in two instructions, for a multiple of 16. */
+__device__ __forceinline__ void st_global_16x2(void* p, const uint32_t (&v)[8]) {
+    uint4* d = static_cast<uint4*>(p);
+    d[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    d[1] = make_uint4(v[4], v[5], v[6], v[7]);
 }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
@@ -840,7 +847,8 @@ cross_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         for (int e = 0; e < 8; ++e)
                             h[e] = l == 0.f ? 0u : ptx::pack_bf16x2(__uint_as_float(o[16 * i + 2 * e]) * inv,
                                                                     __uint_as_float(o[16 * i + 2 * e + 1]) * inv);
-                        st_global_32(dst + 16 * i, h);
+                        if (p.out_32) st_global_32(dst + 16 * i, h);
+                        else st_global_16x2(dst + 16 * i, h);
                     }
                 } else if (l != 0.f) {
                     float* dst = p.rec_o + rec * 128 + 32 * c;
@@ -1035,6 +1043,7 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     p.rec_lse = p.rec_o + (size_t)2 * p.grid * kRows * 128;
     p.cuts = reinterpret_cast<Cut*>(p.rec_lse + (size_t)2 * p.grid * kRows);
     p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.out_32 = host_aligned(a->out, 32);
     p.lse = a->softmax_lse;
     p.seq_lens = a->seq_lens;
     p.block_table = a->block_table;

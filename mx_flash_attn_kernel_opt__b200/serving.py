@@ -330,8 +330,9 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     float8_e4m3fn (an element of KV head h is worth e4m3 * k_scale[h], v_scale for V),
     block_table [B, width] int32, seq_lens [B] int32 (0: the sequence's rows are zeros).
 
-    Returns out (contiguous, q's shape) or (out, lse) with `return_lse`: fp32 [Hq, tokens]
-    for packed q, else [B, Hq, Sq]; -inf where a row sees no key.  Rows of packed tokens
+    Returns out (contiguous, q's shape; 16-byte aligned, as every tensor of 16-bit or 8-bit
+    elements here) or (out, lse) with `return_lse`: fp32 [Hq, tokens] for packed q, else
+    [B, Hq, Sq]; -inf where a row sees no key.  Rows of packed tokens
     behind the last sequence are left as they are in `out`."""
     what = "cross_attention"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
