@@ -242,7 +242,8 @@ int pgqa_noalloc_check_device_error(void* stream);
  * Operators around the decode (no counterpart in the reference).  They allocate nothing
  * and keep nothing between calls, may be captured into a CUDA graph after one eager call
  * on the device, and may run on several streams at once as long as the calls' outputs and
- * pages differ.  Their device-side errors go to one word per device, which
+ * pages differ.  What a call reads (lengths, tables, cu_seqlens among it) must not be written
+ * while it runs, but by the call itself where that is said.  Their device-side errors go to one word per device, which
  * pgqa_check_device_error(NULL, stream) reads and clears.
  */
 

@@ -104,6 +104,7 @@ struct Params {
     float scale_log2;
     uint64_t wait_limit_ns;
     int32_t debug_stuck;     // test hook: > 0 makes every CTA's first load expect 16 bytes too many
+    int32_t debug_long;      // test hook: key tiles that the last slice believes to have too many
     int32_t out_32;          // out is 32-byte aligned (torch gives a view any multiple of its element)
 };
 
@@ -181,6 +182,12 @@ __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
         if (lane >= o) incl += v;
     }
     if (lane == 31) wsum[warp] = incl;
+    if (tid == 0) {  // an empty slice, should no sequence below be found to hold its start
+        out.lo = INT64_MAX;
+        out.hi = out.base = out.item_lo = 0;
+        out.item_len = 1;
+        out.b = 0;
+    }
     __syncthreads();
     int64_t run = incl - local, total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
@@ -225,7 +232,10 @@ struct Item {
     bool cut;                                  // other CTAs have tiles of it too
 };
 
-/* Walks a slice's items; called by whole warps, every role with a copy of its own. */
+/* Walks a slice's items; called by whole warps, every role with a copy of its own.  Lengths are
+ * read again on the way: should they have changed since the slice was cut (or the slice be
+ * longer than what there is), the walk ends with the error word set.  It never passes the
+ * last sequence, and every item it gives lies within the tensors. */
 struct Walker {
     int64_t left;             // of the slice
     int32_t b, kvh, pair, off;  // the next item, and where in it the slice goes on
@@ -239,8 +249,13 @@ struct Walker {
         cur.pairs = __shfl_sync(0xffffffffu, mine.pairs, cur_lane);
         cur.items = __shfl_sync(0xffffffffu, mine.items, cur_lane);
     }
+    __device__ void stop(const Params& p, int lane) {
+        left = 0;
+        if (lane == 0) atomicOr(p.err, kDevErrBadSeqlen);
+    }
     __device__ void init(const Params& p, const Slice& s, int lane) {
         left = s.hi - s.lo;
+        if (left > 0 && s.hi == s.total) left += p.debug_long;
         b = s.b;
         cur_lane = 0;
         kvh = pair = off = 0;
@@ -248,6 +263,10 @@ struct Walker {
             mine = load_seq(p, b + lane, false);
             pick();
             const int64_t in = s.lo - s.base;  // a cut moved to the sequence's end: kvh = Hkv
+            if (cur.items == 0 || in > cur.size()) {
+                stop(p, lane);
+                return;
+            }
             const int32_t unit = (int32_t)(in / cur.len());
             off = (int32_t)(in - (int64_t)unit * cur.len());
             kvh = unit / cur.pairs;
@@ -269,6 +288,10 @@ struct Walker {
             while (some == 0) {
                 b += 32 - from;
                 from = 0;
+                if (b >= p.B) {
+                    stop(p, lane);
+                    return false;
+                }
                 mine = load_seq(p, b + lane, false);
                 some = __ballot_sync(0xffffffffu, mine.items > 0);
             }
@@ -283,7 +306,7 @@ struct Walker {
         it.L = cur.L;
         it.t0 = max(0, off - kItemCost);
         const bool ends = left >= cur.len() - off;
-        it.t1 = ends ? cur.n : off + (int32_t)left - kItemCost;
+        it.t1 = ends ? cur.n : max(it.t0, off + (int32_t)left - kItemCost);
         it.cut = off > 0 || !ends;
         left -= ends ? cur.len() - off : (int32_t)left;
         off = 0;
@@ -310,6 +333,7 @@ __device__ Cut cut_of(const Params& p, int32_t c, const Slice& s) {
     if (off > 0 && snapped(off, s.item_len, tol) == s.item_len) --last;
     const Seq q = load_seq(p, s.b, false);
     const int32_t unit = (int32_t)((s.item_lo - s.base) / s.item_len);
+    if (unit >= q.items) return k;  // the lengths have changed; the walk reports it
     k.is = 1;
     k.last = last;
     k.b = s.b;
@@ -1068,6 +1092,8 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     if (p.wait_limit_ns == 0 || p.wait_limit_ns > 10 * kWaitLimitNs) p.wait_limit_ns = kWaitLimitNs;
     const char* stuck = getenv("PGQA_DEBUG_STUCK_BARRIER");
     p.debug_stuck = (stuck && *stuck) ? atoi(stuck) : 0;
+    const char* longer = getenv("PGQA_DEBUG_LONG_SLICE");
+    p.debug_long = (longer && *longer) ? atoi(longer) : 0;
     CUtensorMap qm, km, vm;
     const int64_t slots = a->num_pages * a->page_size;
     const int64_t row = kv8 ? 128 : 256;
