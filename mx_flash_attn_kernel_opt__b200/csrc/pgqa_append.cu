@@ -44,14 +44,14 @@ append_kv_kernel(const AppendArgs a) {
         const int64_t bs = row / a.Hkv;
         const int32_t s = (int32_t)(bs % a.S_new);
         const int32_t b = (int32_t)(bs / a.S_new);
-        const int32_t L0 = __ldg(a.seq_lens + b);
+        const int32_t L0 = ptx::ld(a.seq_lens + b);
         const int64_t t = (int64_t)L0 + s;
         if (L0 < 0 || t >= a.cap_tokens) { bad |= kAppendBadSeqlen; continue; }
-        const int32_t pid = __ldg(a.block_table + (int64_t)b * a.bt_stride + t / a.P);
+        const int32_t pid = ptx::ld(a.block_table + (int64_t)b * a.bt_stride + t / a.P);
         if (pid < 0 || pid >= a.num_pages) { bad |= kAppendBadPage; continue; }
         const int64_t dst = ((((int64_t)pid * a.P + t % a.P) * a.Hkv + kvh) << sh) + piece;
-        const uint4 kv = __ldg(a.k_new + x);
-        const uint4 vv = __ldg(a.v_new + x);
+        const uint4 kv = ptx::ld(a.k_new + x);
+        const uint4 vv = ptx::ld(a.v_new + x);
         a.k_cache[dst] = kv;
         a.v_cache[dst] = vv;
     }

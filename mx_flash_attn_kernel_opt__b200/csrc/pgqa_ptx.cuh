@@ -162,6 +162,35 @@ __device__ __forceinline__ void griddep_launch_dependents() {
  * (ld.global.nc), whose data may not change while the kernel runs. */
 template <typename T>
 __device__ __forceinline__ T ld(const T* p) { return *p; }
+/* The same where the compiler should stay free to move the load past other memory operations
+ * (TMA issues, barriers), as it is with the read-only path: tie() after griddepcontrol.wait
+ * gives the address a value that exists only from there on, so a load from it cannot move in
+ * front of the wait.  Only for memory that this kernel does not write. */
+template <typename T>
+__device__ __forceinline__ const T* tie(const T* p) {
+    asm volatile("" : "+l"(p) : : "memory");
+    return p;
+}
+__device__ __forceinline__ uint32_t ld_tied(const uint32_t* p) {
+    uint32_t v;
+    asm("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int32_t ld_tied(const int32_t* p) {
+    int32_t v;
+    asm("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float ld_tied(const float* p) {
+    float v;
+    asm("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ld_tied(const uint2* p) {
+    uint2 v;
+    asm("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
 
 /* Explicit shared-memory accesses by 32-bit shared-window address. */
 __device__ __forceinline__ float4 lds_f4(uint32_t addr) {

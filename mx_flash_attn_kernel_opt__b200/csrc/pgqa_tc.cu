@@ -124,7 +124,7 @@ struct Walker {
             const int64_t r = cs - (int64_t)pre[b] * p.Hkv;
             j = (r <= kSmallProduct) ? (int32_t)((uint32_t)r / (uint32_t)n) : (int32_t)(r / n);
             c = (int32_t)(r - (int64_t)j * n);
-            L = clamp_len((int64_t)__ldg(p.seq_lens + b) + p.len_add, p.cap_tokens);
+            L = clamp_len((int64_t)ptx::ld(p.seq_lens + b) + p.len_add, p.cap_tokens);
         }
     }
     __device__ bool next(const TcParams& p, Tile& t) {
@@ -144,7 +144,7 @@ struct Walker {
                 j = 0;
                 do { ++b; } while (pre[b + 1] == pre[b]);
                 n = (int32_t)(pre[b + 1] - pre[b]);
-                L = clamp_len((int64_t)__ldg(p.seq_lens + b) + p.len_add, p.cap_tokens);
+                L = clamp_len((int64_t)ptx::ld(p.seq_lens + b) + p.len_add, p.cap_tokens);
             }
         }
         return true;
@@ -347,7 +347,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
         int32_t bad = 0;
         uint32_t local = 0, cmin = 0xffffffffu, cmax = 0;
         for (int b = s0; b < s1; ++b) {
-            const int32_t L0 = __ldg(p.seq_lens + b);
+            const int32_t L0 = ptx::ld(p.seq_lens + b);
             const int64_t Lk = (int64_t)L0 + p.len_add;
             if (L0 < 0 || Lk > p.cap_tokens) bad = 1;
             const uint32_t nb = (uint32_t)seq_chunks(Lk, p.cap_tokens);
@@ -375,7 +375,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
         if (tid == kThreads - 1) pre[p.B] = run + local;
         for (int b = s0; b < s1; ++b) {
             pre[b] = run;
-            run += (uint32_t)seq_chunks((int64_t)__ldg(p.seq_lens + b) + p.len_add, p.cap_tokens);
+            run += (uint32_t)seq_chunks((int64_t)ptx::ld(p.seq_lens + b) + p.len_add, p.cap_tokens);
         }
         if (bad && blockIdx.x == 0) atomicOr(p.err, kErrBadSeqlen);
         __syncthreads();
@@ -443,7 +443,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 // ceil(L / P) = ceil(16 n / P) (P a multiple of 16): no wait for the length
                 const int32_t npg = page_of(t.n * kChunkTokens + P - 1);
                 const int32_t pg = page0 + lane;
-                win_pid = (pg < npg) ? __ldg(p.block_table + (int64_t)t.b * p.bt_stride + pg) : 0;
+                win_pid = (pg < npg) ? ptx::ld(p.block_table + (int64_t)t.b * p.bt_stride + pg) : 0;
             }
             const int k = lane < t.nc ? lane : 0;
             const int32_t tok = (t.c0 + k) * kChunkTokens;
@@ -643,7 +643,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                     const uint4* src = valid ? reinterpret_cast<const uint4*>(p.q + row_offset<MQ>(p, t.b, t.kvh, r)) : nullptr;
 #pragma unroll
                     for (int kc = 0; kc < 16; ++kc) {
-                        const uint4 v = valid ? __ldg(src + kc) : make_uint4(0, 0, 0, 0);
+                        const uint4 v = valid ? ptx::ld(src + kc) : make_uint4(0, 0, 0, 0);
                         ptx::sts_u4(qs + (uint32_t)(kc * NP + r) * 16u, v);
                     }
                 } else {
@@ -652,7 +652,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                         const uint4* src = reinterpret_cast<const uint4*>(p.q + row_offset<MQ>(p, t.b, t.kvh, r));
 #pragma unroll
                         for (int kc = 0; kc < 16; ++kc) {
-                            const uint4 v = __ldg(src + kc);
+                            const uint4 v = ptx::ld(src + kc);
                             const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -672,7 +672,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                     if (mx > 0.f) e = 7 - ((int)((__float_as_uint(mx) >> 23) & 0xff) - 127);
                     e = max(-100, min(100, e));
                     const float up = exp2f((float)e);
-                    const float ks = (p.k_scale != nullptr) ? __ldg(p.k_scale + t.kvh) : 1.f;
+                    const float ks = (p.k_scale != nullptr) ? ptx::ld(p.k_scale + t.kvh) : 1.f;
                     mul = p.scale_log2 * ks * exp2f((float)-e);
 #pragma unroll
                     for (int kc = 0; kc < 8; ++kc) {  // 16 dims per 16-byte row of a core matrix
@@ -998,7 +998,7 @@ pgqa_tc_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
                 if (lane == 0) ptx::mbar_arrive(QFREE(qb));
 #pragma unroll
                 for (int r = 0; r < NP; ++r) { m_ref[r] = -INFINITY; l_part[r] = 0.f; }
-                if (KV8) vsc = (p.v_scale != nullptr) ? __ldg(p.v_scale + t.kvh) : 1.f;
+                if (KV8) vsc = (p.v_scale != nullptr) ? ptx::ld(p.v_scale + t.kvh) : 1.f;
                 causal_base = t.L - p.Sq + 1;
                 piece_c0 = t.c0;
             }

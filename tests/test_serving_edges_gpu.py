@@ -6,7 +6,7 @@ import torch
 
 import mx_flash_attn_kernel_opt__b200 as pgqa
 from mx_flash_attn_kernel_opt__b200 import PgqaError
-from tests import test_cross_gpu
+from tests import _paged, test_cross_gpu, test_rope_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -56,4 +56,49 @@ def test_cross_slice_longer_than_its_items_ends(new, lens, kv, cuda_device, monk
     monkeypatch.delenv("PGQA_DEBUG_LONG_SLICE")
     monkeypatch.delenv("PGQA_WAIT_LIMIT_NS")
     assert torch.equal(pgqa.cross_attention(*a, cu_seqlens_q=cu), want)
+    pgqa.check_device_error()
+
+
+@pytest.mark.parametrize("Sq", [1, 5])
+def test_chains_without_a_stop_between_the_calls(Sq, both_kernels, cuda_device):
+    """rope -> decode -> weights -> evict -> decode and append at the lengths that the eviction
+    wrote, step after step: calls queued without a wait equal calls that wait for each other."""
+    dev, P, Hq, Hkv, B, keep = cuda_device, 16, 32, 4, 6, 900
+    g = torch.Generator().manual_seed(70)
+    cap = 1024
+    bt, pages = _paged.table([cap] * B, P, g)
+    k, v = (_paged.pool(pages, P, Hkv, g) for _ in range(2))
+    cos, sin = (x.to(dev) for x in test_rope_gpu.tables(2048, 128))
+    bt = bt.to(dev)
+    xs = [torch.randn(B, Sq, Hq + 2 * Hkv, 128, generator=g).to(torch.bfloat16).to(dev) for _ in range(6)]
+    first = torch.tensor([880, 10, 899, 0, 600, 890], dtype=torch.int32, device=dev)
+    more = torch.randn(2, B, 3, Hkv, 128, generator=g).to(torch.bfloat16).to(dev)
+
+    def run(wait):
+        stop = torch.cuda.synchronize if wait else (lambda: None)
+        kd, vd, w, lens, got = k.to(dev), v.to(dev), torch.zeros(pages, Hkv, P, device=dev), first.clone(), []
+        torch.cuda.synchronize()
+        for x in xs:
+            q = pgqa.rope_append_kv(x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:], kd, vd, bt, lens, cos, sin,
+                                    weights=w)
+            stop()
+            full = lens + Sq
+            out, lse = pgqa.decode(q, kd, vd, bt, full, causal=True, return_lse=True)
+            stop()
+            pgqa.accumulate_weights(q, kd, bt, full, lse, w, causal=True)
+            stop()
+            kept, lens = pgqa.evict_kv(kd, vd, w, bt, full, keep, sinks=4, recent=64)
+            stop()
+            again = pgqa.decode(q, kd, vd, bt, lens, causal=True)
+            stop()
+            pgqa.append_kv(more[0], more[1], kd, vd, bt, lens)
+            stop()
+            got += [q, out, lse, kept, lens, again]
+        torch.cuda.synchronize()
+        return got + [kd, vd, w]
+
+    want = run(True)
+    for _ in range(4):
+        for a, b in zip(run(False), want):
+            assert torch.equal(a, b)
     pgqa.check_device_error()
