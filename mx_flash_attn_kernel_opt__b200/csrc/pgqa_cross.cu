@@ -1023,7 +1023,7 @@ size_t workspace_bytes(int grid) { return (size_t)grid * (2 * kRows * (128 + 1) 
 template <bool KV8>
 int launch(const Params& p, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int dev,
            cudaStream_t stream) {
-    static int done[kHostMaxDevices] = {0};
+    static HostSmemDone done;
     using G = Geo<KV8>;
     const int st = host_smem_limit(cross_kernel<KV8>, dev, G::kSmem, done);
     if (st != PGQA_OK) return st;

@@ -591,7 +591,7 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
     p.cluster = 2;
     while (p.cluster < kMaxCluster && items * 2 * p.cluster <= kCtasPerSm * sms && p.cap_tokens / (2 * p.cluster) >= 1024)
         p.cluster *= 2;
-    static int done[kHostMaxDevices] = {0};
+    static HostSmemDone done;
     if ((st = host_smem_limit(evict_kernel, dev, kSmem, done)) != PGQA_OK) return st;
     return host_launch(evict_kernel, dim3((unsigned)(items * p.cluster)), kThreads, kSmem, stream, p.cluster, p);
 }

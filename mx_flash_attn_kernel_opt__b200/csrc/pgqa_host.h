@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/pgqa.h"
 
 namespace pgqa {
@@ -33,18 +35,21 @@ bool host_pdl();
 /* cuTensorMapEncodeTiled, or NULL when the driver does not export it. */
 void* host_encode_tiled();
 
-/* Raises a kernel's dynamic shared-memory limit on device `dev`; `done` is the caller's
- * per-kernel table of limits already set. */
+/* Allows a kernel `bytes` of dynamic shared memory on device `dev`.  `bytes` is the most that
+ * any of its launches takes there, the same in every call, so that neither the order of the
+ * calls nor two threads at once can leave a lower limit behind; `done` is the caller's
+ * per-kernel table of devices already seen to. */
 constexpr int kHostMaxDevices = 64;
+typedef std::atomic<bool> HostSmemDone[kHostMaxDevices];
 template <typename K>
-int host_smem_limit(K kernel, int dev, int bytes, int (&done)[kHostMaxDevices]) {
+int host_smem_limit(K kernel, int dev, int bytes, HostSmemDone& done) {
     if (dev < 0 || dev >= kHostMaxDevices) return PGQA_ERR_NO_DEVICE;
-    if (done[dev] >= bytes) return PGQA_OK;
+    if (done[dev].load(std::memory_order_acquire)) return PGQA_OK;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
         cudaGetLastError();
         return PGQA_ERR_CUDA;
     }
-    done[dev] = bytes;
+    done[dev].store(true, std::memory_order_release);
     return PGQA_OK;
 }
 

@@ -415,12 +415,14 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
 template <bool KV8, int NT>
 int launch(const Params& p, int dev, int sms, int optin, cudaStream_t stream) {
     const int smem = kWarps * warp_smem(NT) + (p.B + 1) * 4;
-    // the chunk counts before each sequence live in shared memory; two CTAs per SM
-    if (smem > optin / 2 - 1024) return PGQA_ERR_UNSUPPORTED;
-    static int done[kHostMaxDevices] = {0};
+    // the chunk counts before each sequence live in shared memory; two CTAs per SM (the static
+    // bytes and the system's fit into the 1024)
+    const int most = optin / 2 - 1024;
+    if (smem > most) return PGQA_ERR_UNSUPPORTED;
+    static HostSmemDone done;
     auto kern = weights_kernel<KV8, NT>;
-    int st = PGQA_OK;
-    if (smem > 48 * 1024 && (st = host_smem_limit(kern, dev, smem, done)) != PGQA_OK) return st;
+    const int st = host_smem_limit(kern, dev, most, done);
+    if (st != PGQA_OK) return st;
     return host_launch(kern, dim3((unsigned)(2 * sms)), kThreads, (size_t)smem, stream, 1, p);
 }
 

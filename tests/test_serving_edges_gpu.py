@@ -1,5 +1,8 @@
 """Calls at the edges of what the operators around the decode take."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -9,6 +12,23 @@ from mx_flash_attn_kernel_opt__b200 import PgqaError
 from tests import _paged, test_cross_gpu, test_rope_gpu
 
 pytestmark = pytest.mark.gpu
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+ONE_BATCH = """
+import sys, torch
+import mx_flash_attn_kernel_opt__b200 as pgqa
+B, Sq = int(sys.argv[1]), int(sys.argv[2])
+z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device="cuda")
+lens = z(B, dtype=torch.int32)
+lens[-1] = 5
+w = z(1, 1, 16)
+q, k = z(B, Sq, 1, 128, dtype=torch.bfloat16), z(1, 16, 1, 128, dtype=torch.bfloat16)
+pgqa.accumulate_weights(q, k, z(B, 1, dtype=torch.int32), lens, z(B, 1, Sq), w)
+pgqa.check_device_error()
+# scores of 0 and a log-sum-exp of 0: each row adds exp(0)
+assert torch.equal(w.flatten().cpu(), torch.tensor([float(Sq)] * 5 + [0.0] * 11)), w
+"""
 
 
 @pytest.mark.parametrize("kv", ["bf16", "e4m3"])
@@ -102,3 +122,42 @@ def test_chains_without_a_stop_between_the_calls(Sq, both_kernels, cuda_device):
         for a, b in zip(run(False), want):
             assert torch.equal(a, b)
     pgqa.check_device_error()
+
+
+@pytest.mark.parametrize("B,Sq", [(12279, 1), (12284, 1), (12287, 8), (3575, 16), (3580, 16), (3583, 9)])
+def test_weights_of_a_batch_whose_table_ends_near_48_kb(B, Sq, cuda_device):
+    """The kernel's shared memory, its few static bytes included, lies around the size up to
+    which a launch needs no raised limit.  In a fresh process: no larger call has raised it."""
+    r = subprocess.run([sys.executable, "-c", ONE_BATCH, str(B), str(Sq)], cwd=REPO, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+TWO_THREADS = """
+import threading, torch
+import mx_flash_attn_kernel_opt__b200 as pgqa
+torch.cuda.init()
+z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device="cuda")
+bad = []
+def calls(B):
+    try:
+        k, w = z(1, 16, 1, 128, dtype=torch.bfloat16), z(1, 1, 16)
+        a = (z(B, 1, 128, dtype=torch.bfloat16), k, z(B, 1, dtype=torch.int32), z(B, dtype=torch.int32), z(B, 1, 1), w)
+        go.wait()
+        for _ in range(50):
+            pgqa.accumulate_weights(*a)
+    except Exception as e:
+        bad.append((B, repr(e)))
+go = threading.Barrier(4)
+ts = [threading.Thread(target=calls, args=(B,)) for B in (13000, 28000, 100, 20000)]
+[t.start() for t in ts]
+[t.join() for t in ts]
+pgqa.check_device_error()
+assert not bad, bad
+"""
+
+
+def test_weights_of_small_and_large_batches_from_several_threads(cuda_device):
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", TWO_THREADS], cwd=REPO, capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
