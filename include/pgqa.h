@@ -436,8 +436,9 @@ int pgqa_last_status(void);
 const char* pgqa_status_string(int status);
 
 /* Synchronous: waits for `stream`, reads and clears the device-side error word of
- * `workspace` (NULL = the library workspace of the current device).  Returns
- * PGQA_OK or one of the PGQA_ERR_DEVICE_* codes. */
+ * `workspace` (NULL = the library workspace of the current device, and the word of the
+ * operators that take none; both are cleared, the operators' error is returned first).
+ * Returns PGQA_OK or one of the PGQA_ERR_DEVICE_* codes. */
 int pgqa_check_device_error(void* workspace, void* stream);
 
 /*

@@ -2113,13 +2113,13 @@ extern "C" int pgqa_check_device_error(void* workspace, void* stream) {
             std::lock_guard<std::mutex> lk(g_dev_mu);
             word = g_error_word_ptr[dev];
         }
-        if (word != nullptr) {
-            const int st = read_error_word(word, static_cast<cudaStream_t>(stream));
-            if (st != PGQA_OK) return st;
-        }
+        int st = PGQA_OK;
+        if (word != nullptr) st = read_error_word(word, static_cast<cudaStream_t>(stream));
+        // both words are read and cleared, so that no error is left for a later check
         std::lock_guard<std::mutex> lk(g_ws_mu);
-        if (dev < 0 || dev >= kMaxDevices || g_ws[dev].ptr == nullptr) return PGQA_OK;
-        workspace = g_ws[dev].ptr;
+        if (dev < 0 || dev >= kMaxDevices || g_ws[dev].ptr == nullptr) return st;
+        const int ws_st = read_error_word(g_ws[dev].ptr, static_cast<cudaStream_t>(stream));
+        return st != PGQA_OK ? st : ws_st;
     }
     return read_error_word(workspace, static_cast<cudaStream_t>(stream));
 }

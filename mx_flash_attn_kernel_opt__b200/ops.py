@@ -323,7 +323,8 @@ def run_kernel_cabi(q, k_cache_paged, v_cache_paged, output, cache_seqlens, bloc
 
 
 def check_device_error(workspace=None, device=None):
-    """Synchronously read and clear the device error word (raises on error)."""
+    """Synchronously read and clear the device error word of `workspace`, or without one those
+    of the library's own workspace and of the operators that take none (raises on error)."""
     L = lib()
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     with torch.cuda.device(dev):

@@ -161,3 +161,20 @@ def test_weights_of_small_and_large_batches_from_several_threads(cuda_device):
     for _ in range(3):
         r = subprocess.run([sys.executable, "-c", TWO_THREADS], cwd=REPO, capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_one_check_clears_the_errors_of_every_entry_point(cuda_device):
+    """A decode in the library's own workspace and a rotary append both go wrong: one check
+    reports, and the next one finds nothing."""
+    c = test_rope_gpu.Case([5, 20], [2, 2], seed=1, rows=64).to(cuda_device)
+    c.d["pos"][0, 3] = 64
+    c.call()
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=cuda_device)  # noqa: E731
+    k, bt = z(2, 16, 2, 128), torch.tensor([[0], [1]], dtype=torch.int32, device=cuda_device)
+    lens = torch.tensor([3, 17], dtype=torch.int32, device=cuda_device)      # 17 tokens in one page of 16
+    pgqa.run_kernel_cabi(z(2, 8, 128), k, k, z(2, 8, 128), lens, bt, 2, 16, 1, 8, 2, 128, 16, 2, 0)
+    torch.cuda.synchronize()
+    with pytest.raises(PgqaError) as e:
+        pgqa.check_device_error()
+    assert e.value.status in (10, 12)
+    pgqa.check_device_error()
