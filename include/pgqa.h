@@ -262,8 +262,8 @@ int pgqa_noalloc_check_device_error(void* stream);
  *   k_new, v_new bf16 [tokens, Hkv, 128]; both NULL: nothing to append (the pools and the
  *                table are then not used; seq_lens only where positions is NULL)
  *   *_strides    element strides of q, k_new, v_new between sequences, tokens and heads
- *                (multiples of 8; the 128 elements of a head are contiguous); q_out is
- *                contiguous
+ *                (multiples of 8, not negative; those of a dimension of one entry are not
+ *                used; the 128 elements of a head are contiguous); q_out is contiguous
  *   cu_seqlens   NULL: [batch_size, seqlen] tokens, tokens = batch_size * seqlen.
  *                Else int32 [batch_size + 1], ascending from 0: tokens of all sequences
  *                packed, those of sequence b at [cu[b], cu[b + 1]); the sequence stride is

@@ -308,10 +308,12 @@ int entry(const pgqa_rope_args* a, cudaStream_t stream) {
     for (int i = 0; i < a->rotary_dim / 2; ++i)
         if (a->pair_axis[i] >= a->num_axes) return PGQA_ERR_BAD_SHAPE;
     Params p = {};
+    // a dimension of one entry may come with any stride: no address depends on it
+    const bool used[3] = {!a->cu_seqlens && a->batch_size > 1, (a->cu_seqlens ? a->tokens : a->seqlen) > 1, true};
     for (int i = 0; i < 3; ++i) {
-        p.qs[i] = a->q_strides[i];
-        p.ks[i] = a->k_strides[i];
-        p.vs[i] = a->v_strides[i];
+        p.qs[i] = used[i] && (i < 2 || Hq > 1) ? a->q_strides[i] : 0;
+        p.ks[i] = used[i] && (i < 2 || Hk > 1) ? a->k_strides[i] : 0;
+        p.vs[i] = used[i] && (i < 2 || Hk > 1) ? a->v_strides[i] : 0;
     }
     if ((a->q && !strides_ok(p.qs)) || (append && (!strides_ok(p.ks) || !strides_ok(p.vs)))) return PGQA_ERR_MISALIGNED;
     if (!host_aligned(a->q, 16) || !host_aligned(a->k_new, 16) || !host_aligned(a->v_new, 16) ||

@@ -178,3 +178,30 @@ def test_one_check_clears_the_errors_of_every_entry_point(cuda_device):
         pgqa.check_device_error()
     assert e.value.status in (10, 12)
     pgqa.check_device_error()
+
+
+def odd_strides(x):
+    """The same elements with strides of 7 for every dimension of size 1."""
+    return x.as_strided(x.shape, [7 if n == 1 else s for n, s in zip(x.shape, x.stride())])
+
+
+@pytest.mark.parametrize("lens,new,Hq,Hkv,packed", [
+    ([5], [3], 8, 2, False), ([5, 9, 2], [1, 1, 1], 8, 2, False), ([4], [1], 1, 1, False), ([3], [4], 1, 1, False),
+    ([7], [1], 4, 1, True)])
+def test_strides_of_dimensions_of_size_one(lens, new, Hq, Hkv, packed, cuda_device):
+    """torch gives such a dimension any stride, and no address depends on it."""
+    c = test_rope_gpu.Case(lens, new, Hq=Hq, Hkv=Hkv, packed=packed, seed=len(lens) + Hq).to(cuda_device)
+    x = c.d["qkv"]
+    cu = None
+    pos = c.d["pos"]
+    q, k, v = c.split(x)
+    if packed:
+        cu = torch.tensor([0, sum(new)], dtype=torch.int32, device=cuda_device)
+    else:
+        q, k, v = (t.unflatten(0, (len(new), new[0])) for t in (q, k, v))
+        pos = pos.unflatten(1, (len(new), new[0]))
+    q, k, v = (odd_strides(t) for t in (q, k, v))
+    out = pgqa.rope_append_kv(q, k, v, c.d["kc"], c.d["vc"], c.d["bt"], c.d["lens"], c.d["cos"], c.d["sin"],
+                              positions=pos, axes=c.axes, cu_seqlens=cu, weights=c.d["w"])
+    pgqa.check_device_error()
+    c.check(out)
