@@ -277,10 +277,11 @@ def accumulate_weights(q, k_cache, block_table, seq_lens, lse, weights, *, scale
         ks = _scales(k_scale, Hkv, dev)
     elif k_scale is not None:
         raise ValueError("k_scale applies to float8_e4m3fn pools only")
-    _call(lib().pgqa_accumulate_weights, _WEIGHTS.pack(
-        _WEIGHTS.size, qp, kp, lsep, wp, lp, tp, 0 if ks is None else ks.data_ptr(), B, Sq, Hq, Hkv, D,
-        P, num_pages, width, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale,
-        1 if fp8 else 0), dev, "pgqa_accumulate_weights")
+    if B:  # torch gives empty tensors no address
+        _call(lib().pgqa_accumulate_weights, _WEIGHTS.pack(
+            _WEIGHTS.size, qp, kp, lsep, wp, lp, tp, 0 if ks is None else ks.data_ptr(), B, Sq, Hq, Hkv, D,
+            P, num_pages, width, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale,
+            1 if fp8 else 0), dev, "pgqa_accumulate_weights")
     return weights
 
 
@@ -307,9 +308,10 @@ def evict_kv(k_cache, v_cache, weights, block_table, seq_lens, keep, *, sinks=0,
     if keep < 1:
         raise PgqaError(2, f"{what}: keep must be at least 1")
     kept, new_lens = seq_lens.new_empty((B, Hkv, keep)), seq_lens.new_empty((B,))
-    _call(lib().pgqa_evict, _EVICT.pack(
-        _EVICT.size, kp, vp, wp, op, lp, tp, kept.data_ptr(), new_lens.data_ptr(), B, Hkv, D, P,
-        num_pages, width, keep, sinks, recent, 1 if fp8 else 0, 0), dev, "pgqa_evict")
+    if B:
+        _call(lib().pgqa_evict, _EVICT.pack(
+            _EVICT.size, kp, vp, wp, op, lp, tp, kept.data_ptr(), new_lens.data_ptr(), B, Hkv, D, P,
+            num_pages, width, keep, sinks, recent, 1 if fp8 else 0, 0), dev, "pgqa_evict")
     return kept, new_lens
 
 

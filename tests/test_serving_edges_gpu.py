@@ -205,3 +205,23 @@ def test_strides_of_dimensions_of_size_one(lens, new, Hq, Hkv, packed, cuda_devi
                               positions=pos, axes=c.axes, cu_seqlens=cu, weights=c.d["w"])
     pgqa.check_device_error()
     c.check(out)
+
+
+def test_empty_batches(cuda_device):
+    """A step in which no sequence is left: every operator returns outputs of no rows."""
+    z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=cuda_device)  # noqa: E731
+    bf, i32 = torch.bfloat16, torch.int32
+    k, v = z(4, 16, 2, 128, dtype=bf), z(4, 16, 2, 128, dtype=bf)
+    w, bt, lens, t = z(4, 2, 16) + 3, z(0, 2, dtype=i32), z(0, dtype=i32), z(8, 64)
+    q, kn = z(0, 8, 128, dtype=bf), z(0, 2, 128, dtype=bf)
+    assert pgqa.rope_append_kv(q, kn, kn, k, v, bt, lens, t, t, weights=w).shape == (0, 8, 128)
+    assert pgqa.accumulate_weights(q, k, bt, lens, z(0, 8, 1), w) is w
+    kept, new = pgqa.evict_kv(k, v, w, bt, lens, 5)
+    assert kept.shape == (0, 2, 5) and kept.dtype == i32 and new.shape == (0,) and new.dtype == i32
+    assert pgqa.cross_attention(z(0, 3, 8, 128, dtype=bf), k, v, bt, lens).shape == (0, 3, 8, 128)
+    assert (w == 3).all()
+    with pytest.raises(PgqaError):
+        pgqa.evict_kv(k, v, w, bt, lens, 0)
+    with pytest.raises(PgqaError):
+        pgqa.accumulate_weights(q, k, bt, lens, z(0, 7, 1), w)
+    pgqa.check_device_error()
