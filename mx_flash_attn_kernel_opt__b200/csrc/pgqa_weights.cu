@@ -22,8 +22,9 @@
  *
  * e4m3 keys become f16 in registers, exactly (4 significant bits), and q is turned into f16
  * once per unit: each row times the power of two that brings its largest element to [2^14,
- * 2^15), undone in fp32 (8 significant bits fit f16's 11; an element 2^28 times smaller than
- * its row's largest is rounded to 2^-25).
+ * 2^15), undone in fp32.  8 significant bits fit f16's 11; elements more than 2^31 times smaller
+ * than their row's largest are rounded to a multiple of 2^-24, which is off by 2^-39 of the
+ * largest at most.  Rows whose largest is below 2^-112 are only brought up by 2^126.
  *
  * Measured: 290,000 tokens in 256 sequences, 8 KV heads, 4 rows each, bf16 101 us (6.1 TB/s,
  * 0.93 of a copy's rate); 2 sequences of 32,768 tokens, e4m3: 20 us with 8 rows per KV head
@@ -116,7 +117,8 @@ __device__ __forceinline__ void load_group(const Params& p, int32_t b, int32_t k
         }
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = max(-100, min(100, 14 - ((int)(mx >> 23) - 127)));
+        // every finite maximum down to 2^-112; 2^e and 2^-e are both normal numbers
+        const int e = max(-113, min(126, 14 - ((int)(mx >> 23) - 127)));
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         down = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll

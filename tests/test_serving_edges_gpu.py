@@ -9,7 +9,7 @@ import torch
 
 import mx_flash_attn_kernel_opt__b200 as pgqa
 from mx_flash_attn_kernel_opt__b200 import PgqaError
-from tests import _paged, test_cross_gpu, test_rope_gpu
+from tests import _paged, test_cross_gpu, test_rope_gpu, test_weights_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -225,3 +225,24 @@ def test_empty_batches(cuda_device):
     with pytest.raises(PgqaError):
         pgqa.accumulate_weights(q, k, bt, lens, z(0, 7, 1), w)
     pgqa.check_device_error()
+
+
+@pytest.mark.parametrize("Hq,Sq", [(8, 1), (8, 5)])
+@pytest.mark.parametrize("up", [2.0 ** 118, 2.0 ** -116])
+def test_weights_of_very_large_and_very_small_queries(up, Hq, Sq, cuda_device):
+    """q times 2^n and the scale of K times 2^-n: the same scores, so the same weights and bounds."""
+    q, k, bt, lens, lse, w, scale, ks = test_weights_gpu.make([33, 7], Hq, 2, 16, Sq, "e4m3", seed=50 + Sq)
+    big = (q.float() * up).to(torch.bfloat16)
+    assert big.isfinite().all() and (up < 1 or torch.equal(big.float() / up, q.float()))
+    test_weights_gpu.run_and_check((big, k, bt, lens, lse, w, scale, ks / up), False, cuda_device)
+
+
+@pytest.mark.parametrize("Hq,Sq", [(8, 1), (8, 5)])
+def test_weights_of_queries_with_elements_far_below_the_largest(Hq, Sq, cuda_device):
+    """Each row's elements span 2^40: those far below the largest keep fewer bits in f16.  What
+    that may move a score, 2^-25 of the scaled row against 2^14 at the least, 2^-39 of the largest
+    element for each product, is far inside the bound, which counts 2^-16 of the products' sum."""
+    q, k, bt, lens, lse, w, scale, ks = test_weights_gpu.make([33, 7], Hq, 2, 16, Sq, "e4m3", seed=60 + Sq)
+    g = torch.Generator().manual_seed(61)
+    small = (q.float() * 2.0 ** -torch.randint(0, 41, q.shape, generator=g).float()).to(torch.bfloat16)
+    test_weights_gpu.run_and_check((small, k, bt, lens, lse, w, scale, ks), False, cuda_device)
