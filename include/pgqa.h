@@ -344,8 +344,8 @@ int pgqa_accumulate_weights(const pgqa_weights_args* args, void* stream);
  * min(L, keep) slots and is otherwise left as it was).
  *   kept      int32 [B, Hkv, keep]: the indices kept, ascending; a sequence of L <= keep
  *             tokens is not changed and gets 0 .. L-1 and then -1
- *   new_lens  int32 [B]: min(L, keep); not seq_lens itself, which both launches read
- *             (PGQA_ERR_BAD_SHAPE)
+ *   new_lens  int32 [B]: min(L, keep); shares no element with seq_lens, which the clusters
+ *             of other heads and sequences still read (PGQA_ERR_BAD_SHAPE)
  * weights and weights_out are 16-byte aligned.
  * Sequences that share pages cannot be cut (a row kept by one would be overwritten by the
  * other).  The pages from ceil(keep / P) on are the caller's to free.

@@ -557,8 +557,12 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
     if (a->keep <= 0 || a->keep > INT32_MAX || a->sinks < 0 || a->recent < 0 || a->sinks > a->keep ||
         a->recent > a->keep - a->sinks)
         return PGQA_ERR_BAD_SHAPE;
-    if (a->new_lens == a->seq_lens) return PGQA_ERR_BAD_SHAPE;
     if (a->batch_size * a->num_heads_k > INT32_MAX / kMaxCluster) return PGQA_ERR_UNSUPPORTED;
+    {  // the clusters of a sequence's heads read its length when another's may have been written
+        const uintptr_t r = reinterpret_cast<uintptr_t>(a->seq_lens), w = reinterpret_cast<uintptr_t>(a->new_lens);
+        const uintptr_t bytes = 4 * (uintptr_t)a->batch_size;
+        if (r < w + bytes && w < r + bytes) return PGQA_ERR_BAD_SHAPE;
+    }
     if (!host_aligned(a->k_cache, 16) || !host_aligned(a->v_cache, 16) || !host_aligned(a->weights, 16) ||
         !host_aligned(a->weights_out, 16) || !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) ||
         !host_aligned(a->kept, 4) || !host_aligned(a->new_lens, 4))
