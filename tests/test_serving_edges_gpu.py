@@ -9,7 +9,7 @@ import torch
 
 import mx_flash_attn_kernel_opt__b200 as pgqa
 from mx_flash_attn_kernel_opt__b200 import PgqaError
-from tests import _paged, test_cross_gpu, test_rope_gpu, test_weights_gpu
+from tests import _paged, test_cross_gpu, test_evict_gpu, test_rope_gpu, test_weights_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -246,3 +246,73 @@ def test_weights_of_queries_with_elements_far_below_the_largest(Hq, Sq, cuda_dev
     g = torch.Generator().manual_seed(61)
     small = (q.float() * 2.0 ** -torch.randint(0, 41, q.shape, generator=g).float()).to(torch.bfloat16)
     test_weights_gpu.run_and_check((small, k, bt, lens, lse, w, scale, ks), False, cuda_device)
+
+
+@pytest.mark.parametrize("interleaved,table", [(False, "fp32"), (True, "bf16")])
+def test_packed_prompts_into_e4m3_pages(interleaved, table, cuda_device):
+    c = test_rope_gpu.Case([0, 7, 31, 2], [5, 0, 40, 1], R=64, kv="e4m3", axes="turn", packed=True,
+                           interleaved=interleaved, table=table, seed=80).to(cuda_device)
+    c.check(c.call())
+    pgqa.check_device_error()
+
+
+def evict_cluster(pairs, capacity):
+    """CTAs per (sequence, KV head), by the rule in csrc/pgqa_evict.cu."""
+    places, n = 2 * torch.cuda.get_device_properties(0).multi_processor_count, 2
+    while n < 8 and pairs * 2 * n <= places and capacity // (2 * n) >= 1024:
+        n *= 2
+    return n
+
+
+@pytest.mark.parametrize("lens,Hkv,keep,sinks,recent,cluster", [
+    ([4200, 4100, 60, 0, 30], 8, 1500, 4, 64, 4), ([4097, 4096], 1, 4095, 0, 0, 4), ([2300] * 2, 2, 700, 1, 2, 2),
+    ([9000, 100], 2, 2100, 0, 300, 8)])
+@pytest.mark.parametrize("kv,apart", [("bf16", False), ("e4m3", True)])
+def test_evict_in_clusters_of_each_size(lens, Hkv, keep, sinks, recent, cluster, kv, apart, cuda_device):
+    case = test_evict_gpu.make(lens, Hkv, 16, kv, seed=90 + cluster)
+    assert evict_cluster(len(lens) * Hkv, 16 * case[3].shape[1]) == cluster
+    test_evict_gpu.run_and_check(case, keep, sinks, recent, cuda_device, apart=apart)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_pools_of_more_than_2_31_elements(kv, cuda_device):
+    """The same calls on the last pages of a large pool and on a small one: equal results, and
+    no byte of the large pool changes anywhere else."""
+    dev, P, Hq, Hkv, S = cuda_device, 16, 16, 8, 3
+    g = torch.Generator().manual_seed(100)
+    lens = [70, 1, 200]
+    bt, pages = _paged.table([n + S for n in lens], P, g)
+    more = 140000                       # pages of 16 x 8 x 128 elements
+    assert more * P * Hkv * 128 > 2 ** 31
+    k, v = (_paged.pool(pages, P, Hkv, g, kv) for _ in range(2))
+    w0 = torch.rand(pages, Hkv, P, generator=g) * 0.01
+    cos, sin = (x.to(dev) for x in test_rope_gpu.tables(512, 128))
+    x = torch.randn(len(lens), S, Hq + 2 * Hkv, 128, generator=g).to(torch.bfloat16).to(dev)
+    before = torch.tensor(lens, dtype=torch.int32, device=dev)
+    after = before + S
+    scale = dict(k_scale=0.7, v_scale=0.9) if kv == "e4m3" else {}
+    ks = {n: s for n, s in scale.items() if n == "k_scale"}
+
+    def run(kd, vd, w, table):
+        q = pgqa.rope_append_kv(x[:, :, :Hq], x[:, :, Hq:Hq + Hkv], x[:, :, Hq + Hkv:], kd, vd, table, before, cos,
+                                sin, weights=w, **scale)
+        out, lse = pgqa.cross_attention(q, kd, vd, table, after, return_lse=True, **scale)
+        pgqa.accumulate_weights(q, kd, table, after, lse, w, **ks)
+        kept, new = pgqa.evict_kv(kd, vd, w, table, after, 50, sinks=2, recent=5)
+        pgqa.check_device_error()
+        return q, out, lse, kept, new
+
+    small = [t.to(dev) for t in (k, v, w0)]
+    want = run(*small, bt.to(dev))
+    large = []
+    for t in (k, v, w0):
+        big = torch.zeros(more + pages, *t.shape[1:], dtype=t.dtype, device=dev)
+        big.view(torch.uint8)[more:] = t.view(torch.uint8).to(dev)
+        large.append(big)
+    used = bt != 2 ** 30
+    got = run(*large, torch.where(used, bt + more, bt).to(dev))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for a, b in zip(large, small):
+        assert torch.equal(_paged.raw(a[more:]), _paged.raw(b))
+        assert not a[:more].view(torch.uint8).any()
