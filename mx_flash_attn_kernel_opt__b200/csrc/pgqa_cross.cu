@@ -103,8 +103,9 @@ struct Params {
     int32_t grid;            // CTAs of the first launch
     float scale_log2;
     uint64_t wait_limit_ns;
-    int32_t debug_stuck;     // test hook: > 0 makes every CTA's first load expect 16 bytes too many
-    int32_t debug_long;      // test hook: key tiles that the last slice believes to have too many
+    // Test hooks, PGQA_DEBUG_STUCK_BARRIER = n or -n, read per call:
+    int32_t debug_stuck;     // > 0 makes every CTA's first load expect 16 bytes too many
+    int32_t debug_long;      // key tiles that the last slice believes to have too many
     int32_t out_32;          // out is 32-byte aligned (torch gives a view any multiple of its element)
 };
 
@@ -1091,9 +1092,9 @@ int entry(const pgqa_cross_args* a, cudaStream_t stream) {
     p.wait_limit_ns = (lim && *lim) ? strtoull(lim, nullptr, 10) : kWaitLimitNs;
     if (p.wait_limit_ns == 0 || p.wait_limit_ns > 10 * kWaitLimitNs) p.wait_limit_ns = kWaitLimitNs;
     const char* stuck = getenv("PGQA_DEBUG_STUCK_BARRIER");
-    p.debug_stuck = (stuck && *stuck) ? atoi(stuck) : 0;
-    const char* longer = getenv("PGQA_DEBUG_LONG_SLICE");
-    p.debug_long = (longer && *longer) ? atoi(longer) : 0;
+    const int hook = (stuck && *stuck) ? atoi(stuck) : 0;
+    p.debug_stuck = hook > 0 ? hook : 0;
+    p.debug_long = hook < 0 ? -hook : 0;
     CUtensorMap qm, km, vm;
     const int64_t slots = a->num_pages * a->page_size;
     const int64_t row = kv8 ? 128 : 256;

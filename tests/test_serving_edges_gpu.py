@@ -66,14 +66,14 @@ def test_cross_slice_longer_than_its_items_ends(new, lens, kv, cuda_device, monk
     cu = cu.to(cuda_device)
     want = pgqa.cross_attention(*a, cu_seqlens_q=cu)
     pgqa.check_device_error()
-    monkeypatch.setenv("PGQA_DEBUG_LONG_SLICE", "1")
+    monkeypatch.setenv("PGQA_DEBUG_STUCK_BARRIER", "-1")
     monkeypatch.setenv("PGQA_WAIT_LIMIT_NS", "3000000")
     out = pgqa.cross_attention(*a, cu_seqlens_q=cu)
     with pytest.raises(PgqaError) as e:
         pgqa.check_device_error()
     assert e.value.status == 10
     assert torch.equal(out, want)
-    monkeypatch.delenv("PGQA_DEBUG_LONG_SLICE")
+    monkeypatch.delenv("PGQA_DEBUG_STUCK_BARRIER")
     monkeypatch.delenv("PGQA_WAIT_LIMIT_NS")
     assert torch.equal(pgqa.cross_attention(*a, cu_seqlens_q=cu), want)
     pgqa.check_device_error()
