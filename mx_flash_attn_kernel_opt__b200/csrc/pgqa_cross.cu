@@ -183,7 +183,7 @@ __device__ void find_slice(const Params& p, int32_t c, Slice& out) {
         if (lane >= o) incl += v;
     }
     if (lane == 31) wsum[warp] = incl;
-    if (tid == 0) {  // an empty slice, should no sequence below be found to hold its start
+    if (tid == kThreads - 1) {  // an empty slice, should no sequence below be found to hold its start
         out.lo = INT64_MAX;
         out.hi = out.base = out.item_lo = 0;
         out.item_len = 1;
