@@ -243,8 +243,8 @@ int pgqa_noalloc_check_device_error(void* stream);
  * and keep nothing between calls, may be captured into a CUDA graph after one eager call
  * on the device, and may run on several streams at once as long as the calls' outputs and
  * pages differ.  What a call reads (lengths, tables, cu_seqlens among it) must not be written
- * while it runs, but by the call itself where that is said.  Their device-side errors go to one word per device, which
- * pgqa_check_device_error(NULL, stream) reads and clears.
+ * while it runs, but by the call itself where that is said.  Device-side errors go to one
+ * word per device, which pgqa_check_device_error(NULL, stream) reads and clears.
  */
 
 /*
@@ -312,8 +312,9 @@ int pgqa_rope_append(const pgqa_rope_args* args, void* stream);
  * lengths (of the sequences attended over, appended tokens included), causal and scale are
  * those of the decode; softmax_lse [B, Hq, Sq] fp32 is what it returned.  weights is fp32
  * [num_pages, Hkv, P].  A row whose log-sum-exp is -inf adds nothing; entries from a
- * sequence's length on are not touched.  Each entry gets one addition per call, in one
- * order, unless sequences share a page: then their sums are added in any order.
+ * sequence's length on are not touched.  Each entry gets one fp32 addition per 32 query rows
+ * of its KV head, in one order, unless sequences share a page: then their sums are added in
+ * any order.
  * seqlen_q is at most 4096 and batch_size at most about 11,000 (28,000 with up to 8 query
  * rows per KV head; PGQA_ERR_UNSUPPORTED).
  */
@@ -371,7 +372,9 @@ int pgqa_evict(const pgqa_evict_args* args, void* stream);
  * Cross attention: out[x, h] = softmax(scale * q[x, h] . K^T) . V over the first seq_lens[b]
  * tokens of sequence b's pages, for every query token x of sequence b.  No causal mask; the
  * number of query tokens and of keys are unrelated.  A sequence without keys gives zeros
- * (and a log-sum-exp of -inf).  q and out bf16, fp32 scores, sums and accumulators.
+ * (and a log-sum-exp of -inf).  q and out bf16; scores, softmax sums and accumulators are
+ * fp32, and the weights that multiply V are rounded to bf16 (2^-8 relative at most; their
+ * sum, which normalises, is not), so a result is rounded twice.
  *   q            [tokens, Hq, 128], token stride q_stride elements (a multiple of 8, at
  *                least Hq * 128), heads contiguous
  *   out          [tokens, Hq, 128], contiguous, 16-byte aligned

@@ -29,20 +29,24 @@
  *                   a weight of 0 never meets a NaN left in a page.
  *   warps 12-15     (e4m3 pages) turn the tiles that TMA brings as they are into bf16, exactly,
  *                   in the ring that the MMAs read (four slots then); the scales go into the
- *                   score's factor and the normaliser.  2 x 4096 tokens, 32 + 8 heads, over 8192
- *                   keys: 1.03 ms, 0.92 ms from bf16 pages on the same GPU; two such
- *                   warpgroups leave 96 registers a thread, and the spills cost more (1.12 ms).
+ *                   score's factor and the normaliser.  Two such warpgroups leave 96
+ *                   registers a thread, and the spills cost more (long prompts 9% slower).
  *   warps 9, 10     issue the MMAs of tile 0 and of tile 1: S = Q K^T (both from shared
  *                   memory), O += P V (P from TMEM).
  * TMEM: two score buffers of 64 columns for each tile (from columns 0 and 128), O at 256 and
  * 384.  The scores of step i + 2 are issued right behind the PV of step i, which frees their
  * buffer, so while a warpgroup works on step i + 1 its next scores are computed and neither
  * waits for the other.  The price is QK^T with N = 64, which re-reads Q from shared memory
- * twice as often: 48 clocks an MMA instead of 32.  Measured: 2 x 4096 tokens, 32 + 8 heads, over
- * 8192 keys each 1.01 to 1.04 ms back to back (1060 TFLOP/s, at the power cap) and 859 us in
- * single calls; with one buffer of 128 columns per tile, where the softmax waits for PV and
- * QK^T of every step, 1.19 ms back to back.  Prompts of 17 to 1024 tokens over 197 to 4097 keys,
- * 28 + 4 heads: 160 us (930 TFLOP/s).
+ * twice as often: 48 clocks an MMA instead of 32.  With one buffer of 128 columns per tile, where
+ * the softmax waits for PV and QK^T of every step, long prompts took 15% more.
+ *
+ * Measured, 40 calls after a pause / a loop of 0.6 s, in which the 1000 W cap holds the clock
+ * down (us):                                                    bf16 pages    e4m3 pages
+ *   2 x 4096 tokens, 32 + 8 heads, over 8192 keys              916 / 1045    1029 / 1116
+ *   8 prompts of 17 to 1024 tokens, 28 + 4 heads, 197 to 4097   166 / 180     190 / 193
+ *   16 x 3 tokens, 32 + 8 heads, over 16,000 keys               200 / 234     250 / 250
+ * The first is 1200 / 1052 TFLOP/s, the second 897 / 826; K and V of the third take 161 us (e4m3
+ * 81 us) to read once.
  *
  * Every wait is bounded: one that expires sets the device error word and the CTA's abort
  * flag, every role leaves its loop, loads and MMAs in flight are drained and TMEM is freed.
@@ -80,9 +84,10 @@ struct Geo {
     static constexpr int kSmem = 1024 + kBarOff + kBars * 8 + 16;
 };
 constexpr int kRows = 2 * kTile;           // rows of a work item
-// What an item costs beside its key tiles, in key tiles (1 to 4 measured: 175, 159, 167, 166 us
-// for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys), and the least length of a slice
-// (1, 2 and 3: 17.7, 14.0, 16.7 us for 10 + 13 tokens over 1024 keys, 32 + 8 heads).
+// What an item costs beside its key tiles, in key tiles (1 to 4 measured in one session: 175, 159,
+// 167, 166 us for ragged prompts of 17 to 1024 tokens over 197 to 4097 keys; calls of one build
+// spread by as much as 2 from 3 and 4, so only 1 is ruled out), and the least length of a slice
+// (1, 2 and 3: 17.7, 14.0, 16.7 us for 10 + 13 tokens over 1024 keys, 32 + 8 heads, in a graph).
 constexpr int kItemCost = 2, kMinSlice = 2;
 constexpr int kSnap = 24;
 constexpr float kLazyLog2 = 8.f;
@@ -348,8 +353,9 @@ __device__ Cut cut_of(const Params& p, int32_t c, const Slice& s) {
  * bits stand in the low bits of bf16's, which is the value times 2^(7 - 127), subnormals
  * too, and the product with 2^120 is exact.  Shifts by multiplication, so that the integer
  * and the FMA pipes share the work; the four converting warps are what bounds short prompts
- * (16 x 3 tokens, 32 + 8 heads, over 16,000 keys: 262 us with conversion instructions, which
- * leave at a fraction of the rate, 245 us with shifts and masks, 224 to 232 us so). */
+ * (16 x 3 tokens, 32 + 8 heads, over 16,000 keys, in one session: 262 us with conversion
+ * instructions, which leave at a fraction of the rate, 245 us with shifts and masks, 224 to 232
+ * us so; in later sessions 250 us). */
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t b, uint32_t& lo, uint32_t& hi) {
     // 16-bit lanes 0000 s eeee mmm 0000; the sign goes from bit 11 to bit 15: + 15 * 2^11
     const uint32_t x = __byte_perm(b, 0, 0x4140) * 16u, y = __byte_perm(b, 0, 0x4342) * 16u;
@@ -927,7 +933,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p) {
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     // kParts parts in flight, with their log-sum-exps: one token over 8000 keys, 8 + 1 heads,
     // 27 -> 19 us; with four in flight the registers cost more where whole tiles are joined (ragged
-    // prompts: 169 instead of 163 us)
+    // prompts: 169 instead of 163 us in one session)
 #pragma unroll 1
     for (int32_t c0 = j; c0 <= last; c0 += kParts) {
         float l2[kParts], top = m;

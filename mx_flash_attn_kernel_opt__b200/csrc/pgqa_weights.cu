@@ -17,8 +17,8 @@
  * addresses as B fragments.  Two or three chunks
  * are held, one at work and the others in flight.  The four lanes
  * that share a token add their partial sums by shuffles, and the token's weight gets one
- * red.add: no other warp of the call adds to it (unless sequences share a page), so the
- * result does not depend on any order.
+ * red.add for every 32 query rows, all from the same lane: no other warp of the call adds to it
+ * (unless sequences share a page), so the result does not depend on any order.
  *
  * e4m3 keys become f16 in registers, exactly (4 significant bits), and q is turned into f16
  * once per unit: each row times the power of two that brings its largest element to [2^14,
@@ -27,9 +27,14 @@
  * largest at most.  Rows whose largest is below 2^-112 are only brought up by 2^126.
  *
  * Measured: 290,000 tokens in 256 sequences, 8 KV heads, 4 rows each, bf16 101 us (6.1 TB/s,
- * 0.93 of a copy's rate); 2 sequences of 32,768 tokens, e4m3: 20 us with 8 rows per KV head
- * (start and end of the call, about 8 us, included), 31 us with 32 and 54 us with 64, where
- * the products and exponentials of a chunk take longer than its load.
+ * 0.93 of a copy's rate).  2 sequences of 32,768 tokens, 8 KV heads, rows per KV head:
+ *               1      8     16     32     64    256   (us; start and end of the call, about 8)
+ *   bf16       27     27     28     36     66    240   K takes 21 us to read
+ *   e4m3       20     20     24     31     54    190   11 us
+ * From 32 rows on the products and exponentials of a chunk take longer than its load, and every
+ * 32 rows are a pass over K of their own.  Rows that are no multiple of 16 or 32 cost as much as
+ * the next one, and lose the path without comparisons (28 rows over 4 KV heads, half the
+ * keys: 24 us bf16, 22 us e4m3, where half of the 32 rows' are 18 and 16).
  */
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -361,7 +366,8 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const Params p) {
                 if (NT == 1) {
                     add(qf, cl);
                 } else if ((c + 1) * kChunkTokens <= all_see) {
-                    // nearly every chunk of a long sequence: no comparisons and no selects (2
+                    // nearly every chunk of a long sequence, in turns without a padding row or a row
+                    // that saw nothing (their bounds are 0): no comparisons and no selects (2
                     // sequences of 32,768 tokens, 32 rows: 33.7 -> 30.9 us e4m3, 40.2 -> 36.2 us bf16)
 #pragma unroll 4
                     for (int j = 0; j < NT; ++j) {

@@ -260,7 +260,8 @@ def accumulate_weights(q, k_cache, block_table, seq_lens, lse, weights, *, scale
     q, k_cache, block_table, seq_lens (the lengths attended over), scale, causal and k_scale
     are the decode's, lse [B, Hq, Sq] fp32 is what it returned with `return_lse`.  A row that
     sees no token (lse -inf) adds nothing, and entries past a sequence's length are left as
-    they are.  Unless sequences share pages, the result does not depend on any order."""
+    they are.  The sums are fp32, one addition to an entry per 32 query rows of its KV head;
+    unless sequences share pages, the result does not depend on any order."""
     what = "accumulate_weights"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
     num_pages, P, Hkv, D = shape
@@ -328,14 +329,16 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
 
     q [B, Sq, Hq, 128] bf16, or packed [tokens, Hq, 128] with `cu_seqlens_q` [B + 1] int32,
     ascending from 0; its token stride may be any multiple of 8 elements (a slice of a
-    projection), heads contiguous.  k_cache / v_cache [num_pages, P, Hkv, 128] bf16 or
-    float8_e4m3fn (an element of KV head h is worth e4m3 * k_scale[h], v_scale for V),
-    block_table [B, width] int32, seq_lens [B] int32 (0: the sequence's rows are zeros).
+    projection), heads contiguous, sequences one after the other.  k_cache / v_cache
+    [num_pages, P, Hkv, 128] bf16 or float8_e4m3fn (an element of KV head h is worth
+    e4m3 * k_scale[h], v_scale for V), block_table [B, width] int32, seq_lens [B] int32 (0:
+    the sequence's rows are zeros).
 
     Returns out (contiguous, q's shape; 16-byte aligned, as every tensor of 16-bit or 8-bit
     elements here) or (out, lse) with `return_lse`: fp32 [Hq, tokens] for packed q, else
-    [B, Hq, Sq]; -inf where a row sees no key.  Rows of packed tokens
-    behind the last sequence are left as they are in `out`."""
+    [B, Hq, Sq]; -inf where a row sees no key.  Scores, sums and accumulators are fp32, the
+    weights that multiply V are rounded to bf16.  Rows of packed tokens behind the last
+    sequence are left as they are in `out`."""
     what = "cross_attention"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
     num_pages, P, Hkv, D = shape
