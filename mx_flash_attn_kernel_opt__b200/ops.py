@@ -290,18 +290,28 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         cache_seqlens = cache_seqlens.to(torch.int32)
     if rotary:
         from .serving import _turn
-        what, S = "flash_attn_with_kvcache", k.shape[1]
+        what = "flash_attn_with_kvcache"
+        # everything that the decode refuses is refused before the new tokens enter the cache
+        if k_cache.dim() != 4 or k.dim() != 4:
+            raise PgqaError(2, f"{what}: the caches must be [num_pages, P, Hkv, D], k and v [B, S_new, Hkv, D]")
+        if cache_seqlens.shape != (B,) or block_table.dim() != 2 or block_table.shape[0] != B:
+            raise PgqaError(2, f"{what}: cache_seqlens must be [B], block_table [B, width]")
+        if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:
+            raise PgqaError(2, f"{what}: softmax_scale must be positive and finite")
+        S, (_, P, Hkv, _) = k.shape[1], k_cache.shape
+        ws = workspace_for(B, q.shape[2], Hkv, q.shape[3], P, q.device, seqlen_q=q.shape[1])
         # q has places of its own where it is not one token per new token, or where it has one
         # place for all of its tokens
         together = q.shape[1] == S and (causal or S == 1)
-        turned = _turn(what, q if together else None, k, v, k_cache, v_cache, block_table, cache_seqlens,
-                       rotary_cos, rotary_sin, None, None, rotary_interleaved, None, None, None, None, None)
+        turned = None
         if not together:
             places = None if causal else cache_seqlens[:, None].expand(B, q.shape[1]).contiguous()
             turned = _turn(what, q, None, None, None, None, None, cache_seqlens, rotary_cos, rotary_sin,
                            places, None, rotary_interleaved, None, None, None, None, None)
-        return decode(turned, k_cache, v_cache, block_table, cache_seqlens + S, scale=softmax_scale,
-                      causal=bool(causal), return_lse=bool(return_softmax_lse))
+        appended = _turn(what, q if together else None, k, v, k_cache, v_cache, block_table, cache_seqlens,
+                         rotary_cos, rotary_sin, None, None, rotary_interleaved, None, None, None, None, None)
+        return decode(appended if together else turned, k_cache, v_cache, block_table, cache_seqlens + S,
+                      scale=softmax_scale, workspace=ws, causal=bool(causal), return_lse=bool(return_softmax_lse))
     return decode(q, k_cache, v_cache, block_table, cache_seqlens, scale=softmax_scale,
                   causal=bool(causal), k_new=k, v_new=v, return_lse=bool(return_softmax_lse))
 

@@ -316,3 +316,36 @@ def test_pools_of_more_than_2_31_elements(kv, cuda_device):
     for a, b in zip(large, small):
         assert torch.equal(_paged.raw(a[more:]), _paged.raw(b))
         assert not a[:more].view(torch.uint8).any()
+
+
+def test_refused_rotary_calls_leave_the_cache(cuda_device):
+    """flash_attn_with_kvcache with rotary inputs: whatever it refuses, it refuses before the new
+    tokens enter the cache, as it does without them."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(110)
+    B, S, Hq, Hkv, P = 2, 3, 8, 2, 16
+    bt, pages = _paged.table([20 + S, 5 + S], P, g)
+    k, v = (_paged.pool(pages, P, Hkv, g).to(dev) for _ in range(2))
+    before = _paged.raw(k), _paged.raw(v)
+    cos, sin = (x.to(dev) for x in test_rope_gpu.tables(64, 128))
+    bt, lens = bt.to(dev), torch.tensor([20, 5], dtype=torch.int32, device=dev)
+    z = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(dev)  # noqa: E731
+    q, kn = z(B, S, Hq, 128), z(B, S, Hkv, 128)
+    for error, kw in (
+            (PgqaError, dict(k=z(B, Hkv, 128), v=z(B, Hkv, 128))),              # no dimension of tokens
+            (PgqaError, dict(k=z(B, Hkv, 128), v=z(B, Hkv, 128), causal=True)),
+            (TypeError, dict(q=z(B, 5, Hq, 128).half())), (TypeError, dict(q=z(B, S, Hq, 128).half(), causal=True)),
+            (PgqaError, dict(q=z(B, S, 7, 128))), (PgqaError, dict(q=z(B, 5, 7, 128))),
+            (PgqaError, dict(q=z(3, 5, Hq, 128))), (PgqaError, dict(softmax_scale=0.0)),
+            (PgqaError, dict(softmax_scale=float("nan"), causal=True)), (PgqaError, dict(softmax_scale=-1.0, q=z(B, 1, Hq, 128)))):
+        a = dict(q=q, k=kn, v=kn, rotary_cos=cos, rotary_sin=sin, cache_seqlens=lens, block_table=bt)
+        a.update(kw)
+        with pytest.raises(error):
+            pgqa.flash_attn_with_kvcache(a.pop("q"), k, v, **a)
+        torch.cuda.synchronize()
+        assert torch.equal(_paged.raw(k), before[0]) and torch.equal(_paged.raw(v), before[1]), kw
+    pgqa.check_device_error()
+    # and what it takes still enters
+    pgqa.flash_attn_with_kvcache(q, k, v, k=kn, v=kn, rotary_cos=cos, rotary_sin=sin, cache_seqlens=lens, block_table=bt)
+    assert not torch.equal(_paged.raw(k), before[0]) and not torch.equal(_paged.raw(v), before[1])
+    pgqa.check_device_error()
