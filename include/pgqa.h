@@ -347,7 +347,8 @@ int pgqa_accumulate_weights(const pgqa_weights_args* args, void* stream);
  *             tokens is not changed and gets 0 .. L-1 and then -1
  *   new_lens  int32 [B]: min(L, keep); shares no element with seq_lens, which the clusters
  *             of other heads and sequences still read (PGQA_ERR_BAD_SHAPE)
- * weights and weights_out are 16-byte aligned.
+ * weights and weights_out are 16-byte aligned.  The K and V pools are two
+ * (PGQA_ERR_BAD_SHAPE where they overlap): each moves its rows on its own.
  * Sequences that share pages cannot be cut (a row kept by one would be overwritten by the
  * other).  The pages from ceil(keep / P) on are the caller's to free.
  */

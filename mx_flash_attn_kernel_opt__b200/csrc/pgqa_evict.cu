@@ -567,6 +567,11 @@ int entry(const pgqa_evict_args* a, cudaStream_t stream) {
         !host_aligned(a->weights_out, 16) || !host_aligned(a->seq_lens, 4) || !host_aligned(a->block_table, 4) ||
         !host_aligned(a->kept, 4) || !host_aligned(a->new_lens, 4))
         return PGQA_ERR_MISALIGNED;
+    {  // K and V rows move independently of each other, in place
+        const uintptr_t k = reinterpret_cast<uintptr_t>(a->k_cache), v = reinterpret_cast<uintptr_t>(a->v_cache);
+        const uintptr_t bytes = (uintptr_t)a->num_pages * a->page_size * a->num_heads_k * (a->kv_format == 1 ? 128 : 256);
+        if (k < v + bytes && v < k + bytes) return PGQA_ERR_BAD_SHAPE;
+    }
     int dev, sms, optin;
     if ((st = host_device(&dev, &sms, &optin)) != PGQA_OK) return st;
     Params p = {};

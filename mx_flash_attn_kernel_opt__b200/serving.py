@@ -299,7 +299,8 @@ def evict_kv(k_cache, v_cache, weights, block_table, seq_lens, keep, *, sinks=0,
 
     The weights move along, in place or into `weights_out` (the entries of every sequence's
     first new_lens slots; the others are left as they are).  Pages from ceil(keep / P) on
-    are the caller's to free.  Sequences that share pages cannot be cut."""
+    are the caller's to free.  Sequences that share pages cannot be cut, nor one pool that
+    holds both K and V."""
     what = "evict_kv"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
     num_pages, P, Hkv, D = shape
