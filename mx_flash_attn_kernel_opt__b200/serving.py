@@ -225,7 +225,8 @@ def rope_append_kv(q, k_new, v_new, k_cache, v_cache, block_table, seq_lens, cos
                    positions=None, axes=None, interleaved=False, cu_seqlens=None, weights=None,
                    k_scale=None, v_scale=None, q_out=None):
     """Turn q and k_new by their positions and append k_new / v_new to the paged cache, in
-    one launch.  Returns the turned q (contiguous bf16, or `q_out`).
+    one launch.  Returns the turned q (contiguous bf16, or `q_out`; rows of packed tokens behind
+    the last sequence are not written).
 
     q [B, S, Hq, 128], k_new / v_new [B, S, Hkv, 128] bf16 (or [B, heads, 128] for one token
     per sequence; or packed [tokens, heads, 128] with `cu_seqlens` [B + 1] int32, ascending
@@ -339,7 +340,7 @@ def cross_attention(q, k_cache, v_cache, block_table, seq_lens, *, cu_seqlens_q=
     elements here) or (out, lse) with `return_lse`: fp32 [Hq, tokens] for packed q, else
     [B, Hq, Sq]; -inf where a row sees no key.  Scores, sums and accumulators are fp32, the
     weights that multiply V are rounded to bf16.  Rows of packed tokens behind the last
-    sequence are left as they are in `out`."""
+    sequence are left as they are in `out` (without `out`, and in lse, they hold anything)."""
     what = "cross_attention"
     dev, fp8, shape, B, width, kp, tp, lp = _cache(what, k_cache, block_table, seq_lens)
     num_pages, P, Hkv, D = shape
